@@ -19,12 +19,14 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/flashhead.h"
 #include "fh_batched.cuh"
 #include "fh_stage2_tc.cuh"
 #include "fh_spec.cuh"
+#include "fh_w4.cuh"
 
 static_assert(fh::kS2MaskWords == 8, "the selection kernel writes 8 bit-map words per cluster");
 
@@ -1615,6 +1617,185 @@ FH_API int fh_spec_accept(const int32_t *draft_ids, const int32_t *target_ids,
                          dim3(32 * warps_per_block), 0, s, false, draft_ids, target_ids,
                          bonus_ids, cu_num_draft, batch, max_spec_len, placeholder, out_ids),
                   "draft acceptance launch");
+  return FH_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// 4-bit head weight
+// ---------------------------------------------------------------------------
+static int check_w4(const fh_w4_desc *d, const void *hidden, int rows, const void *out) {
+  if (!d) return fail(FH_ERR_INVALID_ARGUMENT, "null descriptor");
+  if (rows < 0) return fail(FH_ERR_INVALID_ARGUMENT, "rows=%d < 0", rows);
+  if (d->vocab < 1 || d->vocab > 0x7FFFFF00)
+    return fail(FH_ERR_INVALID_ARGUMENT, "vocab=%d out of range", d->vocab);
+  if (d->group_size != 32 && d->group_size != 64 && d->group_size != 128)
+    return fail(FH_ERR_INVALID_ARGUMENT, "group_size=%d must be 32, 64 or 128", d->group_size);
+  if (d->hidden <= 0 || d->hidden % d->group_size != 0 || d->hidden > FH_W4_MAX_HIDDEN)
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "hidden=%d must be a positive multiple of group_size=%d, at most %d", d->hidden,
+                d->group_size, FH_W4_MAX_HIDDEN);
+  if (d->dtype != FH_BF16 && d->dtype != FH_FP16)
+    return fail(FH_ERR_INVALID_ARGUMENT, "dtype must be FH_BF16 or FH_FP16");
+  if (rows == 0) return FH_OK;
+  if (!d->qweight || !d->scales || !hidden || !out)
+    return fail(FH_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!aligned16(d->qweight) || !aligned16(d->scales) || !aligned16(d->zeros) ||
+      !aligned16(hidden))
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "qweight, scales, zeros and hidden must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(out) & 1u) != 0)
+    return fail(FH_ERR_INVALID_ARGUMENT, "out must be 2-byte aligned");
+  return FH_OK;
+}
+
+static fh::W4Args w4_args(const fh_w4_desc *d, const void *hidden, int rows, void *out) {
+  fh::W4Args a;
+  memset(&a, 0, sizeof(a));
+  a.qw = d->qweight;
+  a.scales = d->scales;
+  a.zeros = d->zeros;
+  a.V = d->vocab;
+  a.D = d->hidden;
+  a.nb = (d->hidden + fh::kW4Block - 1) / fh::kW4Block;
+  a.tiles = (d->vocab + 127) / 128 * 8;
+  a.hidden = hidden;
+  a.rows = rows;
+  a.out = out;
+  return a;
+}
+
+template <typename Kern>
+static cudaError_t raise_smem(Kern kern, int bytes, bool (&done)[128]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 128) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_attr_mutex);
+  if (!done[dev]) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    done[dev] = true;
+  }
+  return cudaSuccess;
+}
+
+constexpr int kW4SmemMax = 227 * 1024;
+
+template <typename T, int GPK, bool ZP, int NT>
+static cudaError_t launch_w4_mv_t(const fh::W4Args &a, int grid, cudaStream_t s) {
+  static bool done[128];
+  auto kern = fh::k_w4_mv<T, GPK, ZP, NT>;
+  const cudaError_t e = raise_smem(kern, kW4SmemMax, done);
+  if (e != cudaSuccess) return e;
+  return launch(kern, dim3(grid), dim3(32 * fh::kW4Warps), fh::w4_mv_smem_bytes(a.nb, NT), s,
+                false, a);
+}
+
+template <typename T, int GPK, bool ZP>
+static cudaError_t launch_w4_mv_n(const fh::W4Args &a, int nt, int grid, cudaStream_t s) {
+  return nt == 1 ? launch_w4_mv_t<T, GPK, ZP, 1>(a, grid, s)
+                 : launch_w4_mv_t<T, GPK, ZP, 2>(a, grid, s);
+}
+
+template <typename T, int GPK, bool ZP>
+static cudaError_t launch_w4_probes_t(const fh::W4Args &a, unsigned grid, cudaStream_t s) {
+  return launch(fh::k_w4_probes<T, GPK, ZP>, dim3(grid), dim3(32 * fh::kW4ProbeWarps), 0, s, false,
+                a);
+}
+
+// Calls f.template operator()<T, groups per block, zero points>() for a descriptor.
+template <typename F>
+static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
+  const int gpk = fh::kW4Block / d->group_size;
+  const bool zp = d->zeros != nullptr;
+#define FH_W4_CASE(T, G)                                                       \
+  (zp ? f(static_cast<T *>(nullptr), std::integral_constant<int, G>(), std::true_type()) \
+      : f(static_cast<T *>(nullptr), std::integral_constant<int, G>(), std::false_type()))
+  if (d->dtype == FH_BF16) {
+    if (gpk == 1) return FH_W4_CASE(__nv_bfloat16, 1);
+    if (gpk == 2) return FH_W4_CASE(__nv_bfloat16, 2);
+    return FH_W4_CASE(__nv_bfloat16, 4);
+  }
+  if (gpk == 1) return FH_W4_CASE(__half, 1);
+  if (gpk == 2) return FH_W4_CASE(__half, 2);
+  return FH_W4_CASE(__half, 4);
+#undef FH_W4_CASE
+}
+
+extern "C" {
+
+FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows) {
+  (void)desc;
+  (void)rows;
+  return 0;
+}
+
+FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows, void *out,
+                        int64_t out_stride, void *workspace, size_t workspace_bytes,
+                        fh_stream_t stream) {
+  const int st = check_w4(desc, hidden, rows, out);
+  if (st != FH_OK || rows == 0) return st;
+  (void)workspace;
+  (void)workspace_bytes;
+  if (out_stride < desc->vocab)
+    return fail(FH_ERR_INVALID_ARGUMENT, "out_stride=%lld < vocab=%d", (long long)out_stride,
+                desc->vocab);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  fh::W4Args a = w4_args(desc, hidden, rows, out);
+  a.ldo = out_stride;
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  // few units: the 16 warps of a CTA share units so that every SM has work
+  const int units = a.tiles / 2;
+  a.ksplit = 1;
+  while (a.ksplit < fh::kW4Warps && a.ksplit * 2 <= a.nb &&
+         (long long)units * a.ksplit < 2ll * sms * fh::kW4Warps)
+    a.ksplit *= 2;
+  const int teams = fh::kW4Warps / a.ksplit;
+  const int grid = std::min(sms, (units + teams - 1) / teams);
+  for (int r0 = 0; r0 < rows;) {
+    int nt = rows - r0 > 8 ? 2 : 1;
+    if (fh::w4_mv_smem_bytes(a.nb, nt) > (size_t)kW4SmemMax) nt = 1;
+    a.hidden = reinterpret_cast<const char *>(hidden) + (size_t)r0 * a.D * 2;
+    a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
+    a.rows = std::min(8 * nt, rows - r0);
+    const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto gpk, auto zp) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      return launch_w4_mv_n<T, decltype(gpk)::value, decltype(zp)::value>(a, nt, grid, s);
+    });
+    FH_CHECK_LAUNCH(e, "4-bit logits launch");
+    r0 += 8 * nt;
+  }
+  return FH_OK;
+}
+
+FH_API int fh_w4_block_sparse_logits(const fh_w4_desc *desc, const void *hs, int T,
+                                     const int64_t *ci, int P, int n_clusters, int cluster_size,
+                                     void *out, fh_stream_t stream) {
+  if (P < 0) return fail(FH_ERR_INVALID_ARGUMENT, "P=%d < 0", P);
+  const int st = check_w4(desc, hs, P == 0 ? std::min(T, 0) : T, out);
+  if (st != FH_OK || T == 0 || P == 0) return st;
+  if (!ci) return fail(FH_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (n_clusters < 1 || cluster_size < 1 ||
+      (long long)n_clusters * cluster_size > (long long)desc->vocab)
+    return fail(FH_ERR_INVALID_ARGUMENT, "n_clusters=%d * cluster_size=%d exceeds vocab=%d",
+                n_clusters, cluster_size, desc->vocab);
+  const long long n = (long long)P * cluster_size;
+  const long long ctas = (long long)T * ((n + 15) / 16);
+  if (n > 0x7FFFFF00ll || ctas > 0x7FFFFFFFll)
+    return fail(FH_ERR_INVALID_ARGUMENT, "T * P * cluster_size too large");
+  fh::W4Args a = w4_args(desc, hs, T, out);
+  a.ci = ci;
+  a.P = P;
+  a.K = n_clusters;
+  a.cap = cluster_size;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto gpk, auto zp) {
+    using Ty = std::remove_pointer_t<decltype(t)>;
+    return launch_w4_probes_t<Ty, decltype(gpk)::value, decltype(zp)::value>(a, (unsigned)ctas, s);
+  });
+  FH_CHECK_LAUNCH(e, "4-bit block-sparse logits launch");
   return FH_OK;
 }
 

@@ -64,11 +64,26 @@ class HeadDesc(ctypes.Structure):
     ]
 
 
+class W4Desc(ctypes.Structure):
+    """Mirror of ``fh_w4_desc``."""
+
+    _fields_ = [
+        ("vocab", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("qweight", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _U64 = ctypes.c_uint64
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_I64 = ctypes.c_int64
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -94,6 +109,9 @@ SIGNATURES = {
     "fh_tp_local_candidates": (_I, [_P, _P, _I, _I, _F, _U64, _U64, _P, _P, _SZ, _P]),
     "fh_tp_select_and_score": (_I, [_P, _P, _I, _I, _P, _I, _F, _U64, _U64, _P, _P, _SZ, _P]),
     "fh_tp_finalize": (_I, [_P, _I, _P, _P]),
+    "fh_w4_workspace_bytes": (_SZ, [ctypes.POINTER(W4Desc), _I]),
+    "fh_w4_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I64, _P, _SZ, _P]),
+    "fh_w4_block_sparse_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I, _I, _I, _P, _P]),
     "fh_spec_accept": (_I, [_P, _P, _P, _P, _I, _I, ctypes.c_int32, _P, _P]),
 }
 

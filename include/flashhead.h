@@ -320,6 +320,54 @@ FH_API int fh_block_sparse_argmax_atomic(const void *hs, int T, int D,
                                          fh_stream_t stream);
 
 /*
+ * Products with a head weight held in 4 bits (no counterpart in the
+ * reference): w[v, k] = (q[v, k] - z[v, g]) * s[v, g] with q in 0..15 and one
+ * scale s (and zero point z) per group g = k / group_size of a row. The group
+ * sums are exact products summed in fp32 and scaled in fp32; results are
+ * rounded once, to the hidden states' type.
+ *
+ *   vocab      V, weight rows
+ *   hidden     D, columns: a multiple of group_size, at most FH_W4_MAX_HIDDEN
+ *   group_size 32, 64 or 128
+ *   dtype      FH_BF16 or FH_FP16: type of the scales, hidden states, outputs
+ *   qweight    u32 [T][B][16][4][4], T = V / 16 rounded up to a multiple of 8
+ *              (tiles of 16 rows), B = ceil(D / 128): word j of quad c of row r
+ *              of block b holds the 8 columns 128 b + 32 j + 8 c + e, column
+ *              e = 2i in bits 4i..4i+3, e = 2i + 1 in bits 16+4i..19+4i
+ *   scales     [T][B][16][128 / group_size]; 0 in padded rows and groups
+ *   zeros      u8, the shape of scales; NULL: every zero point is 8
+ * The Python loader (flash_head/w4.py) makes this layout. Pointers 16-byte
+ * aligned, device memory.
+ */
+#define FH_W4_MAX_HIDDEN 12288
+typedef struct fh_w4_desc {
+  int32_t vocab;
+  int32_t hidden;
+  int32_t group_size;
+  int32_t dtype;
+  const uint32_t *qweight;
+  const void *scales;
+  const uint8_t *zeros;
+} fh_w4_desc;
+
+/* out[r * out_stride + v] = logit of weight row v for hidden row r: the dense
+ * head's logits (the reference's F.linear over the head weight,
+ * flash_head.py:292-301). out_stride >= V, in elements. The workspace
+ * (fh_w4_workspace_bytes; it may be 0, then NULL is fine) needs no zeroing. */
+FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows);
+FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows,
+                        void *out, int64_t out_stride, void *workspace,
+                        size_t workspace_bytes, fh_stream_t stream);
+
+/* fused.py:82-93 over a 4-bit w_perm (weight row = cluster * cluster_size +
+ * slot): ci [T, P] int64 cluster ids, out [T, P * cluster_size]. Candidates of
+ * a cluster id outside [0, n_clusters) get -inf. */
+FH_API int fh_w4_block_sparse_logits(const fh_w4_desc *desc, const void *hs,
+                                     int T, const int64_t *ci, int P,
+                                     int n_clusters, int cluster_size,
+                                     void *out, fh_stream_t stream);
+
+/*
  * Tensor-parallel steps (clusters partitioned across ranks; no reference
  * counterpart: the reference replicates the head on every rank,
  * loading.py:144-164). The caller moves the candidate words between ranks
