@@ -26,6 +26,7 @@
 #include "fh_batched.cuh"
 #include "fh_stage2_tc.cuh"
 #include "fh_spec.cuh"
+#include "fh_sample.cuh"
 #include "fh_w4.cuh"
 
 static_assert(fh::kS2MaskWords == 8, "the selection kernel writes 8 bit-map words per cluster");
@@ -1622,6 +1623,97 @@ FH_API int fh_spec_accept(const int32_t *draft_ids, const int32_t *target_ids,
 
 }  // extern "C"
 
+template <typename Kern>
+static cudaError_t raise_smem(Kern kern, int bytes, bool (&done)[128]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 128) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(g_attr_mutex);
+  if (!done[dev]) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    done[dev] = true;
+  }
+  return cudaSuccess;
+}
+
+// ---------------------------------------------------------------------------
+// Sampling from logits
+// ---------------------------------------------------------------------------
+template <typename E>
+static cudaError_t launch_sample_t(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
+  static bool done[128];
+  auto kern = fh::k_sample<E>;
+  const cudaError_t e = raise_smem(kern, (int)sizeof(fh::SmpShared), done);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)rows * (unsigned)cluster);
+  cfg.blockDim = dim3(fh::kSmpThreads);
+  cfg.dynamicSmemBytes = sizeof(fh::SmpShared);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
+                                       int64_t row_stride, const fh_sample_params *params,
+                                       int64_t *out_ids, float *out_prob, fh_stream_t stream) {
+  if (rows < 0 || rows > (1 << 27)) return fail(FH_ERR_INVALID_ARGUMENT, "rows=%d out of range", rows);
+  if (n < 0 || n > (1 << 28)) return fail(FH_ERR_INVALID_ARGUMENT, "n=%d outside 0..2^28", n);
+  if (dtype != FH_BF16 && dtype != FH_FP16 && dtype != FH_FP32)
+    return fail(FH_ERR_INVALID_ARGUMENT, "dtype must be FH_BF16, FH_FP16 or FH_FP32");
+  if (row_stride < n)
+    return fail(FH_ERR_INVALID_ARGUMENT, "row_stride=%lld < n=%d", (long long)row_stride, n);
+  if (!params) return fail(FH_ERR_INVALID_ARGUMENT, "null parameters");
+  if (params->ids && params->ids_stride != 0 && params->ids_stride < n)
+    return fail(FH_ERR_INVALID_ARGUMENT, "ids_stride=%lld is neither 0 nor >= n=%d",
+                (long long)params->ids_stride, n);
+  if (rows == 0) return FH_OK;
+  if ((n > 0 && !logits) || !params->uniforms || !out_ids)
+    return fail(FH_ERR_INVALID_ARGUMENT, "null pointer argument");
+  const size_t elem = dtype == FH_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % elem != 0)
+    return fail(FH_ERR_INVALID_ARGUMENT, "logits must be aligned to their element size");
+  fh::SampleArgs a;
+  memset(&a, 0, sizeof(a));
+  a.logits = logits;
+  a.n = n;
+  a.stride = row_stride;
+  a.temperature = params->temperature;
+  a.top_k = params->top_k;
+  a.top_p = params->top_p;
+  a.min_p = params->min_p;
+  a.temperature0 = params->temperature_all;
+  a.top_k0 = params->top_k_all;
+  a.top_p0 = params->top_p_all;
+  a.min_p0 = params->min_p_all;
+  a.uniforms = params->uniforms;
+  a.ids = params->ids;
+  a.ids_stride = params->ids_stride;
+  a.out = out_ids;
+  a.prob = out_prob;
+  // few rows: several CTAs per row, as long as each keeps 4096 entries
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  int cluster = 1;
+  while (cluster < fh::kSmpMaxCluster && (long long)rows * cluster * 2 <= sms &&
+         n / (cluster * 2) >= 4096)
+    cluster *= 2;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == FH_BF16   ? launch_sample_t<__nv_bfloat16>(a, rows, cluster, s)
+                        : dtype == FH_FP16 ? launch_sample_t<__half>(a, rows, cluster, s)
+                                           : launch_sample_t<float>(a, rows, cluster, s);
+  FH_CHECK_LAUNCH(e, "sampling launch");
+  return FH_OK;
+}
+
 // ---------------------------------------------------------------------------
 // 4-bit head weight
 // ---------------------------------------------------------------------------
@@ -1664,21 +1756,6 @@ static fh::W4Args w4_args(const fh_w4_desc *d, const void *hidden, int rows, voi
   a.rows = rows;
   a.out = out;
   return a;
-}
-
-template <typename Kern>
-static cudaError_t raise_smem(Kern kern, int bytes, bool (&done)[128]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 128) return cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> lock(g_attr_mutex);
-  if (!done[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-    done[dev] = true;
-  }
-  return cudaSuccess;
 }
 
 constexpr int kW4SmemMax = 227 * 1024;

@@ -78,6 +78,24 @@ class W4Desc(ctypes.Structure):
     ]
 
 
+class SampleParams(ctypes.Structure):
+    """Mirror of ``fh_sample_params``."""
+
+    _fields_ = [
+        ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_void_p),
+        ("top_p", ctypes.c_void_p),
+        ("min_p", ctypes.c_void_p),
+        ("uniforms", ctypes.c_void_p),
+        ("ids", ctypes.c_void_p),
+        ("ids_stride", ctypes.c_int64),
+        ("temperature_all", ctypes.c_float),
+        ("top_k_all", ctypes.c_int32),
+        ("top_p_all", ctypes.c_float),
+        ("min_p_all", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _U64 = ctypes.c_uint64
@@ -109,6 +127,7 @@ SIGNATURES = {
     "fh_tp_local_candidates": (_I, [_P, _P, _I, _I, _F, _U64, _U64, _P, _P, _SZ, _P]),
     "fh_tp_select_and_score": (_I, [_P, _P, _I, _I, _P, _I, _F, _U64, _U64, _P, _P, _SZ, _P]),
     "fh_tp_finalize": (_I, [_P, _I, _P, _P]),
+    "fh_sample_logits": (_I, [_P, _I, _I, _I, _I64, ctypes.POINTER(SampleParams), _P, _P, _P]),
     "fh_w4_workspace_bytes": (_SZ, [ctypes.POINTER(W4Desc), _I]),
     "fh_w4_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I64, _P, _SZ, _P]),
     "fh_w4_block_sparse_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I, _I, _I, _P, _P]),

@@ -320,6 +320,51 @@ FH_API int fh_block_sparse_argmax_atomic(const void *hs, int T, int D,
                                          fh_stream_t stream);
 
 /*
+ * Sampling from logits (no counterpart in the reference, whose sampling knows
+ * a temperature alone): per row temperature, min-p, top-k and top-p, then an
+ * inverse-CDF draw with a given uniform number.
+ *
+ * The entries above -inf (NaN counts as masked) of a row are ordered by
+ * falling logit, then rising column; e_i = exp((x_i - max) / T), held in 64
+ * bits. Every filter keeps a prefix of that order:
+ *   min_p  the entries with e_i >= min_p (the largest always; off at <= 0)
+ *   top_k  the first k of them (off at <= 0)
+ *   top_p  the shortest prefix that holds top_p of their mass (off at >= 1;
+ *          <= 0 keeps the first entry)
+ * and the draw is the first kept column, in column order, whose running mass
+ * exceeds u * (kept mass). A temperature <= 0 (or NaN) takes the first entry.
+ * +inf entries, if there are any, share all the mass. A row without entries
+ * gives -1 and probability 0.
+ *
+ * Every parameter is an array of one value per row or, where the pointer is
+ * NULL, the scalar for every row; NaN top_p or min_p switches that filter off.
+ *   uniforms [rows] double in [0, 1)
+ *   ids      column -> id, int32: one list per row, ids_stride elements apart
+ *            (0: one list for all rows); NULL: the column itself is returned
+ */
+typedef struct fh_sample_params {
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+  const double *uniforms;
+  const int32_t *ids;
+  int64_t ids_stride;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+} fh_sample_params;
+
+/* logits [rows, n] of dtype FH_BF16, FH_FP16 or FH_FP32, rows row_stride >= n
+ * elements apart; out_ids [rows] int64; out_prob [rows] fp32, the drawn
+ * entry's share of the kept mass (may be NULL). n is at most 2^28. */
+FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
+                            int64_t row_stride, const fh_sample_params *params,
+                            int64_t *out_ids, float *out_prob,
+                            fh_stream_t stream);
+
+/*
  * Products with a head weight held in 4 bits (no counterpart in the
  * reference): w[v, k] = (q[v, k] - z[v, g]) * s[v, g] with q in 0..15 and one
  * scale s (and zero point z) per group g = k / group_size of a row. The group
