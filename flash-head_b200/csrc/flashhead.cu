@@ -1641,17 +1641,19 @@ static cudaError_t raise_smem(Kern kern, int bytes, bool (&done)[128]) {
 // ---------------------------------------------------------------------------
 // Sampling from logits
 // ---------------------------------------------------------------------------
-template <typename E>
-static cudaError_t launch_sample_t(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
+template <typename E, bool CACHED>
+static cudaError_t launch_sample_c(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
   static bool done[128];
-  auto kern = fh::k_sample<E>;
-  const cudaError_t e = raise_smem(kern, (int)sizeof(fh::SmpShared), done);
+  auto kern = fh::k_sample<E, CACHED>;
+  const size_t smem = sizeof(fh::SmpShared) +
+                      (CACHED ? sizeof(uint4) * fh::kSmpCache * fh::kSmpThreads : 0);
+  const cudaError_t e = raise_smem(kern, (int)smem, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)rows * (unsigned)cluster);
   cfg.blockDim = dim3(fh::kSmpThreads);
-  cfg.dynamicSmemBytes = sizeof(fh::SmpShared);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1661,6 +1663,15 @@ static cudaError_t launch_sample_t(const fh::SampleArgs &a, int rows, int cluste
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <typename E>
+static cudaError_t launch_sample_t(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
+  // vectors of a row (at most one more than its length: it may start inside one)
+  const long long nv = ((long long)a.n + 2 * fh::SmpElem<E>::kVec - 2) / fh::SmpElem<E>::kVec;
+  const long long per_warp = (nv + cluster * fh::kSmpWarps - 1) / (cluster * fh::kSmpWarps);
+  return per_warp <= 32 * fh::kSmpCache ? launch_sample_c<E, true>(a, rows, cluster, s)
+                                        : launch_sample_c<E, false>(a, rows, cluster, s);
 }
 
 extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
@@ -1700,10 +1711,10 @@ extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, 
   a.ids_stride = params->ids_stride;
   a.out = out_ids;
   a.prob = out_prob;
-  // few rows: several CTAs per row, as long as each keeps 4096 entries
+  // few rows: several CTAs per row (one CTA per SM), as long as each keeps 4096 entries
   const int sms = sm_count() > 0 ? sm_count() : 148;
   int cluster = 1;
-  while (cluster < fh::kSmpMaxCluster && (long long)rows * cluster * 2 <= sms &&
+  while (cluster < fh::kSmpMaxCluster && (long long)rows * cluster * 2 <= sms + sms / 8 &&
          n / (cluster * 2) >= 4096)
     cluster *= 2;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
