@@ -38,10 +38,12 @@
 
 namespace fh {
 
-constexpr int kSmpThreads = 512;
+constexpr int kSmpThreads = 256;
+constexpr int kSmpResident = 2;  // CTAs per SM
 constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBands = 16;
 constexpr int kSmpMaxCluster = 8;
+constexpr int kSmpChunk = 2048;  // vectors of the segment of the draw looked at together
 constexpr int kSmpList = 2048;   // candidates one CTA sorts
 constexpr int kSmpMaxK = 1024;   // largest top-k that goes through the list
 constexpr int kSmpCache = 8;     // vectors of a row that a thread keeps (CACHED)
@@ -75,6 +77,10 @@ struct __align__(16) SmpShared {
       unsigned long long order[kSmpList];  // ~column << 32 | position in item
       double w[kSmpList];
     } list;
+    struct {
+      double mass[kSmpChunk];
+      int ties[kSmpChunk];
+    } vec;  // kept mass and ties of the vectors of a piece of the row
   };
   // values exchanged between the CTAs of a cluster, double-buffered so that
   // one cluster barrier per exchange is enough
@@ -82,11 +88,15 @@ struct __align__(16) SmpShared {
   unsigned long long x_cnt[2][kSmpBands];
   double sum_mass[kSmpBands];
   unsigned long long sum_cnt[kSmpBands];
-  double seg_d[kSmpMaxCluster * kSmpWarps];
-  int seg_i[kSmpMaxCluster * kSmpWarps];
+  // per warp: kept mass of its segment in units of 2^warp_k, and ties; of the
+  // first pass: largest logit, whether the mass has to be summed again
   double warp_d[kSmpWarps];
+  double warp_k[kSmpWarps];
   int warp_i[kSmpWarps];
   float warp_f[kSmpWarps];
+  int warp_bad[kSmpWarps];
+  double seg_before;
+  long long seg_left;
   double scan_d[kSmpWarps];
   int scan_i[33];
   int count;  // list entries
@@ -97,6 +107,12 @@ struct __align__(16) SmpShared {
 
 // Order of the logits: monotone in x, with -0 equal to +0.
 __device__ __forceinline__ uint32_t smp_key(float x) { return mono(x + 0.0f); }
+
+// A key as a threshold that logits are compared with. No logit has the key of
+// -0, but +0 > -0 does not hold: the next lower number stands for it.
+__device__ __forceinline__ float smp_float(uint32_t key) {
+  return unmono(key == 0x7FFFFFFFu ? 0x7FFFFFFEu : key);
+}
 
 template <typename E>
 struct SmpElem;
@@ -147,6 +163,9 @@ struct SmpRow {
   __device__ __forceinline__ uint4 raw(int v) const {
     const int c0 = column(v);
     if (c0 >= 0 && c0 + kVec <= n) return __ldg(reinterpret_cast<const uint4 *>(p + c0));
+    return edge(p, c0, n);
+  }
+  __device__ __noinline__ static uint4 edge(const E *p, int c0, int n) {
     union {
       uint4 u;
       E e[kVec];
@@ -156,52 +175,59 @@ struct SmpRow {
       x.e[i] = c0 + i >= 0 && c0 + i < n ? p[c0 + i] : SmpElem<E>::none();
     return x.u;
   }
-  // NaN is masked like -inf
+  // NaN stays: it fails every comparison (and key range) below, as -inf does
   __device__ __forceinline__ static void unpack(const uint4 &u, float *f) {
     SmpElem<E>::unpack(u, f);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = f[i] == f[i] ? f[i] : -INFINITY;
   }
 };
 
-// 2^t for -100 < t <= 0 (a relative error below 2e-14): t = n + f with n the
-// nearest integer, 2^f by a polynomial of degree 9 through the Chebyshev nodes
-// of [-1/2, 1/2], n added to the exponent.
-__device__ __forceinline__ double smp_exp2(double t) {
-  const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is n
-  const double r = t + magic;
-  const int n = __double2loint(r);
-  const double f = t - (r - magic);
-  double p = 1.02059053204931027e-07;
-  p = fma(p, f, 1.32596452439290570e-06);
-  p = fma(p, f, 1.52526729253468732e-05);
-  p = fma(p, f, 1.54034337512549968e-04);
-  p = fma(p, f, 1.33335582007937186e-03);
-  p = fma(p, f, 9.61812919393430395e-03);
-  p = fma(p, f, 5.55041086646516774e-02);
-  p = fma(p, f, 2.40226506956403407e-01);
-  p = fma(p, f, 6.93147180559946174e-01);
-  p = fma(p, f, 1.00000000000001354e+00);
-  return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
-}
+// Polynomial of 2^f through the Chebyshev nodes of [-1/2, 1/2], relative error
+// below 2e-14; in constant memory, so that a fused multiply-add takes its
+// coefficient as an operand.
+__constant__ double kSmpExp2[10] = {
+    1.00000000000001354e+00, 6.93147180559946174e-01, 2.40226506956403407e-01,
+    5.55041086646516774e-02, 9.61812919393430395e-03, 1.33335582007937186e-03,
+    1.54034337512549968e-04, 1.52526729253468732e-05, 1.32596452439290570e-06,
+    1.02059053204931027e-07};
 
-// Mass of a logit relative to the row's largest, 2^((x - m) c). `depth` is
-// (m - x) c in fp32: a monotone measure of how far down a logit is, which also
-// drops masses below 2^-72, less than the rounding of their sum.
+// Mass of a logit in units of 2^k0: 2^(x c - k0) with c = log2(e) / T and k0
+// the integer next to ref * c, so that x c - k0 is rounded once (fma) however
+// large the two are. With 1.5 * 2^52 added, the sum's low word is its nearest
+// integer n; the rest f is within 1/2, 2^f a polynomial, and n is added to the
+// exponent. Masses below 2^-72 of the reference's are dropped: less than the
+// rounding of their sum. `depth` is the same exponent, falling and in fp32: a
+// monotone measure of how far down a logit lies.
+// For |ref| c above 2^40 neighbouring fp32 logits differ by a factor of 2^(2^16):
+// c is held there, where only the reference's equals keep a mass (`held`).
 struct SmpMass {
-  double md, c;
-  float m, cf;
-  __device__ __forceinline__ SmpMass(float m_, float T)
-      : md((double)m_), c(1.4426950408889634 / (double)T), m(m_),
-        cf(fminf((float)(2.0 * c), 3.402823466e38f)) {}
-  // halved first: m - x may pass the largest fp32
-  __device__ __forceinline__ float depth(float x) const { return fmaf(-0.5f, x, 0.5f * m) * cf; }
-  __device__ __forceinline__ double at_depth(float x, float d) const {
-    return d < 72.f ? smp_exp2(((double)x - md) * c) : 0.0;
+  double c, k0, k1;
+  float ref, xlo, cf;
+  bool held;
+  __device__ __forceinline__ SmpMass(float ref_, float T) : ref(ref_) {
+    const double c0 = 1.4426950408889634 / (double)T, most = 1099511627776.0;
+    held = fabs((double)ref) * c0 > most;
+    c = held ? most / fabs((double)ref) : c0;
+    k0 = rint((double)ref * c);
+    k1 = 6755399441055744.0 - k0;
+    xlo = fminf((float)((double)ref - 72.0 / c), nextafterf(ref, -INFINITY));
+    cf = fminf((float)(2.0 * c), 3.402823466e38f);
   }
-  __device__ __forceinline__ double operator()(float x) const {
-    return at_depth(x, depth(x));
+  // halved first: ref - x may pass the largest fp32. Rounded here, so that it
+  // is the same number wherever it is used.
+  __device__ __forceinline__ float depth(float x) const {
+    return __fmul_rn(fmaf(-0.5f, x, 0.5f * ref), cf);
   }
+  // for x > xlo (and up to 2^900 above the reference)
+  __device__ __forceinline__ double raw(float x) const {
+    const double xd = (double)x;
+    const double r = fma(xd, c, k1);
+    const double f = fma(xd, c, k1 - r);
+    double p = kSmpExp2[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) p = fma(p, f, kSmpExp2[i]);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));
+  }
+  __device__ __forceinline__ double operator()(float x) const { return x > xlo ? raw(x) : 0.0; }
 };
 
 // A prefix of the order: keys above `key`, and the first `ties` equal ones.
@@ -291,8 +317,10 @@ __device__ __forceinline__ void smp_exchange(Ctx &C, int n) {
   __syncthreads();
 }
 
-// Exclusive prefix sum of one double per thread, in a fixed order.
-__device__ __forceinline__ double smp_scan(SmpShared &S, double v, double *total) {
+// Exclusive prefix sum of one double per thread, in a fixed order. (Out of
+// line, like the other helpers of the short paths: a launch of few rows waits
+// for instructions more than for anything else.)
+__device__ __noinline__ double smp_scan(SmpShared &S, double v, double *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double x = v;
 #pragma unroll
@@ -313,25 +341,31 @@ __device__ __forceinline__ double smp_scan(SmpShared &S, double v, double *total
   return before + (x - v);
 }
 
-// Sums the threads' bands: warp b band b, lane by lane, then over the cluster.
+__device__ __noinline__ int smp_count_scan(SmpShared &S, int v, int *total) {
+  return block_exclusive_scan(v, S.scan_i, total);
+}
+
+// Sums the threads' bands: one warp a band, lane by lane, then over the cluster.
 template <bool MASS, bool CNT, typename Ctx>
 __device__ __forceinline__ void smp_band_sums(Ctx &C) {
   SmpShared &S = C.S;
   __syncthreads();
-  double d = 0.0;
-  unsigned long long k = 0ull;
-  for (int i = C.lane; i < kSmpThreads; i += 32) {
-    if (MASS) d += S.band.mass[C.warp][i];
-    if (CNT) k += S.band.cnt[C.warp][i];
-  }
+  for (int b = C.warp; b < kSmpBands; b += kSmpWarps) {
+    double d = 0.0;
+    unsigned long long k = 0ull;
+    for (int i = C.lane; i < kSmpThreads; i += 32) {
+      if (MASS) d += S.band.mass[b][i];
+      if (CNT) k += S.band.cnt[b][i];
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (MASS) d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
-    if (CNT) k += __shfl_xor_sync(0xFFFFFFFFu, k, o);
-  }
-  if (C.lane == 0) {
-    S.x_mass[C.phase & 1][C.warp] = d;
-    S.x_cnt[C.phase & 1][C.warp] = k;
+    for (int o = 16; o > 0; o >>= 1) {
+      if (MASS) d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
+      if (CNT) k += __shfl_xor_sync(0xFFFFFFFFu, k, o);
+    }
+    if (C.lane == 0) {
+      S.x_mass[C.phase & 1][b] = d;
+      S.x_cnt[C.phase & 1][b] = k;
+    }
   }
   smp_exchange(C, kSmpBands);
 }
@@ -456,14 +490,14 @@ __device__ __forceinline__ void smp_top_p(Ctx &C, const SmpMass &w, const SmpCut
   }
 }
 
-// Smallest key whose mass is at least min_p (at most the largest entry's).
-__device__ __forceinline__ uint32_t smp_min_key(const SmpMass &w, float m, float min_p) {
+// Smallest key whose mass is at least min_p times the largest entry's.
+__device__ __noinline__ uint32_t smp_min_key(float m, float T, float min_p) {
   const uint32_t top = smp_key(m);
-  const double t = log2((double)min_p);
-  auto enough = [&](uint32_t k) { return ((double)unmono(k) - w.md) * w.c >= t; };
+  const double t = log2((double)min_p), c = 1.4426950408889634 / (double)T;
+  auto enough = [&](uint32_t k) { return ((double)unmono(k) - (double)m) * c >= t; };
   // bisect the keys; the border's rounded value is nearly always within a step
   uint32_t lo = smp_key(-INFINITY), hi = top;  // lo: too little, hi: enough
-  const uint32_t g = smp_key((float)fmin((double)m, w.md + t / w.c));
+  const uint32_t g = smp_key((float)fmin((double)m, (double)m + t / c));
   if (g > lo + 2u && !enough(g - 2u)) lo = g - 2u;
   if (g + 2u < hi && enough(g + 2u)) hi = g + 2u;
   while (hi - lo > 1u) {
@@ -476,37 +510,40 @@ __device__ __forceinline__ uint32_t smp_min_key(const SmpMass &w, float m, float
   return hi;
 }
 
-// The three nested band levels of a top-p descent, in units of depth (a
-// factor 2 of mass): 2, 1/8 and 1/128 wide, the last of a level open-ended.
-// Each is a monotone step function of the logit, so that a band is a run of
-// the order whatever the rounding.
-struct SmpBand {
-  int level;      // levels already chosen
-  int j0, j1, j2; // the chosen bands
-  __device__ __forceinline__ static int clamp(float x) {
-    return (int)fmaxf(0.f, fminf(x, (float)(kSmpBands - 1)));
+// Bands of a top-p descent: a run of the order, logits in (lo, hi], split in
+// 16 by depth; the last band also takes what lies deeper. Any rounding of the
+// depth keeps the bands runs of the order, since it is monotone.
+struct SmpBands {
+  float lo, hi;        // logits
+  float from, scale;   // depth of the first band, bands per unit of depth
+  __device__ __forceinline__ int band(float d) const {
+    return (int)fmaxf(0.f, fminf(__fmul_rn(d - from, scale), (float)(kSmpBands - 1)));
   }
-  __device__ __forceinline__ static int band0(float d) { return clamp(d * 0.5f); }
-  __device__ __forceinline__ int band1(float d) const { return clamp((d - 2.f * j0) * 8.f); }
-  __device__ __forceinline__ int band2(float d) const {
-    return clamp((d - 2.f * j0 - 0.125f * j1) * 128.f);
-  }
-  // -1: before the chosen band, +1: behind it, 0: in it
-  __device__ __forceinline__ int side(float d) const {
-    int s = band0(d) - j0;
-    if (s == 0 && level > 1) s = band1(d) - j1;
-    if (s == 0 && level > 2) s = band2(d) - j2;
-    return s;
-  }
-  __device__ __forceinline__ int next(float d) const {
-    return level == 0 ? band0(d) : level == 1 ? band1(d) : band2(d);
-  }
+  __device__ __forceinline__ float begin(int j) const { return from + (float)j / scale; }
 };
 
-// Entries with in(x) into this CTA's list; returns the cluster's total, and
+// Largest logit in (b.lo, b.hi] that lies in band j or behind (b.lo if none):
+// each round of 32 probes by a warp's lanes narrows its key 32-fold.
+__device__ __noinline__ float smp_band_top(const SmpMass &w, const SmpBands &b, int j) {
+  const int lane = threadIdx.x & 31;
+  uint32_t lo = smp_key(b.lo), hi = smp_key(b.hi);  // lo holds, keys above hi do not
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 31u) / 32u;
+    const uint32_t k = (hi - lo) / step > (uint32_t)lane ? lo + step * (uint32_t)(lane + 1) : hi;
+    const unsigned in = __ballot_sync(0xFFFFFFFFu, b.band(w.depth(unmono(k))) >= j);
+    const int n = in == 0xFFFFFFFFu ? 32 : __ffs(~in) - 1;  // probes that hold
+    const uint32_t l = n ? __shfl_sync(0xFFFFFFFFu, k, n - 1) : lo;
+    const uint32_t h = n < 32 ? __shfl_sync(0xFFFFFFFFu, k, n) - 1u : l;
+    lo = l;
+    hi = max(l, h);
+  }
+  return unmono(lo);
+}
+
+// Entries in (lo, hi] into this CTA's list; returns the cluster's total, and
 // gathers the lists in rank 0's when they fit. Contains cluster barriers.
-template <typename Ctx, typename In>
-__device__ __forceinline__ int smp_collect(Ctx &C, In in) {
+template <typename Ctx>
+__device__ __forceinline__ int smp_collect(Ctx &C, float lo, float hi) {
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   SmpShared &S = C.S;
@@ -517,17 +554,14 @@ __device__ __forceinline__ int smp_collect(Ctx &C, In in) {
     constexpr int kVec = decltype(C.row)::kVec;
     uint32_t hit = 0u;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) hit |= in(f[i]) ? 1u << i : 0u;
+    for (int i = 0; i < kVec; ++i) hit |= f[i] > lo && f[i] <= hi ? 1u << i : 0u;
     if (hit) {
       int at = atomicAdd(&S.count, __popc(hit));
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        if ((hit >> i) & 1u) {
-          if (at < kSmpList)
-            S.list.item[at] = ((unsigned long long)smp_key(f[i]) << 32) |
+        if (((hit >> i) & 1u) && at < kSmpList)
+          S.list.item[at++] = ((unsigned long long)smp_key(f[i]) << 32) |
                               (0xFFFFFFFFu - (uint32_t)(C.row.column(v) + i));
-          ++at;
-        }
     }
   });
   __syncthreads();
@@ -551,21 +585,67 @@ __device__ __forceinline__ int smp_collect(Ctx &C, In in) {
   return (int)total;
 }
 
-// Descending bitonic sort of n2 (a power of two) words by the whole CTA.
-__device__ __forceinline__ void smp_sort(unsigned long long *a, int n2) {
-  for (int size = 2; size <= n2; size <<= 1) {
+// Descending bitonic sort of n2 (a power of two, at most kSmpList) words by
+// the whole CTA: thread t holds words kPer * t .. in registers, so that short
+// strides stay in a thread, those below 32 * kPer in a warp (shuffles), and
+// only the few longer ones go through shared memory.
+constexpr int kSmpPer = kSmpList / kSmpThreads;
+__device__ __noinline__ void smp_sort(unsigned long long *a, int n2) {
+  const int tid = threadIdx.x, base = tid * kSmpPer;
+  unsigned long long x[kSmpPer];
+  __syncthreads();
+  const bool mine = base < n2;
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i) x[i] = base + i < n2 ? a[base + i] : 0ull;
+  const int n = max(n2, kSmpPer);
+  for (int size = 2; size <= n; size <<= 1) {
     for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n2 / 2; t += kSmpThreads) {
-        const int i = 2 * t - (t & (step - 1)), j = i + step;
-        const unsigned long long x = a[i], y = a[j];
-        if ((x < y) == ((i & size) == 0)) {
-          a[i] = y;
-          a[j] = x;
+      if (step >= 32 * kSmpPer) {
+        __syncthreads();
+        if (mine)
+#pragma unroll
+          for (int i = 0; i < kSmpPer; ++i) a[base + i] = x[i];
+        __syncthreads();
+        if (mine)
+#pragma unroll
+          for (int i = 0; i < kSmpPer; ++i) {
+            const int at = base + i;
+            const unsigned long long y = a[at ^ step];
+            // the lower index keeps the larger word in a falling run
+            const bool big = ((at & step) == 0) == ((at & size) == 0);
+            x[i] = (x[i] > y) == big ? x[i] : y;
+          }
+      } else if (step >= kSmpPer) {
+        if (base - (tid & 31) * kSmpPer < n2) {  // the whole warp or none of it
+#pragma unroll
+          for (int i = 0; i < kSmpPer; ++i) {
+            const int at = base + i;
+            const unsigned long long y = __shfl_xor_sync(0xFFFFFFFFu, x[i], step / kSmpPer);
+            const bool big = ((at & step) == 0) == ((at & size) == 0);
+            x[i] = (x[i] > y) == big ? x[i] : y;
+          }
+        }
+      } else if (mine) {
+#pragma unroll
+        for (int s = kSmpPer / 2; s > 0; s >>= 1) {
+          if (s != step) continue;
+#pragma unroll
+          for (int i = 0; i < kSmpPer; ++i) {
+            if (i & s) continue;
+            const bool fall = ((base + i) & size) == 0;
+            const unsigned long long u = x[i], v = x[i | s];
+            const bool swap = (u < v) == fall;
+            x[i] = swap ? v : u;
+            x[i | s] = swap ? u : v;
+          }
         }
       }
     }
   }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i)
+    if (base + i < n2) a[base + i] = x[i];
   __syncthreads();
 }
 
@@ -573,7 +653,6 @@ __device__ __forceinline__ int smp_pow2(int n) { return n <= 2 ? 2 : 1 << (32 - 
 
 // Sorts the list and leaves its masses in list.w. Returns this thread's
 // exclusive prefix of the masses of items kPer * tid .. + kPer - 1.
-constexpr int kSmpPer = kSmpList / kSmpThreads;
 template <typename Ctx>
 __device__ __forceinline__ double smp_sort_list(Ctx &C, const SmpMass &w, int n, double *wt,
                                                 double *total) {
@@ -641,7 +720,44 @@ __device__ __forceinline__ void smp_draw_list(Ctx &C, const SampleArgs &a, int r
   }
 }
 
-// The draw from the prefix `cut` of the whole row.
+// Kept mass and ties of this warp's segment, for the prefix `cut`; returns
+// its largest logit.
+template <bool TIES, typename Ctx>
+__device__ __forceinline__ float smp_segment(Ctx &C, const SmpMass &w, const SmpCut &cut) {
+  constexpr int kVec = decltype(C.row)::kVec;
+  const float xc = smp_float(cut.key), above = fmaxf(xc, w.xlo);
+  double sum0 = 0.0, sum1 = 0.0;
+  int ties = 0;
+  float top = -INFINITY;
+  C.each([&](int, const float *f) {
+    double x[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x[i] = w.raw(f[i]);
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2) {
+      if (f[i] > above) sum0 += x[i];
+      if (f[i + 1] > above) sum1 += x[i + 1];
+      top = fmaxf(top, fmaxf(f[i], f[i + 1]));
+      if (TIES) ties += (f[i] == xc) + (f[i + 1] == xc);
+    }
+  });
+  double sum = sum0 + sum1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (TIES) ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
+  }
+  if (C.lane == 0) {
+    C.S.warp_d[C.warp] = sum;
+    C.S.warp_k[C.warp] = w.k0;
+    C.S.warp_i[C.warp] = ties;
+  }
+  return top;
+}
+
+// The draw from the prefix `cut` of the whole row: the segments' masses are in
+// warp_* of every CTA, in units of 2^warp_k; w gives masses in units of 2^w.k0.
 template <typename E, typename Ctx>
 __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const SmpMass &w,
                                              const SmpCut &cut, double tie_w, int r, double u) {
@@ -649,44 +765,29 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   cg::cluster_group cl = cg::this_cluster();
   constexpr int kVec = SmpRow<E>::kVec;
   SmpShared &S = C.S;
-  const int tid = C.tid, warp = C.warp, lane = C.lane, size = C.size;
-  const float xc = unmono(cut.key);
-  double sum = 0.0;
-  int ties = 0;
-  C.each([&](int, const float *f) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      if (f[i] > xc) sum += w(f[i]);
-      ties += f[i] == xc;
-    }
-  });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
-  }
-  if (lane == 0) {
-    S.warp_d[warp] = sum;
-    S.warp_i[warp] = ties;
-  }
+  const int tid = C.tid;
+  const float xc = smp_float(cut.key), above = fmaxf(xc, w.xlo);
   if (tid == 0) {
     S.best = 0x7FFFFFFF;
     S.last = -1;
   }
-  cl.sync();
   // every CTA finds the segment of the draw: thread i has segment i
-  const int segs = size * kSmpWarps;
+  const int segs = C.size * kSmpWarps;
   double mass = 0.0;
   int seg_ties = 0;
   if (tid < segs) {
     const SmpShared *R = cl.map_shared_rank(&S, tid / kSmpWarps);
     mass = R->warp_d[tid % kSmpWarps];
     seg_ties = R->warp_i[tid % kSmpWarps];
+    const double shift = R->warp_k[tid % kSmpWarps] - w.k0;
+    if (shift != 0.0) mass = ldexp(mass, (int)fmax(-2000.0, fmin(shift, 2000.0)));
   }
-  int all_ties;
-  const int ties_before = block_exclusive_scan(seg_ties, S.scan_i, &all_ties);
-  const long long left = cut.ties - ties_before;
-  if (left > 0) mass += (double)min(left, (long long)seg_ties) * tie_w;
+  long long left = cut.ties;
+  if (cut.ties > 0) {
+    int all_ties;
+    left -= smp_count_scan(S, seg_ties, &all_ties);
+    if (left > 0) mass += (double)min(left, (long long)seg_ties) * tie_w;
+  }
   double total;
   const double before = smp_scan(S, mass, &total);
   const double target = u * total;
@@ -697,83 +798,172 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   __syncthreads();
   const int seg = S.best != 0x7FFFFFFF ? S.best : S.last;
   if (tid == seg) {
-    S.seg_d[0] = before;
-    S.cut_ties = left;
+    S.seg_before = before;
+    S.seg_left = left;
   }
   __syncthreads();
-  const double seg_before = S.seg_d[0];
-  const long long seg_left = S.cut_ties;
-  if (tid == 0) {
-    S.best = 0x7FFFFFFF;
-    S.last = -1;
-  }
-  __syncthreads();
-  if (seg / kSmpWarps == C.rank) {
-    const int sv0 = (int)((long long)C.row.nv * seg / segs);
-    const int sv1 = (int)((long long)C.row.nv * (seg + 1) / segs);
-    const int per = (sv1 - sv0 + kSmpThreads - 1) / kSmpThreads;
-    const int a0 = min(sv1, sv0 + tid * per), a1 = min(sv1, a0 + per);
-    int t = 0;
-    if (cut.ties > 0) {
-      for (int v = a0; v < a1; ++v) {
-        float f[kVec];
-        C.row.unpack(C.row.raw(v), f);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) t += f[i] == xc;
-      }
-    }
-    int t_total;
-    const int t_before = block_exclusive_scan(t, S.scan_i, &t_total);
-    double d = 0.0;
-    long long lft = seg_left - t_before;
-    for (int v = a0; v < a1; ++v) {
-      float f[kVec];
-      C.row.unpack(C.row.raw(v), f);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        if (f[i] > xc)
-          d += w(f[i]);
-        else if (f[i] == xc && lft-- > 0)
-          d += tie_w;
-      }
-    }
-    double seg_total;
-    double run = seg_before + smp_scan(S, d, &seg_total);
-    lft = seg_left - t_before;
-    int best = 0x7FFFFFFF, last = -1;
-    for (int v = a0; v < a1; ++v) {
-      float f[kVec];
-      C.row.unpack(C.row.raw(v), f);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        double x = 0.0;
-        if (f[i] > xc)
-          x = w(f[i]);
-        else if (f[i] == xc && lft-- > 0)
-          x = tie_w;
-        run += x;
-        if (x > 0.0) {
-          last = C.row.column(v) + i;
-          if (run > target) best = min(best, last);
-        }
-      }
-    }
-    if (best != 0x7FFFFFFF) atomicMin(&S.best, best);
-    if (last >= 0) atomicMax(&S.last, last);
+  if (seg / kSmpWarps != C.rank) return;
+  // the segment in pieces of kSmpChunk vectors: their masses, then the vector
+  // of the draw, then its entry
+  const int sv0 = (int)((long long)C.row.nv * seg / segs);
+  const int sv1 = (int)((long long)C.row.nv * (seg + 1) / segs);
+  constexpr int kEach = kSmpChunk / kSmpThreads;
+  double run = S.seg_before;
+  left = S.seg_left;
+  for (int c0 = sv0; c0 < sv1; c0 += kSmpChunk) {
+    const int cn = min(kSmpChunk, sv1 - c0);
     __syncthreads();
     if (tid == 0) {
-      // past the end by rounding: the last kept column
-      const int col = S.best != 0x7FFFFFFF ? S.best : S.last;
-      const float x = SmpElem<E>::to_float(C.row.p[col]);
-      smp_emit<E>(a, r, col, (x > xc ? w(x) : tie_w) / total);
+      S.best = 0x7FFFFFFF;
+      S.last = -1;
     }
+    for (int i = tid; i < cn; i += kSmpThreads) {
+      float f[kVec];
+      double x[kVec], sum = 0.0;
+      int t = 0;
+      C.row.unpack(C.row.raw(c0 + i), f);
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) x[q] = w.raw(f[q]);
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) {
+        if (f[q] > above) sum += x[q];
+        t += f[q] == xc;
+      }
+      S.vec.mass[i] = sum;
+      S.vec.ties[i] = t;
+    }
+    __syncthreads();
+    double m[kEach], sum = 0.0;
+    long long l[kEach];  // ties still to be kept at the vector
+    if (cut.ties > 0) {
+      int t = 0, all;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) t += tid * kEach + i < cn ? S.vec.ties[tid * kEach + i] : 0;
+      long long lft = left - smp_count_scan(S, t, &all);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        l[i] = lft;
+        lft -= tid * kEach + i < cn ? S.vec.ties[tid * kEach + i] : 0;
+      }
+      left -= all;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = tid * kEach + i;
+      m[i] = at < cn ? S.vec.mass[at] : 0.0;
+      if (cut.ties > 0 && at < cn && l[i] > 0)
+        m[i] += (double)min(l[i], (long long)S.vec.ties[at]) * tie_w;
+      sum += m[i];
+    }
+    double piece;
+    const double base = run + smp_scan(S, sum, &piece);
+    double before_v = base;
+    int hit = 0x7FFFFFFF, last = -1;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (m[i] > 0.0) {
+        last = tid * kEach + i;
+        if (hit == 0x7FFFFFFF && before_v + m[i] > target) hit = last;
+      }
+      before_v += m[i];
+    }
+    if (hit != 0x7FFFFFFF) atomicMin(&S.best, hit);
+    if (last >= 0) atomicMax(&S.last, last);
+    __syncthreads();
+    // past the end by rounding: the last vector with a mass
+    const int at = S.best != 0x7FFFFFFF ? S.best : c0 + kSmpChunk >= sv1 ? S.last : -1;
+    if (at >= 0) {
+      if (at / kEach == tid) {
+        // the vector's entries: the first beyond the target, or the last kept
+        double to = base;
+        long long lft = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (tid * kEach + i < at) to += m[i];
+          if (cut.ties > 0 && tid * kEach + i == at) lft = l[i];
+        }
+        float f[kVec];
+        C.row.unpack(C.row.raw(c0 + at), f);
+        int col = -1;
+        double x = 0.0;
+        bool found = false;
+#pragma unroll
+        for (int q = 0; q < kVec; ++q) {
+          double e = 0.0;
+          if (f[q] > above)
+            e = w.raw(f[q]);
+          else if (cut.ties > 0 && f[q] == xc && lft-- > 0)
+            e = tie_w;
+          to += e;
+          if (e > 0.0 && !found) {
+            col = C.row.column(c0 + at) + q;
+            x = e;
+            found = to > target;
+          }
+        }
+        smp_emit<E>(a, r, col, x / total);
+      }
+      return;
+    }
+    run += piece;
   }
+}
+
+// The list's entries (sorted, rank 0) up to the target mass; `run` is this
+// thread's exclusive prefix.
+__device__ __noinline__ int smp_reach(SmpShared &S, const double *wt, double run, double target,
+                                         int n) {
+  int in = 0, all;
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i) {
+    in += (int)threadIdx.x * kSmpPer + i < n && run < target;
+    run += wt[i];
+  }
+  (void)smp_count_scan(S, in, &all);
+  return max(1, all);
+}
+
+// Masses of the 16 bands of the logits in (b.lo, b.hi], per thread. FIRST: the
+// row is read for the first time and has no upper end; returns the warp's
+// largest logit.
+constexpr float kSmpBand0 = 1.5f;  // depth of a first band: 15 hold all but 2^-22
+template <bool FIRST, typename Ctx>
+__device__ __forceinline__ float smp_bands(Ctx &C, const SmpMass &w, const SmpBands &b) {
+  constexpr int kVec = decltype(C.row)::kVec;
+  SmpShared &S = C.S;
+#pragma unroll
+  for (int i = 0; i < kSmpBands; ++i) S.band.mass[i][C.tid] = 0.0;
+  const float least = fmaxf(b.lo, w.xlo), hi = b.hi;
+  double *mine = &S.band.mass[0][C.tid];
+  float top = -INFINITY;
+  if (FIRST) {
+    C.first([&](int, const float *f) {
+      double x[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) x[i] = w.raw(f[i]);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        top = fmaxf(top, f[i]);
+        const int j = b.band(w.depth(f[i]));
+        if (f[i] > least) mine[j * kSmpThreads] += x[i];
+      }
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  } else {
+    C.each([&](int, const float *f) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (f[i] > least && f[i] <= hi) mine[b.band(w.depth(f[i])) * kSmpThreads] += w.raw(f[i]);
+    });
+  }
+  return top;
 }
 
 // CACHED: every lane's share of the row is at most kSmpCache vectors, kept in
 // shared memory.
 template <typename E, bool CACHED>
-__global__ void __launch_bounds__(kSmpThreads, CACHED ? 1 : 2) k_sample(SampleArgs a) {
+__global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) unsigned char smp_raw[];
   SmpShared &S = *reinterpret_cast<SmpShared *>(smp_raw);
@@ -796,27 +986,80 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? 1 : 2) k_sample(SampleAr
   const float mp = a.min_p ? a.min_p[r] : a.min_p0;
   double u = a.uniforms[r];
   u = u > 0.0 ? u : 0.0;
-  const bool greedy = !(T > 0.f);
-  if (greedy) T = 1.f;
-
-  // the thread's and the row's largest logit
-  float mt = -INFINITY;
-  C.first([&](int, const float *f) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) mt = fmaxf(mt, f[i]);
-  });
-  float m = mt;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  if (lane == 0) S.warp_f[warp] = m;
-  cl.sync();
-  m = -INFINITY;
-  for (int i = lane; i < size * kSmpWarps; i += 32)
-    m = fmaxf(m, cl.map_shared_rank(&S, i / kSmpWarps)->warp_f[i % kSmpWarps]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-
+  const bool one = !(T > 0.f) || k == 1 || p <= 0.f;  // the first entry
+  if (!(T > 0.f)) T = 1.f;
+  const bool use_k = !one && k > 0 && k < a.n, use_p = !one && p < 1.f, use_m = !one && mp > 0.f;
+  const bool all = !one && !use_k && !use_p && !use_m;  // no filter
+  const bool nucleus = use_p && !use_k && !use_m;       // top-p alone
   const uint32_t key_none = smp_key(-INFINITY);
+  SmpCut cut{key_none, 0};
+
+  // The first pass: the row's largest logit. Without a filter it sums the
+  // masses as well, with a top-p alone those of its bands, in units that the
+  // row's first entries give.
+  float mt = -INFINITY, m;
+  int first = 0x7FFFFFFF;
+  SmpMass w(0.f, T);
+  int bad = 1;
+  if (all || nucleus) {
+    // without a filter a warp's units are its own; bands need the row's
+    float ref = -INFINITY, f[kVec];
+    const int v = all ? C.v0 + lane : (int)((long long)C.row.nv * tid / kSmpThreads);
+    if (v < (all ? C.v1 : C.row.nv)) {
+      C.row.unpack(C.row.raw(v), f);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) ref = fmaxf(ref, f[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xFFFFFFFFu, ref, o));
+    if (nucleus) {
+      if (lane == 0) S.warp_f[warp] = ref;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kSmpWarps; ++i) ref = fmaxf(ref, S.warp_f[i]);
+      __syncthreads();
+    }
+    if (!(fabsf(ref) < INFINITY)) ref = 0.f;
+    w = SmpMass(ref, T);
+    if (all) {
+      if constexpr (CACHED) C.first([](int, const float *) {});
+      m = smp_segment<false>(C, w, cut);
+    } else {
+      m = smp_bands<true>(C, w, SmpBands{-INFINITY, INFINITY, 0.f, 1.f / kSmpBand0});
+    }
+    bad = w.held || w.depth(m) < -900.f;
+  } else {
+    C.first([&](int v, const float *f) {
+      float x = f[0];
+#pragma unroll
+      for (int i = 1; i < kVec; ++i) x = fmaxf(x, f[i]);
+      if (x > mt) {
+        mt = x;
+        first = v;
+      }
+    });
+    m = mt;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  }
+  if (lane == 0) {
+    S.warp_f[warp] = m;
+    S.warp_bad[warp] = bad;
+  }
+  if (nucleus)
+    smp_band_sums<true, false>(C);
+  else
+    cl.sync();
+  bad = 0;
+  m = -INFINITY;
+  for (int i = lane; i < size * kSmpWarps; i += 32) {
+    const SmpShared *R = cl.map_shared_rank(&S, i / kSmpWarps);
+    m = fmaxf(m, R->warp_f[i % kSmpWarps]);
+    bad |= R->warp_bad[i % kSmpWarps];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  bad = __any_sync(0xFFFFFFFFu, bad);
   if (m == -INFINITY) {  // nothing left in this row
     if (rank == 0 && tid == 0) {
       a.out[r] = -1;
@@ -825,201 +1068,222 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? 1 : 2) k_sample(SampleAr
     cl.sync();
     return;
   }
-  const SmpMass w(m, T);
   const uint32_t key_max = smp_key(m);
-  const bool use_k = k > 0 && k < a.n, use_p = p < 1.f;
-  SmpCut cut{key_none, 0};
+  if (one) {
+    // the first column of the largest logit
+    if (tid == 0) S.best = 0x7FFFFFFF;
+    __syncthreads();
+    if (mt == m) {
+      float f[kVec];
+      C.row.unpack(C.row.raw(first), f);
+      int col = 0x7FFFFFFF;
+#pragma unroll
+      for (int i = kVec - 1; i >= 0; --i)
+        if (f[i] == m) col = C.row.column(first) + i;
+      atomicMin(&S.best, col);
+    }
+    cl.sync();
+    if (rank == 0 && tid == 0) {
+      int col = S.best;
+      for (int q = 1; q < size; ++q) col = min(col, cl.map_shared_rank(&S, q)->best);
+      smp_emit<E>(a, r, col, 1.0);
+    }
+    cl.sync();
+    return;
+  }
+  if (all) {
+    // a common unit for the masses: the row's largest logit
+    w = SmpMass(m < INFINITY ? m : 0.f, T);
+  } else if (bad) {
+    w = SmpMass(m < INFINITY ? m : 0.f, T);
+  }
   double tie_w = 1.0;
   bool drawn = false;
-  if (greedy || k == 1 || p <= 0.f) {
-    cut.key = key_max;
-    cut.ties = 1;
-  } else if (m == INFINITY) {
+  if (m == INFINITY) {
     // the +inf entries are equal and have all the mass: every filter counts
     int cnt = 0;
     C.each([&](int, const float *f) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i) cnt += f[i] == INFINITY;
     });
-    const int all = __reduce_add_sync(0xFFFFFFFFu, cnt);
-    if (lane == 0) S.x_cnt[C.phase & 1][warp] = (unsigned long long)all;
-    smp_exchange(C, kSmpBands);
+    cnt = __reduce_add_sync(0xFFFFFFFFu, cnt);
+    if (lane == 0) S.x_cnt[C.phase & 1][warp] = (unsigned long long)cnt;
+    smp_exchange(C, kSmpWarps);
     cut.key = key_max;
     for (int i = 0; i < kSmpWarps; ++i) cut.ties += (long long)S.sum_cnt[i];
     if (use_k) cut.ties = min(cut.ties, k);
     if (use_p) cut.ties = smp_ties((double)p * (double)cut.ties, cut.ties);
-  } else {
-    if (mp > 0.f) cut.key = smp_min_key(w, m, fminf(mp, 1.f)) - 1u;
-    bool done = !use_k && !use_p && !(mp > 0.f);
-    if (!done && ((use_k && k <= kSmpMaxK) || (!use_k && mp > 0.f))) {
-      // candidates above a threshold that keeps the first k
-      uint32_t thr = cut.key + 1u;
+    bad = 1;
+  } else if (!all) {
+    if (use_m) cut.key = smp_min_key(m, T, fminf(mp, 1.f)) - 1u;
+    const float xb = smp_float(cut.key);  // the base: logits above
+    // What is tried next: the list of the candidates of a top-k or min-p, a
+    // split of the band with the cut, the list of a band's whole prefix, the
+    // list of a band, the cut key by key; kRow: the cut is known.
+    enum { kList, kSplit, kPrefix, kBand, kKeys, kRow } next;
+    float lo = xb, hi = m;
+    SmpBands bands{xb, m, 0.f, 1.f / kSmpBand0};
+    int level = 0;
+    bool summed = nucleus && !bad;  // the first bands' masses are known
+    double target = 0.0, above = 0.0, in_band = 0.0;
+    float band_lo = xb, band_hi = m, band_d0 = 0.f, band_d1 = 0.f;
+    if (!nucleus && (!use_k || k <= kSmpMaxK)) {
+      next = kList;
       if (use_k) {
-        // about `want` entries of a row in random order lie above the
-        // threads' rank-th largest maximum: a thread's maximum is above it
-        // with probability 1 - exp(-want / threads)
-        const float want = fminf(3.f * (float)k + 256.f, 1500.f);
+        // of a row in random order, about `want` entries lie above the
+        // threads' rank_t-th largest maximum: a thread's maximum is above it
+        // with probability 1 - exp(-want / threads). `want` leaves room for
+        // the spread of the count and for the highest of the CTAs' thresholds.
+        const float want = 1.1f * (float)k + 10.f * sqrtf((float)k) + 32.f;
         const int rank_t = max(1, (int)(kSmpThreads *
-                                        (1.f - expf(-want / (float)(kSmpThreads * size)))));
+                                        (1.f - __expf(-want / (float)(kSmpThreads * size)))));
         const uint32_t kt = smp_key(mt);
         uint32_t pre = 0u;
+#pragma unroll 1
         for (int bit = 31; bit >= 12; --bit) {
           const uint32_t c = pre | (1u << bit);
           if (__syncthreads_count(kt >= c) >= rank_t) pre = c;
         }
         if (size > 1) {
-          if (tid == 0) S.x_cnt[C.phase & 1][0] = pre;
           const int b = C.phase & 1;
           ++C.phase;
+          if (tid == 0) S.x_cnt[b][0] = pre;
           cl.sync();
           for (int q = 0; q < size; ++q)
             pre = max(pre, (uint32_t)cl.map_shared_rank(&S, q)->x_cnt[b][0]);
         }
-        thr = max(thr, pre);
+        lo = smp_float(max(cut.key, pre - 1u));
       }
-      const float xt = unmono(thr);
-      const int got = smp_collect(C, [&](float x) { return x >= xt; });
-      if (got <= kSmpList && (thr == cut.key + 1u || got >= k)) {
-        if (rank == 0) {
-          double wt[kSmpPer], z;
-          double run = smp_sort_list(C, w, got, wt, &z);
-          int keep = use_k ? (int)min(k, (long long)got) : got;
-          if (use_p) {
-            // mass of the first `keep`, then the prefix that reaches the target
+    } else {
+      next = use_k ? kKeys : kSplit;
+    }
+#pragma unroll 1
+    while (next != kRow) {
+      if (next == kSplit) {
+        if (level == 4) {
+          next = kKeys;
+          continue;
+        }
+        if (!summed) {
+          smp_bands<false>(C, w, bands);
+          smp_band_sums<true, false>(C);
+        }
+        summed = false;
+        if (level == 0) {
+          for (int i = 0; i < kSmpBands; ++i) target += S.sum_mass[i];
+          target *= (double)p;
+        }
+        // the band of the cut; entries in a band are at least its mass over
+        // its largest mass
+        int j = 0;
+        double entries = 0.0;
+#pragma unroll 1
+        for (; j < kSmpBands; ++j) {
+          band_d0 = j == 0 ? fminf(w.depth(m), bands.from) : bands.begin(j);
+          in_band = S.sum_mass[j] * (double)exp2f(band_d0);
+          entries += in_band;
+          if (above + S.sum_mass[j] >= target || j == kSmpBands - 1) break;
+          above += S.sum_mass[j];
+        }
+        band_d1 = level == 0 && j == kSmpBands - 1 ? 72.f : bands.begin(j + 1);
+        __syncthreads();
+        band_hi = j == 0 ? bands.hi : smp_band_top(w, bands, j);
+        band_lo = j == kSmpBands - 1 ? bands.lo : smp_band_top(w, bands, j + 1);
+        next = level == 0 && entries <= (double)kSmpList ? kPrefix
+               : in_band <= (double)kSmpList             ? kBand
+                                                         : kSplit;
+        lo = band_lo;
+        hi = next == kPrefix ? m : band_hi;
+        if (next == kSplit) {
+          ++level;
+          bands = SmpBands{band_lo, band_hi, band_d0,
+                           (float)kSmpBands / fmaxf(band_d1 - band_d0, 1e-6f)};
+          continue;
+        }
+      }
+      if (next == kKeys) {
+        if (use_k) smp_top_k(C, w, cut.key + 1u, key_max, k, cut);
+        if (use_p) {
+          const SmpCut base = cut;
+          smp_top_p(C, w, base, key_max, (double)p, cut);
+        }
+        break;
+      }
+      const int got = smp_collect(C, lo, hi);
+      const bool fits = got > 0 && got <= kSmpList &&
+                        (next != kList || lo == xb || (long long)got >= k);
+      if (!fits) {
+        if (next == kList) {
+          // min-p alone keeps a long prefix: its threshold is the cut
+          next = use_k ? kKeys : use_p ? kSplit : kRow;
+        } else if (next == kPrefix && in_band <= (double)kSmpList) {
+          next = kBand;
+          hi = band_hi;
+        } else {
+          next = kSplit;
+          ++level;
+          bands = SmpBands{band_lo, band_hi, band_d0,
+                           (float)kSmpBands / fmaxf(band_d1 - band_d0, 1e-6f)};
+        }
+        continue;
+      }
+      if (rank == 0) {
+        double wt[kSmpPer], z;
+        double run = smp_sort_list(C, w, got, wt, &z);
+        int keep = got;
+        if (next == kList) {
+          if (use_k) keep = (int)min(k, (long long)got);
+          if (use_p && keep < got) {  // mass of the first `keep`
             double part = 0.0;
 #pragma unroll
             for (int i = 0; i < kSmpPer; ++i) part += tid * kSmpPer + i < keep ? wt[i] : 0.0;
             smp_scan(S, part, &z);
-            const double target = (double)p * z;
-            int in = 0;
-#pragma unroll
-            for (int i = 0; i < kSmpPer; ++i) {
-              in += tid * kSmpPer + i < keep && run < target;
-              run += wt[i];
-            }
-            int before, all;
-            before = block_exclusive_scan(in, S.scan_i, &all);
-            (void)before;
-            keep = max(1, all);
           }
-          smp_draw_list<E>(C, a, r, keep, u);
-        }
-        drawn = done = true;
-      } else if (!use_k && !use_p) {
-        done = true;  // min-p alone keeps a long prefix: its threshold is the cut
-      }
-    }
-    if (!done && !use_k && use_p) {
-      // top-p over the entries above cut.key: bands of logits
-      const float xb = unmono(cut.key);
-      SmpBand band{0, 0, 0, 0};
-      double above = 0.0, target = 0.0;
-      float width = 2.f, top = 0.f;  // of the bands of this level; depth of the first
-      for (; band.level < 3 && !done;) {
-#pragma unroll
-        for (int i = 0; i < kSmpBands; ++i) S.band.mass[i][tid] = 0.0;
-        C.each([&](int, const float *f) {
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const float d = w.depth(f[i]);
-            if (f[i] > xb && (band.level == 0 || band.side(d) == 0))
-              S.band.mass[band.next(d)][tid] += w.at_depth(f[i], d);
-          }
-        });
-        smp_band_sums<true, false>(C);
-        if (band.level == 0) {
-          double z = 0.0;
-          for (int i = 0; i < kSmpBands; ++i) z += S.sum_mass[i];
           target = (double)p * z;
         }
-        int j = 0;
-        double head = 0.0;  // smallest number of entries that explains the masses before band j
-        for (; j < kSmpBands - 1; ++j) {
-          const double lo_cnt = S.sum_mass[j] * (double)exp2f(top + width * j);
-          if (above + S.sum_mass[j] >= target) {
-            // entries of the band at least: its mass / its largest mass
-            if (band.level == 0 && head + lo_cnt <= kSmpList) head = -1.0;
-            else head = lo_cnt;
-            break;
-          }
-          head += lo_cnt;
-          above += S.sum_mass[j];
-        }
-        __syncthreads();
-        if (band.level == 0) band.j0 = j;
-        else if (band.level == 1) band.j1 = j;
-        else band.j2 = j;
-        ++band.level;
-        top += width * j;
-        width *= 0.0625f;
-        if (head < 0.0) {
-          // the whole prefix down to the band may fit the list
-          const int got = smp_collect(C, [&](float x) { return x > xb && band.side(w.depth(x)) <= 0; });
-          if (got <= kSmpList) {
-            if (rank == 0) {
-              double wt[kSmpPer], z;
-              double run = smp_sort_list(C, w, got, wt, &z);
-              int in = 0;
-#pragma unroll
-              for (int i = 0; i < kSmpPer; ++i) {
-                in += tid * kSmpPer + i < got && run < target;
-                run += wt[i];
-              }
-              int all;
-              (void)block_exclusive_scan(in, S.scan_i, &all);
-              smp_draw_list<E>(C, a, r, max(1, all), u);
-            }
-            drawn = done = true;
-            break;
-          }
-        }
-        if (head > (double)kSmpList) continue;
-        const int got = smp_collect(C, [&](float x) { return x > xb && band.side(w.depth(x)) == 0; });
-        if (got == 0 || got > kSmpList) continue;
-        // the cut lies among these: the key and the ties of its last entry
-        if (rank == 0) {
-          double wt[kSmpPer], z;
-          double run = above + smp_sort_list(C, w, got, wt, &z);
-          int in = 0;
-#pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) {
-            in += tid * kSmpPer + i < got && run < target;
-            run += wt[i];
-          }
-          int all;
-          (void)block_exclusive_scan(in, S.scan_i, &all);
-          const int keep = max(1, all);
+        if (next == kBand) run += above;
+        if (use_p) keep = smp_reach(S, wt, run, target, keep);
+        if (next != kBand) {
+          smp_draw_list<E>(C, a, r, keep, u);
+        } else {
+          // the cut lies among these: the key and the ties of its last entry
           const uint32_t key = (uint32_t)(S.list.item[keep - 1] >> 32);
-          int same = 0;
+          int same = 0, ties;
 #pragma unroll
           for (int i = 0; i < kSmpPer; ++i) {
             const int at = tid * kSmpPer + i;
             same += at < keep && (uint32_t)(S.list.item[at] >> 32) == key;
           }
-          (void)block_exclusive_scan(same, S.scan_i, &all);
+          (void)smp_count_scan(S, same, &ties);
           if (tid == 0) {
             S.cut_key = key;
-            S.cut_ties = all;
+            S.cut_ties = ties;
           }
         }
+      }
+      if (next == kBand) {
         cl.sync();
         const SmpShared *R = cl.map_shared_rank(&S, 0);
         cut.key = (uint32_t)R->cut_key;
         cut.ties = R->cut_ties;
-        cl.sync();  // read before rank 0 writes its cut_ties again
-        done = true;
+      } else {
+        drawn = true;
       }
+      next = kRow;
     }
-    if (!done) {  // key by key
-      if (use_k) smp_top_k(C, w, cut.key + 1u, key_max, k, cut);
-      if (use_p) {
-        const SmpCut base = cut;
-        smp_top_p(C, w, base, key_max, (double)p, cut);
-      }
-    }
+    bad = 1;
     if (cut.ties > 0) tie_w = w(unmono(cut.key));
   }
-  if (!drawn) smp_draw_row<E>(C, a, w, cut, tie_w, r, u);
+  if (!drawn) {
+    if (bad) {  // the segments' masses are not known yet
+      if (cut.ties > 0)
+        smp_segment<true>(C, w, cut);
+      else
+        smp_segment<false>(C, w, cut);
+      cl.sync();
+    }
+    smp_draw_row<E>(C, a, w, cut, tie_w, r, u);
+  }
   cl.sync();
 }
 

@@ -156,6 +156,14 @@ def test_signed_zeros_are_equal():
     check(x, u, k=3)
     check(x, u, k=2)
     check(x, u, T=0.0)
+    # a threshold at zero keeps zeros of both signs
+    check(x, u, m=1.0)
+    check(x, u, k=3, m=0.9, p=0.7)
+    y = torch.zeros(5, 3000, device="cuda")
+    y[:, 1::2] = -0.0
+    y[:, ::7] = -2.0
+    for kw in ({"m": 1.0}, {"k": 900}, {"m": 0.5, "p": 0.4}, {"p": 0.9}):
+        check(y, u, **kw)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
