@@ -39,12 +39,14 @@
 namespace fh {
 
 constexpr int kSmpThreads = 256;
-constexpr int kSmpResident = 2;  // CTAs per SM
+// CTAs per SM: fp64 chains are long, and 32 warps cover them (16: 30 % slower)
+constexpr int kSmpResident = 4;
 constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBands = 16;
 constexpr int kSmpMaxCluster = 8;
 constexpr int kSmpChunk = 2048;  // vectors of the segment of the draw looked at together
 constexpr int kSmpList = 2048;   // candidates one CTA sorts
+constexpr int kSmpPart = 512;    // candidates of one warp
 constexpr int kSmpMaxK = 1024;   // largest top-k that goes through the list
 constexpr int kSmpCache = 8;     // vectors of a row that a thread keeps (CACHED)
 
@@ -73,9 +75,10 @@ struct __align__(16) SmpShared {
       uint32_t cnt[kSmpBands][kSmpThreads];
     } band;
     struct {
-      unsigned long long item[kSmpList];   // key << 32 | ~column
-      unsigned long long order[kSmpList];  // ~column << 32 | position in item
-      double w[kSmpList];
+      // the warps' candidates, key << 32 | column, by column; later the sorted
+      // keys of the whole list
+      unsigned long long part[kSmpWarps][kSmpPart];
+      uint32_t key[kSmpList], col[kSmpList];  // the whole list, by column
     } list;
     struct {
       double mass[kSmpChunk];
@@ -99,7 +102,10 @@ struct __align__(16) SmpShared {
   long long seg_left;
   double scan_d[kSmpWarps];
   int scan_i[33];
-  int count;  // list entries
+  int part_n[kSmpWarps];  // candidates a warp found
+  ulonglong2 sample[kSmpThreads / 2];
+  float lo;
+  int verdict;
   int best, last;
   unsigned long long cut_key;
   long long cut_ties;
@@ -120,6 +126,7 @@ template <>
 struct SmpElem<float> {
   static constexpr int kVec = 4;
   __device__ __forceinline__ static float to_float(float v) { return v; }
+  static constexpr uint32_t kNone = 0xFF800000u;  // -inf in every element of a word
   __device__ __forceinline__ static float none() { return -INFINITY; }
   __device__ __forceinline__ static void unpack(const uint4 &v, float *f) {
     f[0] = __uint_as_float(v.x);
@@ -132,6 +139,7 @@ template <>
 struct SmpElem<__nv_bfloat16> {
   static constexpr int kVec = 8;
   __device__ __forceinline__ static float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static constexpr uint32_t kNone = 0xFF80FF80u;
   __device__ __forceinline__ static __nv_bfloat16 none() { return __float2bfloat16(-INFINITY); }
   __device__ __forceinline__ static void unpack(const uint4 &v, float *f) {
     Vec<__nv_bfloat16>::to_float(v, f);
@@ -141,6 +149,7 @@ template <>
 struct SmpElem<__half> {
   static constexpr int kVec = 8;
   __device__ __forceinline__ static float to_float(__half v) { return __half2float(v); }
+  static constexpr uint32_t kNone = 0xFC00FC00u;
   __device__ __forceinline__ static __half none() { return __float2half(-INFINITY); }
   __device__ __forceinline__ static void unpack(const uint4 &v, float *f) {
     Vec<__half>::to_float(v, f);
@@ -159,6 +168,7 @@ struct SmpRow {
       : p(row), n(n_), mis((int)((reinterpret_cast<uintptr_t>(row) / sizeof(E)) % kVec)) {
     nv = n > 0 ? (n + mis + kVec - 1) / kVec : 0;
   }
+  __device__ __forceinline__ float at(int c) const { return SmpElem<E>::to_float(p[c]); }
   __device__ __forceinline__ int column(int v) const { return v * kVec - mis; }
   __device__ __forceinline__ uint4 raw(int v) const {
     const int c0 = column(v);
@@ -236,62 +246,64 @@ struct SmpCut {
   long long ties;
 };
 
+// A warp's segment of a row, and how it is walked.
 template <typename E, bool CACHED>
-struct SmpCtx {
+struct SmpSpan {
+  static constexpr int kVec = SmpElem<E>::kVec;
   SmpRow<E> row;
-  SmpShared &S;
-  int rank, size;  // CTA in its cluster
-  int v0, v1;      // this warp's segment
-  int phase;       // exchanges so far
-  int tid, warp, lane;
-  uint4 *cache;    // this thread's share of the row in shared memory (CACHED)
+  int v0, v1;
+  int lane;
+  uint4 *cache;  // this thread's share of the row in shared memory (CACHED)
 
-  // The first pass: f(vector, kVec values) over this warp's segment, a lane
-  // every 32 vectors; a CACHED row stays in shared memory.
-  template <typename F>
-  __device__ __forceinline__ void first(F f) {
-    constexpr int kVec = SmpRow<E>::kVec;
+  // f(vector, kVec values), a lane every 32 vectors, by whole warps: lanes past
+  // the segment get -inf. FIRST: the row is read for the first time; a CACHED
+  // row then stays in shared memory.
+  template <bool FIRST, typename F>
+  __device__ __forceinline__ void walk(F f) const {
+    constexpr uint32_t no = SmpElem<E>::kNone;
+    float x[kVec];
     if constexpr (CACHED) {
+      if (FIRST) {
 #pragma unroll
-      for (int i = 0; i < kSmpCache; ++i) {
-        const int v = v0 + lane + 32 * i;
-        if (v < v1) cache[kSmpThreads * i] = row.raw(v);
-      }
-      each(f);
-    } else {
-      int v = v0 + lane;
-      for (; v + 96 < v1; v += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = row.raw(v + 32 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x[kVec];
-          row.unpack(u[i], x);
-          f(v + 32 * i, x);
+        for (int i = 0; i < kSmpCache; ++i) {
+          const int v = v0 + lane + 32 * i;
+          cache[kSmpThreads * i] = v < v1 ? row.raw(v) : make_uint4(no, no, no, no);
         }
       }
-      for (; v < v1; v += 32) {
-        float x[kVec];
-        row.unpack(row.raw(v), x);
-        f(v, x);
-      }
-    }
-  }
-  template <typename F>
-  __device__ __forceinline__ void each(F f) {
-    if constexpr (CACHED) {
-      constexpr int kVec = SmpRow<E>::kVec;
 #pragma unroll 1
-      for (int i = 0, v = v0 + lane; v < v1; ++i, v += 32) {
-        float x[kVec];
+      for (int i = 0, v = v0; v < v1; ++i, v += 32) {
         row.unpack(cache[kSmpThreads * i], x);
-        f(v, x);
+        f(v + lane, x);
       }
     } else {
-      first(f);
+      int v = v0;
+      for (; v + 128 <= v1; v += 128) {
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = row.raw(v + lane + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          row.unpack(u[i], x);
+          f(v + lane + 32 * i, x);
+        }
+      }
+#pragma unroll 1
+      for (; v < v1; v += 32) {
+        row.unpack(v + lane < v1 ? row.raw(v + lane) : make_uint4(no, no, no, no), x);
+        f(v + lane, x);
+      }
     }
   }
+};
+
+template <typename E, bool CACHED>
+struct SmpCtx {
+  using Elem = E;
+  SmpSpan<E, CACHED> span;
+  SmpShared &S;
+  int rank, size;  // CTA in its cluster
+  int phase;       // exchanges so far
+  int tid, warp, lane;
 };
 
 // Sums x_*[phase & 1][0..n) over the cluster's CTAs, in rank order, into
@@ -381,9 +393,9 @@ __device__ __forceinline__ void smp_key_bands(Ctx &C, const SmpMass &w, uint32_t
     if (MASS) S.band.mass[i][C.tid] = 0.0;
     S.band.cnt[i][C.tid] = 0u;
   }
-  C.each([&](int, const float *f) {
+  C.span.template walk<false>([&](int, const float *f) {
 #pragma unroll
-    for (int i = 0; i < decltype(C.row)::kVec; ++i) {
+    for (int i = 0; i < decltype(C.span)::kVec; ++i) {
       const uint32_t k = smp_key(f[i]);
       if (k >= lo && k <= hi) {
         const int b = (int)((k - lo) >> shift);
@@ -540,136 +552,176 @@ __device__ __noinline__ float smp_band_top(const SmpMass &w, const SmpBands &b, 
   return unmono(lo);
 }
 
-// Entries in (lo, hi] into this CTA's list; returns the cluster's total, and
-// gathers the lists in rank 0's when they fit. Contains cluster barriers.
+// The entries that `hit` marks of a warp's vectors (a lane's first column c0)
+// into the warp's part of the list, in column order; n counts on past its end.
+template <int kVec>
+__device__ __forceinline__ void smp_append(const float *f, int c0, uint32_t hit,
+                                           unsigned long long *part, int &n) {
+  if (__any_sync(0xFFFFFFFFu, hit)) {
+    const int mine = __popc(hit);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if ((int)(threadIdx.x & 31) >= o) incl += t;
+    }
+    int at = n + incl - mine;
+    n += __shfl_sync(0xFFFFFFFFu, incl, 31);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if ((hit >> i) & 1u) {
+        if (at < kSmpPart)
+          part[at] = ((unsigned long long)smp_key(f[i]) << 32) | (uint32_t)(c0 + i);
+        ++at;
+      }
+  }
+}
+
+// Exchanges the number of candidates (and x_mass[0] of the caller): the
+// cluster's total in sum_cnt[0], beyond kSmpList also where one warp found
+// more than its part holds.
 template <typename Ctx>
-__device__ __forceinline__ int smp_collect(Ctx &C, float lo, float hi) {
+__device__ __forceinline__ void smp_count_list(Ctx &C) {
+  SmpShared &S = C.S;
+  __syncthreads();
+  if (C.warp == 0) {
+    int n = C.lane < kSmpWarps ? S.part_n[C.lane] : 0;
+    const bool over = __any_sync(0xFFFFFFFFu, n > kSmpPart);
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if (C.lane == 0) S.x_cnt[C.phase & 1][0] = over ? (unsigned long long)kSmpList + 1ull : n;
+  }
+  smp_exchange(C, 1);
+}
+
+// Rank 0 joins the warps' parts into its list, in column order (a cluster
+// barrier before; one after: the other CTAs may go).
+template <typename Ctx>
+__device__ __forceinline__ void smp_gather(Ctx &C) {
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   SmpShared &S = C.S;
+  if (C.rank == 0) {
+    static_assert(kSmpMaxCluster * kSmpWarps <= 64, "two parts per lane");
+    const int parts = C.size * kSmpWarps, g = 2 * C.lane;
+    const SmpShared *R = cl.map_shared_rank(&S, min(g / kSmpWarps, C.size - 1));
+    const int n0 = g < parts ? R->part_n[g % kSmpWarps] : 0;
+    const int n1 = g + 1 < parts ? R->part_n[(g + 1) % kSmpWarps] : 0;
+    int incl = n0 + n1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (C.lane >= o) incl += t;
+    }
+    const int at0 = incl - n0 - n1, at1 = incl - n1;
+    for (int q = C.warp; q < parts; q += kSmpWarps) {
+      const int base = __shfl_sync(0xFFFFFFFFu, q & 1 ? at1 : at0, q / 2);
+      const int cnt = __shfl_sync(0xFFFFFFFFu, q & 1 ? n1 : n0, q / 2);
+      const SmpShared *P = cl.map_shared_rank(&S, q / kSmpWarps);
+      for (int i = C.lane; i < cnt; i += 32) {
+        const unsigned long long e = P->list.part[q % kSmpWarps][i];
+        S.list.key[base + i] = (uint32_t)(e >> 32);
+        S.list.col[base + i] = (uint32_t)e;
+      }
+    }
+  }
+  if (C.size > 1) cl.sync();
   __syncthreads();
-  if (C.tid == 0) S.count = 0;
+}
+
+// Entries in (lo, hi] into the list of rank 0, when they fit; returns their
+// number in the cluster. Contains cluster barriers.
+template <typename Ctx>
+__device__ __forceinline__ int smp_collect(Ctx &C, float lo, float hi) {
+  constexpr int kVec = decltype(C.span)::kVec;
+  SmpShared &S = C.S;
   __syncthreads();
-  C.each([&](int v, const float *f) {
-    constexpr int kVec = decltype(C.row)::kVec;
+  int n = 0;
+  unsigned long long *part = S.list.part[C.warp];
+  C.span.template walk<false>([&](int v, const float *f) {
     uint32_t hit = 0u;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) hit |= f[i] > lo && f[i] <= hi ? 1u << i : 0u;
-    if (hit) {
-      int at = atomicAdd(&S.count, __popc(hit));
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (((hit >> i) & 1u) && at < kSmpList)
-          S.list.item[at++] = ((unsigned long long)smp_key(f[i]) << 32) |
-                              (0xFFFFFFFFu - (uint32_t)(C.row.column(v) + i));
-    }
+    smp_append<kVec>(f, C.span.row.column(v), hit, part, n);
   });
-  __syncthreads();
-  if (C.tid == 0) S.x_cnt[C.phase & 1][0] = (unsigned long long)S.count;
-  smp_exchange(C, 1);
+  if (C.lane == 0) S.part_n[C.warp] = n;
+  smp_count_list(C);
   const unsigned long long total = S.sum_cnt[0];
   if (total > (unsigned long long)kSmpList) return kSmpList + 1;
-  if (C.size > 1) {
-    if (C.rank == 0) {
-      int base = S.count;
-      for (int r = 1; r < C.size; ++r) {
-        const SmpShared *R = cl.map_shared_rank(&S, r);
-        const int cnt = R->count;
-        for (int i = C.tid; i < cnt; i += kSmpThreads) S.list.item[base + i] = R->list.item[i];
-        base += cnt;
-      }
-    }
-    cl.sync();  // the others' lists may go
-  }
-  __syncthreads();
+  smp_gather(C);
   return (int)total;
 }
 
-// Descending bitonic sort of n2 (a power of two, at most kSmpList) words by
-// the whole CTA: thread t holds words kPer * t .. in registers, so that short
-// strides stay in a thread, those below 32 * kPer in a warp (shuffles), and
-// only the few longer ones go through shared memory.
+// Descending bitonic sort of n2 (a power of two, at most kSmpList) keys by the
+// whole CTA. A thread holds kEach = n2 / threads neighbouring keys (one, of
+// fewer threads, below that) in registers: short strides stay in a thread,
+// those within a warp are shuffles, and only the 6 longest of a full CTA go
+// through shared memory.
 constexpr int kSmpPer = kSmpList / kSmpThreads;
-__device__ __noinline__ void smp_sort(unsigned long long *a, int n2) {
-  const int tid = threadIdx.x, base = tid * kSmpPer;
-  unsigned long long x[kSmpPer];
+template <int kEach>
+__device__ __noinline__ void smp_sort_n(uint32_t *a, int n2) {
+  const int tid = threadIdx.x, base = tid * kEach;
+  uint32_t x[kEach];
   __syncthreads();
-  const bool mine = base < n2;
 #pragma unroll
-  for (int i = 0; i < kSmpPer; ++i) x[i] = base + i < n2 ? a[base + i] : 0ull;
-  const int n = max(n2, kSmpPer);
-  for (int size = 2; size <= n; size <<= 1) {
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      if (step >= 32 * kSmpPer) {
-        __syncthreads();
-        if (mine)
+  for (int i = 0; i < kEach; ++i) x[i] = base + i < n2 ? a[base + i] : 0u;
+  const bool live = (tid & ~31) * kEach < n2;  // this warp has keys
+#pragma unroll 1
+  for (int size = 2; size <= n2; size <<= 1) {
+#pragma unroll 1
+    for (int step = size >> 1; step >= 32 * kEach; step >>= 1) {
+      __syncthreads();
+      if (live)
 #pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) a[base + i] = x[i];
-        __syncthreads();
-        if (mine)
+        for (int i = 0; i < kEach; ++i) a[base + i] = x[i];
+      __syncthreads();
+      if (live)
 #pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) {
-            const int at = base + i;
-            const unsigned long long y = a[at ^ step];
-            // the lower index keeps the larger word in a falling run
-            const bool big = ((at & step) == 0) == ((at & size) == 0);
-            x[i] = (x[i] > y) == big ? x[i] : y;
-          }
-      } else if (step >= kSmpPer) {
-        if (base - (tid & 31) * kSmpPer < n2) {  // the whole warp or none of it
-#pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) {
-            const int at = base + i;
-            const unsigned long long y = __shfl_xor_sync(0xFFFFFFFFu, x[i], step / kSmpPer);
-            const bool big = ((at & step) == 0) == ((at & size) == 0);
-            x[i] = (x[i] > y) == big ? x[i] : y;
-          }
+        for (int i = 0; i < kEach; ++i) {
+          // the lower index keeps the larger key in a falling run
+          const uint32_t y = a[(base + i) ^ step];
+          const bool big = (((base + i) & step) == 0) == (((base + i) & size) == 0);
+          x[i] = big ? max(x[i], y) : min(x[i], y);
         }
-      } else if (mine) {
+    }
+    if (!live) continue;
+#pragma unroll 1
+    for (int step = min(size >> 1, 16 * kEach); step >= kEach; step >>= 1) {
+      const bool low = (base & step) == 0;
 #pragma unroll
-        for (int s = kSmpPer / 2; s > 0; s >>= 1) {
-          if (s != step) continue;
+      for (int i = 0; i < kEach; ++i) {
+        const uint32_t y = __shfl_xor_sync(0xFFFFFFFFu, x[i], step / kEach);
+        const bool big = low == (((base + i) & size) == 0);
+        x[i] = big ? max(x[i], y) : min(x[i], y);
+      }
+    }
 #pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) {
-            if (i & s) continue;
-            const bool fall = ((base + i) & size) == 0;
-            const unsigned long long u = x[i], v = x[i | s];
-            const bool swap = (u < v) == fall;
-            x[i] = swap ? v : u;
-            x[i | s] = swap ? u : v;
-          }
-        }
+    for (int step = kEach / 2; step > 0; step >>= 1) {
+      if (step >= size) continue;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (i & step) continue;
+        const bool fall = ((base + i) & size) == 0;
+        const uint32_t u = max(x[i], x[i | step]), v = min(x[i], x[i | step]);
+        x[i] = fall ? u : v;
+        x[i | step] = fall ? v : u;
       }
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kSmpPer; ++i)
+  for (int i = 0; i < kEach; ++i)
     if (base + i < n2) a[base + i] = x[i];
   __syncthreads();
 }
+__device__ __forceinline__ void smp_sort(uint32_t *a, int n2) {
+  static_assert(kSmpPer == 8, "sorts for 1 to 8 keys per thread");
+  if (n2 <= kSmpThreads) return smp_sort_n<1>(a, n2);
+  if (n2 <= 2 * kSmpThreads) return smp_sort_n<2>(a, n2);
+  if (n2 <= 4 * kSmpThreads) return smp_sort_n<4>(a, n2);
+  smp_sort_n<8>(a, n2);
+}
 
 __device__ __forceinline__ int smp_pow2(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
-
-// Sorts the list and leaves its masses in list.w. Returns this thread's
-// exclusive prefix of the masses of items kPer * tid .. + kPer - 1.
-template <typename Ctx>
-__device__ __forceinline__ double smp_sort_list(Ctx &C, const SmpMass &w, int n, double *wt,
-                                                double *total) {
-  SmpShared &S = C.S;
-  const int n2 = smp_pow2(n);
-  for (int i = n + C.tid; i < n2; i += kSmpThreads) S.list.item[i] = 0ull;
-  smp_sort(S.list.item, n2);
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kSmpPer; ++i) {
-    const int at = C.tid * kSmpPer + i;
-    wt[i] = at < n ? w(unmono((uint32_t)(S.list.item[at] >> 32))) : 0.0;
-    if (at < n) S.list.w[at] = wt[i];
-    sum += wt[i];
-  }
-  return smp_scan(S, sum, total);
-}
 
 template <typename E>
 __device__ __forceinline__ void smp_emit(const SampleArgs &a, int r, int col, double prob) {
@@ -677,83 +729,161 @@ __device__ __forceinline__ void smp_emit(const SampleArgs &a, int r, int col, do
   if (a.prob) a.prob[r] = (float)prob;
 }
 
-// The draw from the first `keep` items of the sorted list (rank 0's CTA).
-template <typename E, typename Ctx>
-__device__ __forceinline__ void smp_draw_list(Ctx &C, const SampleArgs &a, int r, int keep,
-                                              double u) {
-  SmpShared &S = C.S;
-  if (keep == 1) {
-    if (C.tid == 0) smp_emit<E>(a, r, (int)(0xFFFFFFFFu - (uint32_t)S.list.item[0]), 1.0);
-    return;
+// The list's prefix (rank 0's CTA): sorts its n keys and cuts them, as the
+// caller says, at the first `keep` (counted among the keys above `least`), or at
+// the mass `target` (target < 0: p times the prefix's own mass), which the
+// entries from `above` on share with mass outside the list. Returns the cut and
+// in *total the mass of the first `keep`.
+struct SmpPick {
+  uint32_t key;
+  int ties, keep;
+};
+__device__ __noinline__ SmpPick smp_pick(SmpShared &S, SmpMass w, int n, uint32_t least,
+                                         long long k, double p, double target, double above,
+                                         double most, bool *sure) {
+  const int tid = threadIdx.x;
+  uint32_t *sorted = reinterpret_cast<uint32_t *>(S.list.part[0]);
+  const int n2 = smp_pow2(n);
+  for (int i = tid; i < n2; i += kSmpThreads) sorted[i] = i < n ? S.list.key[i] : 0u;
+  smp_sort(sorted, n2);
+  uint32_t key[kSmpPer];
+  int in = 0, keep;
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i) {
+    const int at = tid * kSmpPer + i;
+    key[i] = at < n ? sorted[at] : 0u;
+    in += key[i] > least;
   }
-  const int n2 = smp_pow2(keep);
-  for (int i = C.tid; i < n2; i += kSmpThreads)
-    S.list.order[i] = i < keep ? (S.list.item[i] << 32) | (uint32_t)i : 0ull;
-  if (C.tid == 0) {
+  (void)smp_count_scan(S, in, &keep);
+  if (k > 0) keep = (int)min(k, (long long)keep);
+  if (p < 1.0) {
+    double wt[kSmpPer], sum = 0.0, z;
+#pragma unroll
+    for (int i = 0; i < kSmpPer; ++i) {
+      wt[i] = tid * kSmpPer + i < keep ? w(unmono(key[i])) : 0.0;
+      sum += wt[i];
+    }
+    double run = above + smp_scan(S, sum, &z);
+    if (target < 0.0) target = p * z;
+    int reach = 0, reach_most = 0, all;
+#pragma unroll
+    for (int i = 0; i < kSmpPer; ++i) {
+      const bool valid = tid * kSmpPer + i < keep;
+      reach += valid && run < target;
+      reach_most += valid && run < most;
+      run += wt[i];
+    }
+    (void)smp_count_scan(S, reach | (reach_most << 16), &all);
+    // the cut is the same for the least and the most that the target can be
+    if (sure) *sure = (all & 0xFFFF) == (all >> 16) && most < z;
+    keep = max(1, all & 0xFFFF);
+  }
+  SmpPick pick;
+  pick.keep = keep;
+  pick.key = sorted[keep - 1];
+  int higher = 0, all;
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i) higher += key[i] > pick.key;
+  (void)smp_count_scan(S, higher, &all);
+  pick.ties = keep - all;
+  return pick;
+}
+
+// The draw from the list, cut at `pick` (rank 0's CTA).
+template <typename E>
+__device__ __noinline__ void smp_draw_list(SmpShared &S, const SampleArgs &a, SmpMass w, int r,
+                                           int n, SmpPick pick, double u) {
+  const int tid = threadIdx.x;
+  if (tid == 0) {
     S.best = 0x7FFFFFFF;
     S.last = -1;
   }
-  smp_sort(S.list.order, n2);  // rising columns
+  uint32_t key[kSmpPer];
+  int ties = 0, all;
+#pragma unroll
+  for (int i = 0; i < kSmpPer; ++i) {
+    const int at = tid * kSmpPer + i;
+    key[i] = at < n ? S.list.key[at] : 0u;
+    ties += key[i] == pick.key;
+  }
+  int left = pick.ties - smp_count_scan(S, ties, &all);
   double wt[kSmpPer], sum = 0.0, total;
 #pragma unroll
   for (int i = 0; i < kSmpPer; ++i) {
-    const int at = C.tid * kSmpPer + i;
-    wt[i] = at < keep ? S.list.w[(uint32_t)S.list.order[at]] : 0.0;
+    const bool keep = key[i] > pick.key || (key[i] == pick.key && left-- > 0);
+    wt[i] = keep ? w(unmono(key[i])) : 0.0;
     sum += wt[i];
   }
   double run = smp_scan(S, sum, &total);
   const double target = u * total;
+  int best = 0x7FFFFFFF, last = -1;
 #pragma unroll
   for (int i = 0; i < kSmpPer; ++i) {
-    const int at = C.tid * kSmpPer + i;
     run += wt[i];
     if (wt[i] > 0.0) {
-      if (run > target) atomicMin(&S.best, at);
-      atomicMax(&S.last, at);
+      last = tid * kSmpPer + i;
+      if (run > target) best = min(best, last);
     }
   }
+  if (best != 0x7FFFFFFF) atomicMin(&S.best, best);
+  if (last >= 0) atomicMax(&S.last, last);
   __syncthreads();
-  if (C.tid == 0) {
+  if (tid == 0) {
     // past the end by rounding: the last entry with a mass
-    const unsigned long long o = S.list.order[S.best != 0x7FFFFFFF ? S.best : S.last];
-    smp_emit<E>(a, r, (int)(0xFFFFFFFFu - (uint32_t)(o >> 32)), S.list.w[(uint32_t)o] / total);
+    const int at = S.best != 0x7FFFFFFF ? S.best : S.last;
+    smp_emit<E>(a, r, (int)S.list.col[at], w(unmono(S.list.key[at])) / total);
   }
 }
 
-// Kept mass and ties of this warp's segment, for the prefix `cut`; returns
-// its largest logit.
-template <bool TIES, typename Ctx>
-__device__ __forceinline__ float smp_segment(Ctx &C, const SmpMass &w, const SmpCut &cut) {
-  constexpr int kVec = decltype(C.row)::kVec;
-  const float xc = smp_float(cut.key), above = fmaxf(xc, w.xlo);
+// The loops with fp64 exponentials are functions of their own: registers are
+// allotted to them alone.
+struct SmpSum {
+  double sum;
+  float top;
+  int ties;
+};
+template <bool FIRST, bool TIES, typename Span>
+__device__ __noinline__ SmpSum smp_sum(Span span, SmpMass w, float xc) {
+  constexpr int kVec = Span::kVec;
+  const float above = fmaxf(xc, w.xlo);
   double sum0 = 0.0, sum1 = 0.0;
-  int ties = 0;
-  float top = -INFINITY;
-  C.each([&](int, const float *f) {
-    double x[kVec];
+  SmpSum r{0.0, -INFINITY, 0};
+  span.template walk<FIRST>([&](int, const float *f) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) x[i] = w.raw(f[i]);
+    for (int h = 0; h < kVec; h += 4) {
+      double x[4];
 #pragma unroll
-    for (int i = 0; i < kVec; i += 2) {
-      if (f[i] > above) sum0 += x[i];
-      if (f[i + 1] > above) sum1 += x[i + 1];
-      top = fmaxf(top, fmaxf(f[i], f[i + 1]));
-      if (TIES) ties += (f[i] == xc) + (f[i + 1] == xc);
+      for (int i = 0; i < 4; ++i) x[i] = w.raw(f[h + i]);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        if (f[h + i] > above) sum0 += x[i];
+        if (f[h + i + 1] > above) sum1 += x[i + 1];
+        if (FIRST) r.top = fmaxf(r.top, fmaxf(f[h + i], f[h + i + 1]));
+        if (TIES) r.ties += (f[h + i] == xc) + (f[h + i + 1] == xc);
+      }
     }
   });
-  double sum = sum0 + sum1;
+  r.sum = sum0 + sum1;
+  return r;
+}
+
+// Kept mass and ties of this warp's segment, for the prefix `cut`; returns
+// its largest logit (FIRST).
+template <bool FIRST, bool TIES, typename Ctx>
+__device__ __forceinline__ float smp_segment(Ctx &C, const SmpMass &w, const SmpCut &cut) {
+  SmpSum r = smp_sum<FIRST, TIES>(C.span, w, smp_float(cut.key));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (TIES) ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
+    r.sum += __shfl_xor_sync(0xFFFFFFFFu, r.sum, o);
+    if (FIRST) r.top = fmaxf(r.top, __shfl_xor_sync(0xFFFFFFFFu, r.top, o));
+    if (TIES) r.ties += __shfl_xor_sync(0xFFFFFFFFu, r.ties, o);
   }
   if (C.lane == 0) {
-    C.S.warp_d[C.warp] = sum;
+    C.S.warp_d[C.warp] = r.sum;
     C.S.warp_k[C.warp] = w.k0;
-    C.S.warp_i[C.warp] = ties;
+    C.S.warp_i[C.warp] = r.ties;
   }
-  return top;
+  return r.top;
 }
 
 // The draw from the prefix `cut` of the whole row: the segments' masses are in
@@ -805,8 +935,8 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   if (seg / kSmpWarps != C.rank) return;
   // the segment in pieces of kSmpChunk vectors: their masses, then the vector
   // of the draw, then its entry
-  const int sv0 = (int)((long long)C.row.nv * seg / segs);
-  const int sv1 = (int)((long long)C.row.nv * (seg + 1) / segs);
+  const int sv0 = (int)((long long)C.span.row.nv * seg / segs);
+  const int sv1 = (int)((long long)C.span.row.nv * (seg + 1) / segs);
   constexpr int kEach = kSmpChunk / kSmpThreads;
   double run = S.seg_before;
   left = S.seg_left;
@@ -821,7 +951,7 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
       float f[kVec];
       double x[kVec], sum = 0.0;
       int t = 0;
-      C.row.unpack(C.row.raw(c0 + i), f);
+      C.span.row.unpack(C.span.row.raw(c0 + i), f);
 #pragma unroll
       for (int q = 0; q < kVec; ++q) x[q] = w.raw(f[q]);
 #pragma unroll
@@ -883,7 +1013,7 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
           if (cut.ties > 0 && tid * kEach + i == at) lft = l[i];
         }
         float f[kVec];
-        C.row.unpack(C.row.raw(c0 + at), f);
+        C.span.row.unpack(C.span.row.raw(c0 + at), f);
         int col = -1;
         double x = 0.0;
         bool found = false;
@@ -896,7 +1026,7 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
             e = tie_w;
           to += e;
           if (e > 0.0 && !found) {
-            col = C.row.column(c0 + at) + q;
+            col = C.span.row.column(c0 + at) + q;
             x = e;
             found = to > target;
           }
@@ -909,61 +1039,122 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   }
 }
 
-// The list's entries (sorted, rank 0) up to the target mass; `run` is this
-// thread's exclusive prefix.
-__device__ __noinline__ int smp_reach(SmpShared &S, const double *wt, double run, double target,
-                                         int n) {
-  int in = 0, all;
-#pragma unroll
-  for (int i = 0; i < kSmpPer; ++i) {
-    in += (int)threadIdx.x * kSmpPer + i < n && run < target;
-    run += wt[i];
-  }
-  (void)smp_count_scan(S, in, &all);
-  return max(1, all);
-}
-
-// Masses of the 16 bands of the logits in (b.lo, b.hi], per thread. FIRST: the
-// row is read for the first time and has no upper end; returns the warp's
-// largest logit.
+// Masses of the 16 bands of the logits in (b.lo, b.hi], per thread. WIDE: most
+// of the row lies there.
 constexpr float kSmpBand0 = 1.5f;  // depth of a first band: 15 hold all but 2^-22
-template <bool FIRST, typename Ctx>
-__device__ __forceinline__ float smp_bands(Ctx &C, const SmpMass &w, const SmpBands &b) {
-  constexpr int kVec = decltype(C.row)::kVec;
-  SmpShared &S = C.S;
+template <bool WIDE, typename Span>
+__device__ __noinline__ void smp_bands(Span span, SmpMass w, SmpBands b, double *mine) {
+  constexpr int kVec = Span::kVec;
 #pragma unroll
-  for (int i = 0; i < kSmpBands; ++i) S.band.mass[i][C.tid] = 0.0;
+  for (int i = 0; i < kSmpBands; ++i) mine[i * kSmpThreads] = 0.0;
   const float least = fmaxf(b.lo, w.xlo), hi = b.hi;
-  double *mine = &S.band.mass[0][C.tid];
-  float top = -INFINITY;
-  if (FIRST) {
-    C.first([&](int, const float *f) {
-      double x[kVec];
+  span.template walk<false>([&](int, const float *f) {
+    if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) x[i] = w.raw(f[i]);
+      for (int h = 0; h < kVec; h += 4) {
+        double x[4];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        top = fmaxf(top, f[i]);
-        const int j = b.band(w.depth(f[i]));
-        if (f[i] > least) mine[j * kSmpThreads] += x[i];
+        for (int i = 0; i < 4; ++i) x[i] = w.raw(f[h + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = b.band(w.depth(f[h + i]));
+          if (f[h + i] > least) mine[j * kSmpThreads] += x[i];
+        }
       }
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  } else {
-    C.each([&](int, const float *f) {
+    } else {
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
         if (f[i] > least && f[i] <= hi) mine[b.band(w.depth(f[i])) * kSmpThreads] += w.raw(f[i]);
-    });
+    }
+  });
+}
+
+// The first pass of the list path: the thread's largest logit, the entries
+// above `lo` into the CTA's list and, MASS, the row's mass relative to `ref` in
+// fp32, kSmpSlack of it off at most: with t = (x - ref) c, the difference is
+// off by 2^-24 |t| (t > -100, and below 2^-32 nothing counts), c's second word
+// corrects its product, and ex2 (2^-22), the products and a vector's sum add
+// 2^-20.
+constexpr double kSmpSlack = 3.8147e-6;  // 2^-18
+__device__ __forceinline__ float smp_ex2(float t) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  return y;
+}
+struct SmpFirst {
+  double z;
+  float top;
+};
+template <bool MASS, typename Span>
+__device__ __noinline__ SmpFirst smp_first(Span span, float lo, float ref, double c,
+                                           unsigned long long *part, int *part_n) {
+  constexpr int kVec = Span::kVec;
+  const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi), xcut = ref - 100.f / c_hi;
+  SmpFirst r{0.0, -INFINITY};
+  int n = 0;
+  span.template walk<true>([&](int v, const float *f) {
+    uint32_t hit = 0u;
+    float sum = 0.f, top = f[0];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (i) top = fmaxf(top, f[i]);
+      if (MASS) {
+        const float x = f[i] - ref, t = x * c_hi;
+        const float e = smp_ex2(t), d = fmaf(x, c_lo, fmaf(x, c_hi, -t));
+        const float y = fmaf(e, d * 0.69314718f, e);
+        if (f[i] > xcut) sum += y;
+      }
+    }
+    r.top = fmaxf(r.top, top);
+    if (MASS) r.z += (double)sum;
+    if (top > lo) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) hit |= f[i] > lo ? 1u << i : 0u;
+    }
+    smp_append<kVec>(f, span.row.column(v), hit, part, n);
+  });
+  if (span.lane == 0) *part_n = n;
+  return r;
+}
+
+// A threshold above which a row in random order has about `want` entries, and
+// the largest logit of the sample: one vector per thread, spread over the row
+// and the same in every CTA of the cluster. The threshold is the r-th largest
+// of the vectors' maxima.
+template <typename Ctx>
+__device__ __forceinline__ void smp_sample(Ctx &C, float want, float &lo, float &ref) {
+  constexpr int kVec = decltype(C.span)::kVec;
+  SmpShared &S = C.S;
+  float f[kVec];
+  C.span.row.unpack(
+      C.span.row.raw((int)((long long)C.span.row.nv * C.tid / kSmpThreads)), f);
+  float x = f[0];
+#pragma unroll
+  for (int i = 1; i < kVec; ++i) x = fmaxf(x, f[i]);
+  x = fmaxf(x, -INFINITY);  // all NaN
+  // every thread counts the larger ones (equal ones by thread)
+  const unsigned long long key = ((unsigned long long)smp_key(x) << 32) | (uint32_t)~C.tid;
+  reinterpret_cast<unsigned long long *>(S.sample)[C.tid] = key;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kSmpThreads / 2; ++i) {
+    const ulonglong2 k = S.sample[i];
+    above += (int)(k.x > key) + (int)(k.y > key);
   }
-  return top;
+  const int r = min(kSmpThreads, max(4, (int)(want * (kSmpThreads * kVec) / (float)C.span.row.n)));
+  if (above == r - 1) S.lo = x;
+  if (above == 0) S.warp_f[0] = x;
+  __syncthreads();
+  lo = S.lo;
+  ref = S.warp_f[0];
+  __syncthreads();
 }
 
 // CACHED: every lane's share of the row is at most kSmpCache vectors, kept in
 // shared memory.
 template <typename E, bool CACHED>
-__global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs a) {
+__global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpResident) k_sample(SampleArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) unsigned char smp_raw[];
   SmpShared &S = *reinterpret_cast<SmpShared *>(smp_raw);
@@ -972,13 +1163,14 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
   const int size = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int r = blockIdx.x / size;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  SmpCtx<E, CACHED> C{SmpRow<E>(reinterpret_cast<const E *>(a.logits) + (long long)r * a.stride, a.n),
-                      S, rank, size, 0, 0, 0, tid, warp, lane,
-                      reinterpret_cast<uint4 *>(smp_raw + sizeof(SmpShared)) + tid};
+  SmpCtx<E, CACHED> C{
+      {SmpRow<E>(reinterpret_cast<const E *>(a.logits) + (long long)r * a.stride, a.n), 0, 0, lane,
+       reinterpret_cast<uint4 *>(smp_raw + sizeof(SmpShared)) + tid},
+      S, rank, size, 0, tid, warp, lane};
   {
     const int gw = rank * kSmpWarps + warp, warps = size * kSmpWarps;
-    C.v0 = (int)((long long)C.row.nv * gw / warps);
-    C.v1 = (int)((long long)C.row.nv * (gw + 1) / warps);
+    C.span.v0 = (int)((long long)C.span.row.nv * gw / warps);
+    C.span.v1 = (int)((long long)C.span.row.nv * (gw + 1) / warps);
   }
   float T = a.temperature ? a.temperature[r] : a.temperature0;
   const long long k = a.top_k ? a.top_k[r] : a.top_k0;
@@ -995,41 +1187,45 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
   SmpCut cut{key_none, 0};
 
   // The first pass: the row's largest logit. Without a filter it sums the
-  // masses as well, with a top-p alone those of its bands, in units that the
-  // row's first entries give.
-  float mt = -INFINITY, m;
+  // masses as well, every warp in units of the largest of its first entries;
+  // where a filter keeps few entries it collects those above a threshold that
+  // a sample gives (a row in shared memory is better walked twice).
+  const bool fast = !CACHED && !one && !all && (!use_k || k <= kSmpMaxK);
+  float mt = -INFINITY, m, fast_lo = -INFINITY, ref = 0.f;
   int first = 0x7FFFFFFF;
   SmpMass w(0.f, T);
   int bad = 1;
-  if (all || nucleus) {
-    // without a filter a warp's units are its own; bands need the row's
-    float ref = -INFINITY, f[kVec];
-    const int v = all ? C.v0 + lane : (int)((long long)C.row.nv * tid / kSmpThreads);
-    if (v < (all ? C.v1 : C.row.nv)) {
-      C.row.unpack(C.row.raw(v), f);
+  if (all) {
+    float f[kVec];
+    ref = -INFINITY;
+    if (C.span.v0 + lane < C.span.v1) {
+      C.span.row.unpack(C.span.row.raw(C.span.v0 + lane), f);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) ref = fmaxf(ref, f[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xFFFFFFFFu, ref, o));
-    if (nucleus) {
-      if (lane == 0) S.warp_f[warp] = ref;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kSmpWarps; ++i) ref = fmaxf(ref, S.warp_f[i]);
-      __syncthreads();
-    }
     if (!(fabsf(ref) < INFINITY)) ref = 0.f;
     w = SmpMass(ref, T);
-    if (all) {
-      if constexpr (CACHED) C.first([](int, const float *) {});
-      m = smp_segment<false>(C, w, cut);
-    } else {
-      m = smp_bands<true>(C, w, SmpBands{-INFINITY, INFINITY, 0.f, 1.f / kSmpBand0});
-    }
+    m = smp_segment<true, false>(C, w, cut);
     bad = w.held || w.depth(m) < -900.f;
+  } else if (fast) {
+    if (a.n > kSmpList)
+      smp_sample(C, use_k ? 1.1f * (float)k + 10.f * sqrtf((float)k) + 32.f : 600.f, fast_lo, ref);
+    if (!(fabsf(ref) < INFINITY)) ref = 0.f;
+    SmpFirst f;
+    unsigned long long *part = S.list.part[warp];
+    if (nucleus && a.n > kSmpList)
+      f = smp_first<true>(C.span, fast_lo, ref, 1.4426950408889634 / (double)T, part,
+                          &S.part_n[warp]);
+    else
+      f = smp_first<false>(C.span, fast_lo, ref, 1.0, part, &S.part_n[warp]);
+    m = mt = f.top;
+    double z;
+    smp_scan(S, f.z, &z);
+    if (tid == 0) S.x_mass[C.phase & 1][0] = z;
   } else {
-    C.first([&](int v, const float *f) {
+    C.span.template walk<true>([&](int v, const float *f) {
       float x = f[0];
 #pragma unroll
       for (int i = 1; i < kVec; ++i) x = fmaxf(x, f[i]);
@@ -1039,6 +1235,8 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
       }
     });
     m = mt;
+  }
+  if (!all) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   }
@@ -1046,8 +1244,8 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
     S.warp_f[warp] = m;
     S.warp_bad[warp] = bad;
   }
-  if (nucleus)
-    smp_band_sums<true, false>(C);
+  if (fast)
+    smp_count_list(C);
   else
     cl.sync();
   bad = 0;
@@ -1075,11 +1273,11 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
     __syncthreads();
     if (mt == m) {
       float f[kVec];
-      C.row.unpack(C.row.raw(first), f);
+      C.span.row.unpack(C.span.row.raw(first), f);
       int col = 0x7FFFFFFF;
 #pragma unroll
       for (int i = kVec - 1; i >= 0; --i)
-        if (f[i] == m) col = C.row.column(first) + i;
+        if (f[i] == m) col = C.span.row.column(first) + i;
       atomicMin(&S.best, col);
     }
     cl.sync();
@@ -1098,11 +1296,10 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
     w = SmpMass(m < INFINITY ? m : 0.f, T);
   }
   double tie_w = 1.0;
-  bool drawn = false;
   if (m == INFINITY) {
     // the +inf entries are equal and have all the mass: every filter counts
     int cnt = 0;
-    C.each([&](int, const float *f) {
+    C.span.template walk<false>([&](int, const float *f) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i) cnt += f[i] == INFINITY;
     });
@@ -1117,6 +1314,36 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
   } else if (!all) {
     if (use_m) cut.key = smp_min_key(m, T, fminf(mp, 1.f)) - 1u;
     const float xb = smp_float(cut.key);  // the base: logits above
+    const bool whole = xb >= fast_lo;     // the list holds all of it
+    const unsigned long long listed = fast ? S.sum_cnt[0] : 0ull;
+    if (listed > 0 && listed <= (unsigned long long)kSmpList &&
+        (whole || nucleus || (use_k && listed >= (unsigned long long)k))) {
+      const double z_row = S.sum_mass[0];
+      const bool known = whole || !nucleus;
+      smp_gather(C);
+      if (rank != 0 && known) return;
+      if (rank == 0) {
+        // a row's mass known to a factor of 1 +- kSmpSlack is enough, unless the
+        // cut falls between the two
+        double target = -1.0, most = 0.0;
+        bool sure = false;
+        if (!known) {
+          target = (double)p * z_row * exp2((double)ref * w.c - w.k0);
+          most = target * (1.0 + kSmpSlack);
+          target *= 1.0 - kSmpSlack;
+        }
+        const SmpPick pick = smp_pick(S, w, (int)listed, cut.key, use_k ? k : 0,
+                                      use_p ? (double)p : 1.0, target, 0.0, most, &sure);
+        sure = known || (sure && !w.held && target >= 0.0);
+        if (tid == 0) S.verdict = sure;
+        if (sure) smp_draw_list<E>(S, a, w, r, (int)listed, pick, u);
+        if (known) return;
+      }
+      cl.sync();
+      const int ok = cl.map_shared_rank(&S, 0)->verdict;
+      cl.sync();
+      if (ok) return;
+    }
     // What is tried next: the list of the candidates of a top-k or min-p, a
     // split of the band with the cut, the list of a band's whole prefix, the
     // list of a band, the cut key by key; kRow: the cut is known.
@@ -1124,7 +1351,6 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
     float lo = xb, hi = m;
     SmpBands bands{xb, m, 0.f, 1.f / kSmpBand0};
     int level = 0;
-    bool summed = nucleus && !bad;  // the first bands' masses are known
     double target = 0.0, above = 0.0, in_band = 0.0;
     float band_lo = xb, band_hi = m, band_d0 = 0.f, band_d1 = 0.f;
     if (!nucleus && (!use_k || k <= kSmpMaxK)) {
@@ -1164,11 +1390,11 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
           next = kKeys;
           continue;
         }
-        if (!summed) {
-          smp_bands<false>(C, w, bands);
-          smp_band_sums<true, false>(C);
-        }
-        summed = false;
+        if (level == 0)
+          smp_bands<true>(C.span, w, bands, &S.band.mass[0][tid]);
+        else
+          smp_bands<false>(C.span, w, bands, &S.band.mass[0][tid]);
+        smp_band_sums<true, false>(C);
         if (level == 0) {
           for (int i = 0; i < kSmpBands; ++i) target += S.sum_mass[i];
           target *= (double)p;
@@ -1228,37 +1454,15 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
         continue;
       }
       if (rank == 0) {
-        double wt[kSmpPer], z;
-        double run = smp_sort_list(C, w, got, wt, &z);
-        int keep = got;
-        if (next == kList) {
-          if (use_k) keep = (int)min(k, (long long)got);
-          if (use_p && keep < got) {  // mass of the first `keep`
-            double part = 0.0;
-#pragma unroll
-            for (int i = 0; i < kSmpPer; ++i) part += tid * kSmpPer + i < keep ? wt[i] : 0.0;
-            smp_scan(S, part, &z);
-          }
-          target = (double)p * z;
-        }
-        if (next == kBand) run += above;
-        if (use_p) keep = smp_reach(S, wt, run, target, keep);
+        const SmpPick pick =
+            smp_pick(S, w, got, cut.key, use_k ? k : 0, use_p ? (double)p : 1.0,
+                     next == kList ? -1.0 : target, next == kBand ? above : 0.0, 0.0, nullptr);
         if (next != kBand) {
-          smp_draw_list<E>(C, a, r, keep, u);
-        } else {
-          // the cut lies among these: the key and the ties of its last entry
-          const uint32_t key = (uint32_t)(S.list.item[keep - 1] >> 32);
-          int same = 0, ties;
-#pragma unroll
-          for (int i = 0; i < kSmpPer; ++i) {
-            const int at = tid * kSmpPer + i;
-            same += at < keep && (uint32_t)(S.list.item[at] >> 32) == key;
-          }
-          (void)smp_count_scan(S, same, &ties);
-          if (tid == 0) {
-            S.cut_key = key;
-            S.cut_ties = ties;
-          }
+          smp_draw_list<E>(S, a, w, r, got, pick, u);
+        } else if (tid == 0) {
+          // the cut lies among these
+          S.cut_key = pick.key;
+          S.cut_ties = pick.ties;
         }
       }
       if (next == kBand) {
@@ -1267,23 +1471,21 @@ __global__ void __launch_bounds__(kSmpThreads, kSmpResident) k_sample(SampleArgs
         cut.key = (uint32_t)R->cut_key;
         cut.ties = R->cut_ties;
       } else {
-        drawn = true;
+        return;  // drawn; nothing of another CTA is read any more
       }
       next = kRow;
     }
     bad = 1;
     if (cut.ties > 0) tie_w = w(unmono(cut.key));
   }
-  if (!drawn) {
-    if (bad) {  // the segments' masses are not known yet
-      if (cut.ties > 0)
-        smp_segment<true>(C, w, cut);
-      else
-        smp_segment<false>(C, w, cut);
-      cl.sync();
-    }
-    smp_draw_row<E>(C, a, w, cut, tie_w, r, u);
+  if (bad) {  // the segments' masses are not known yet
+    if (cut.ties > 0)
+      smp_segment<false, true>(C, w, cut);
+    else
+      smp_segment<false, false>(C, w, cut);
+    cl.sync();
   }
+  smp_draw_row<E>(C, a, w, cut, tie_w, r, u);
   cl.sync();
 }
 
