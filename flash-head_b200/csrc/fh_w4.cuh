@@ -7,14 +7,14 @@
 // 16 bits.
 //
 // Layout (made once by the loader, flash_head/w4.py). Rows come in tiles of
-// 16, columns in blocks of 128 (both padded; padding has scale 0):
-//   qweight u32 [tile][block][16 rows][4 quads][4 words]: word j of quad c
+// 128, columns in blocks of 128 (both padded; padding has scale 0):
+//   qweight u32 [tile][block][128 rows][4 quads][4 words]: word j of quad c
 //           holds columns 128 * block + 32 * j + 8 * c + e, e = 0..7, column
 //           e = 2i in bits 4i..4i+3 and e = 2i+1 in bits 16+4i..19+4i.
-//   scales  16-bit [tile][block][16 rows][groups per block]
+//   scales  16-bit [tile][block][128 rows][groups per block]
 //   zeros   u8, same shape (absent: every zero point is 8)
-// One 16-row x 128-column block is 1 KB, contiguous: lane (g, c) of a warp
-// reads 16 bytes of row g and 16 of row g + 8, each a full line per quad row.
+// One tile's block is 8 KB, contiguous (one bulk copy), and 16 of its rows are
+// 1 KB: lane (g, c) of a warp reads 16 bytes of row g and 16 of row g + 8.
 // The nibble order makes (w >> 4i) & 0x000F000F a pair of neighbouring
 // columns, i.e. one operand register of mma.m16n8k16 (A: 16 weight rows), and
 // the 8 columns of a word are 16 contiguous bytes of a hidden row (B), so
@@ -27,7 +27,8 @@ namespace fh {
 
 constexpr int kW4Warps = 16;
 constexpr int kW4Block = 128;                   // columns per block
-constexpr int kW4TileWords = 16 * kW4Block / 8;  // u32 of one tile's block
+constexpr int kW4Tile = 128;                     // rows per tile
+constexpr int kW4RowWords = kW4Block / 8;        // u32 of one row's block
 
 struct W4Args {
   const uint32_t *qw;
@@ -36,7 +37,7 @@ struct W4Args {
   int V;        // weight rows
   int D;        // columns
   int nb;       // 128-column blocks: ceil(D / 128)
-  int tiles;    // 16-row tiles (padded: a multiple of 8)
+  int tiles;    // 128-row tiles: ceil(V / 128)
   const void *hidden;  // [rows, D]
   int rows;
   void *out;    // [rows, ldo]
@@ -130,20 +131,22 @@ struct W4Frag {
 };
 
 template <int GPK, bool ZP>
-__device__ __forceinline__ void w4_load(const W4Args &a, long long blk, int r0, int r1, int c,
+__device__ __forceinline__ void w4_load(const W4Args &a, int kb, int r0, int r1, int c,
                                         W4Frag<GPK, ZP> &f) {
   using S = typename W4Group<GPK>::S;
   using Z = typename W4Group<GPK>::Z;
-  const uint32_t *q = a.qw + blk * kW4TileWords + c * 4;
-  f.q[0] = ldg_stream(q + r0 * 16);
-  f.q[1] = ldg_stream(q + r1 * 16);
-  const S *s = reinterpret_cast<const S *>(a.scales) + blk * 16;
-  f.s[0] = __ldg(s + r0);
-  f.s[1] = __ldg(s + r1);
+  // row of the [tile][block][row] order
+  const long long i0 = ((long long)(r0 >> 7) * a.nb + kb) * kW4Tile + (r0 & 127);
+  const long long i1 = ((long long)(r1 >> 7) * a.nb + kb) * kW4Tile + (r1 & 127);
+  f.q[0] = ldg_stream(a.qw + i0 * kW4RowWords + c * 4);
+  f.q[1] = ldg_stream(a.qw + i1 * kW4RowWords + c * 4);
+  const S *s = reinterpret_cast<const S *>(a.scales);
+  f.s[0] = __ldg(s + i0);
+  f.s[1] = __ldg(s + i1);
   if (ZP) {
-    const Z *z = reinterpret_cast<const Z *>(a.zeros) + blk * 16;
-    f.z[0] = __ldg(z + r0);
-    f.z[1] = __ldg(z + r1);
+    const Z *z = reinterpret_cast<const Z *>(a.zeros);
+    f.z[0] = __ldg(z + i0);
+    f.z[1] = __ldg(z + i1);
   }
 }
 
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
 
   const int ks = a.ksplit, kw = warp % ks;
   const int team = warp / ks, teams = kW4Warps / ks;
-  const int units = a.tiles / 2;
+  const int units = a.tiles * (kW4Tile / 32);
   const int per_round = teams * gridDim.x;
   const int my_nb = (a.nb - kw + ks - 1) / ks;  // blocks of this warp
   const int rounds = (units + per_round - 1) / per_round;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
         W4Frag<GPK, ZP> f[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          w4_load<GPK, ZP>(a, (long long)(2 * u + t) * a.nb + kb, g, g + 8, c, f[t]);
+          w4_load<GPK, ZP>(a, kb, 32 * u + 16 * t + g, 32 * u + 16 * t + g + 8, c, f[t]);
         const unsigned char *hk = hl + kb * (kW4Block * 2);
         auto load = [&](int n, int j) { return lds128(hk + (size_t)(8 * n) * rb + j * 64); };
 #pragma unroll
@@ -339,18 +342,7 @@ __global__ void __launch_bounds__(32 * kW4ProbeWarps) k_w4_probes(W4Args a) {
   float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
   for (int kb = warp; kb < a.nb; kb += kW4ProbeWarps) {
     W4Frag<GPK, ZP> f;
-    const long long b0 = (long long)(wr[0] >> 4) * a.nb + kb;
-    const long long b1 = (long long)(wr[1] >> 4) * a.nb + kb;
-    using S = typename W4Group<GPK>::S;
-    using Z = typename W4Group<GPK>::Z;
-    f.q[0] = ldg_stream(a.qw + b0 * kW4TileWords + (wr[0] & 15) * 16 + c * 4);
-    f.q[1] = ldg_stream(a.qw + b1 * kW4TileWords + (wr[1] & 15) * 16 + c * 4);
-    f.s[0] = __ldg(reinterpret_cast<const S *>(a.scales) + b0 * 16 + (wr[0] & 15));
-    f.s[1] = __ldg(reinterpret_cast<const S *>(a.scales) + b1 * 16 + (wr[1] & 15));
-    if (ZP) {
-      f.z[0] = __ldg(reinterpret_cast<const Z *>(a.zeros) + b0 * 16 + (wr[0] & 15));
-      f.z[1] = __ldg(reinterpret_cast<const Z *>(a.zeros) + b1 * 16 + (wr[1] & 15));
-    }
+    w4_load<GPK, ZP>(a, kb, wr[0], wr[1], c, f);
     // one hidden row: column n = 0 of B, the other 7 are zero
     auto load = [&](int, int j) {
       const int x = kb * 16 + j * 4 + c;

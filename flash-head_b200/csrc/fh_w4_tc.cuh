@@ -1,0 +1,429 @@
+// Logits of a 4-bit head for many rows on the 5th-generation tensor cores:
+// out[b, v] = sum_k w[v, k] h[b, k], M = 128 weight rows, N = up to 256 hidden
+// rows per launch.
+//
+// The weight's integers become f16 operands in shared memory: q - z is exact,
+// and its product with the group's scale is rounded to f16 once, 2^-11 relative
+// (a bf16 scale times a 4-bit integer has at most one bit more than f16 holds).
+// That is an eighth of a bf16 output's own rounding; applying the scales to
+// fp32 sums instead, as k_w4_mv does, would read every accumulator back once
+// per group. Rows of scales are brought to [1, 2) by an exact power of two
+// (row_mul), undone in the epilogue, so that no weight leaves f16's range. bf16
+// hidden rows are copied to f16 first, each scaled by a power of two likewise
+// (k_w4_hidden); f16 ones are read as they are.
+//
+// One persistent CTA per SM, 14 warps:
+//   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and
+//               zero points of 128 rows x 128 columns: two or three bulk copies)
+//               into a ring of their own, deep enough to keep HBM busy, and the
+//               hidden tile of every 64 columns (TMA, 128-byte swizzle) into
+//               the stages;
+//   warp 1      allocates TMEM; lane 0 issues tcgen05.mma (K = 16) per stage;
+//   warps 2-9   unpack: a thread takes 32 columns of two rows per block and
+//               writes 16-byte pieces of the swizzled A tile. Lanes cover rows
+//               p and p ^ 5 together: neither their reads (rows of 64 bytes)
+//               nor their writes (rows of 128, pieces exchanged by row) meet in
+//               a bank;
+//   warps 10-13 epilogue: a thread has one weight row and all hidden rows; the
+//               accumulators are double-buffered.
+// Bounds: HBM (the packed weight) up to about 64 rows, the tensor cores and
+// the hidden tiles' way from L2 at 256.
+// Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
+// drains its own copies and MMAs (bounded) and frees TMEM before it returns.
+#pragma once
+
+#include "fh_s1_tc.cuh"
+#include "fh_w4.cuh"
+
+namespace fh {
+
+constexpr int kW4tThreads = 448;
+constexpr int kW4tConvWarps = 8;
+constexpr int kW4tEpiWarps = 4;
+constexpr int kW4tMaxN = 256;
+constexpr int kW4tMaxStages = 6;
+constexpr int kW4tMaxPacked = 12;
+constexpr int kW4tABytes = 128 * 128;  // 128 rows x 64 columns f16
+constexpr int kW4tSmemMax = 227 * 1024;
+
+struct W4TcArgs {
+  const uint32_t *qw;
+  const void *scales;
+  const uint8_t *zeros;
+  const float *row_mul;   // [128 * tiles] powers of two
+  const float *row_fac;   // [rows] factors of the hidden rows, or null
+  int V, nb, nk;          // nk: 64-column stages, ceil(D / 64)
+  int tiles;
+  int rows, n_pad;
+  int stages, packed, n_acc;
+  int tmem_cols;
+  uint32_t idesc;
+  void *out;
+  long long ldo;
+  uint32_t *err;
+  uint32_t polls;
+};
+
+struct W4TcCtrl {
+  uint64_t full[kW4tMaxStages];    // hidden tile landed
+  uint64_t conv[kW4tMaxStages];    // A tile written
+  uint64_t empty[kW4tMaxStages];   // MMAs done
+  uint64_t pfull[kW4tMaxPacked];   // packed block landed
+  uint64_t pempty[kW4tMaxPacked];  // packed block unpacked
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  uint32_t s_err;
+  float fac[kW4tMaxN];
+};
+
+__host__ __device__ inline int w4t_packed_bytes(int gpk, bool zp) {
+  return kW4Tile * kW4RowWords * 4 + kW4Tile * gpk * (zp ? 3 : 2);
+}
+__host__ __device__ inline size_t w4t_stage_bytes(int n_pad) {
+  return (size_t)kW4tABytes + (size_t)n_pad * 128;
+}
+__host__ __device__ inline size_t w4t_smem_bytes(int n_pad, int stages, int packed, int gpk, bool zp) {
+  return 1024 + stages * w4t_stage_bytes(n_pad) + (size_t)packed * w4t_packed_bytes(gpk, zp) +
+         sizeof(W4TcCtrl);
+}
+
+// f16 copy of bf16 hidden rows, one CTA per row: the row's largest finite
+// magnitude is brought to [2^14, 2^15) by a power of two whose inverse goes to
+// fac. Infinities and NaN stay. Also clears the error word.
+__global__ void __launch_bounds__(256)
+    k_w4_hidden(const uint4 *h, uint4 *out, float *fac, int chunks, uint32_t *err) {
+  __shared__ uint32_t top[8];
+  grid_dep_launch();
+  const uint4 *src = h + (size_t)blockIdx.x * chunks;
+  uint32_t m = 0u;  // largest finite magnitude, bf16 bits
+  for (int i = threadIdx.x; i < chunks; i += 256) {
+    const uint4 v = src[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = w[j] & 0x7FFFu, hi = (w[j] >> 16) & 0x7FFFu;
+      if (lo < 0x7F80u) m = max(m, lo);
+      if (hi < 0x7F80u) m = max(m, hi);
+    }
+  }
+  m = __reduce_max_sync(0xFFFFFFFFu, m);
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, top[i]);
+  // exponent of the largest value (a zero or subnormal row counts as 2^-126)
+  const int e = max((int)(m >> 7), 1) - 127;
+  // 2^(14 - e) in two factors: it may pass the largest fp32
+  const int s0 = (14 - e) / 2, s1 = 14 - e - s0;
+  const float f0 = __uint_as_float((uint32_t)(127 + s0) << 23);
+  const float f1 = __uint_as_float((uint32_t)(127 + s1) << 23);
+  uint4 *dst = out + (size_t)blockIdx.x * chunks;
+  for (int i = threadIdx.x; i < chunks; i += 256) {
+    const uint4 v = src[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = __uint_as_float(w[j] << 16) * f0 * f1;
+      const float hi = __uint_as_float(w[j] & 0xFFFF0000u) * f0 * f1;
+      const __half2 x = __floats2half2_rn(lo, hi);
+      o[j] = *reinterpret_cast<const uint32_t *>(&x);
+    }
+    dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  if (threadIdx.x == 0) {
+    // the inverse, 2^(e - 14): may be subnormal as one factor, never zero
+    fac[blockIdx.x] = ldexpf(1.f, e - 14);
+    if (blockIdx.x == 0) *err = 0u;
+  }
+}
+
+// T: type of the scales and outputs. GPK, ZP as in k_w4_mv.
+template <typename T, int GPK, bool ZP>
+__global__ void __launch_bounds__(kW4tThreads, 1)
+    k_w4_tc(const __grid_constant__ CUtensorMap tm_h, W4TcArgs a) {
+  extern __shared__ __align__(1024) unsigned char w4t_sm[];
+  const uint32_t raw = smem_u32(w4t_sm);
+  unsigned char *ring = w4t_sm + (((raw + 1023u) & ~1023u) - raw);
+  const size_t sb = w4t_stage_bytes(a.n_pad);
+  unsigned char *pring = ring + (size_t)a.stages * sb;
+  constexpr int kWords = kW4Tile * kW4RowWords * 4;  // bytes of packed words
+  constexpr int kScales = kW4Tile * GPK * 2, kZeros = ZP ? kW4Tile * GPK : 0;
+  constexpr int pb = kWords + kScales + kZeros;
+  W4TcCtrl &S = *reinterpret_cast<W4TcCtrl *>(pring + (size_t)a.packed * pb);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = gridDim.x, t0 = blockIdx.x;
+
+  if (tid == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&S.full[s], 1);
+      mbar_init(&S.conv[s], kW4tConvWarps);
+      mbar_init(&S.empty[s], 1);
+    }
+    for (int s = 0; s < a.packed; ++s) {
+      mbar_init(&S.pfull[s], 1);
+      mbar_init(&S.pempty[s], kW4tConvWarps);
+    }
+    for (int j = 0; j < 2; ++j) {
+      mbar_init(&S.acc_full[j], 1);
+      mbar_init(&S.acc_empty[j], kW4tEpiWarps);
+    }
+    mbar_init(&S.drain, 1);
+    S.s_err = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&S.tmem_base)),
+                 "r"(a.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // packed blocks run ahead of the hidden tiles by the depth of their ring
+      int issued_s[kW4tMaxStages], issued_p[kW4tMaxPacked];  // parity of the last fill, -1: none
+      for (int j = 0; j < kW4tMaxStages; ++j) issued_s[j] = -1;
+      for (int j = 0; j < kW4tMaxPacked; ++j) issued_p[j] = -1;
+      int pt = t0, pkb = 0, ps = 0, s = 0;
+      uint32_t pph = 0u, ph = 0u;
+      bool ok = true, waited = false;
+      auto fill_packed = [&]() {  // false: its slot is not free yet
+        if (pt >= a.tiles) return true;
+        if (!mbar_try_wait(&S.pempty[ps], pph ^ 1u)) return false;
+        unsigned char *p = pring + (size_t)ps * pb;
+        const size_t blk = (size_t)pt * a.nb + pkb;
+        mbar_expect_tx(&S.pfull[ps], (uint32_t)pb);
+        bulk_g2s(p, reinterpret_cast<const unsigned char *>(a.qw) + blk * kWords, kWords,
+                 &S.pfull[ps]);
+        bulk_g2s(p + kWords, reinterpret_cast<const unsigned char *>(a.scales) + blk * kScales,
+                 kScales, &S.pfull[ps]);
+        if (ZP) bulk_g2s(p + kWords + kScales, a.zeros + blk * kZeros, kZeros, &S.pfull[ps]);
+        issued_p[ps] = (int)pph;
+        if (++ps == a.packed) {
+          ps = 0;
+          pph ^= 1u;
+        }
+        if (++pkb == a.nb) {
+          pkb = 0;
+          pt += G;
+        }
+        return true;
+      };
+      for (int i = 0; i < a.packed; ++i) fill_packed();
+      for (int t = t0; t < a.tiles && ok; t += G) {
+        for (int k = 0; k < a.nk && ok; ++k) {
+          // the stage's hidden tile; meanwhile packed slots that come free
+          bool free = false;
+          for (uint32_t i = 0; i < a.polls && !free; ++i) {
+            fill_packed();
+            free = mbar_try_wait(&S.empty[s], ph ^ 1u);
+          }
+          if (!free) {
+            atomicOr(&S.s_err, kErrCopyTimeout);
+            ok = false;
+            break;
+          }
+          if (!waited) {  // the f16 copy of the hidden rows
+            grid_dep_wait();
+            waited = true;
+          }
+          mbar_expect_tx(&S.full[s], (uint32_t)(a.n_pad * 128));
+          tma_load_2d(ring + (size_t)s * sb + kW4tABytes, &tm_h, k * 64, 0, &S.full[s]);
+          issued_s[s] = (int)ph;
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // blocks whose slots were still taken
+      for (uint32_t i = 0; i < a.polls && ok && pt < a.tiles; ++i) fill_packed();
+      if (ok && pt < a.tiles) atomicOr(&S.s_err, kErrCopyTimeout);
+      // every copy this thread issued has landed before the CTA may leave
+      for (int j = 0; j < a.packed; ++j)
+        if (issued_p[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued_p[j], a.polls))
+          atomicOr(&S.s_err, kErrCopyTimeout);
+      for (int j = 0; j < a.stages; ++j)
+        if (issued_s[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued_s[j], a.polls))
+          atomicOr(&S.s_err, kErrCopyTimeout);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0u;
+      bool ok = true;
+      for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
+        const int buf = i % a.n_acc, use = i / a.n_acc;
+        if (use > 0) {
+          if (!mbar_wait(&S.acc_empty[buf], (uint32_t)((use - 1) & 1), a.polls)) {
+            atomicOr(&S.s_err, kErrCopyTimeout);
+            break;
+          }
+          tc_fence_after();
+        }
+        const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
+        for (int k = 0; k < a.nk; ++k) {
+          if (!mbar_wait(&S.full[s], ph, a.polls) || !mbar_wait(&S.conv[s], ph, a.polls)) {
+            atomicOr(&S.s_err, kErrCopyTimeout);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(ring + (size_t)s * sb);
+          const uint64_t ad = umma_desc_k(st);
+          const uint64_t bd = umma_desc_k(st + (uint32_t)kW4tABytes);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            tc_mma_f16(acc, ad + 2u * q, bd + 2u * q, a.idesc, (k | q) != 0 ? 1u : 0u);
+          tc_commit(&S.empty[s]);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) tc_commit(&S.acc_full[buf]);
+      }
+      tc_commit(&S.drain);
+      if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
+    }
+  } else if (warp < 2 + kW4tConvWarps) {
+    const int c = lane & 3, p = lane >> 3;
+    const int m0 = 8 * (warp - 2) + ((lane & 4) ? p ^ 5 : p);  // rows m0, m0 + 64
+    int s = 0, ps = 0;
+    uint32_t ph = 0u, pph = 0u;
+    bool ok = true;
+    for (int t = t0; t < a.tiles && ok; t += G) {
+      const float mul[2] = {__ldg(a.row_mul + t * kW4Tile + m0),
+                            __ldg(a.row_mul + t * kW4Tile + m0 + 64)};
+      for (int kb = 0; kb < a.nb && ok; ++kb) {
+        if (!mbar_wait(&S.pfull[ps], pph, a.polls)) {
+          atomicOr(&S.s_err, kErrCopyTimeout);
+          ok = false;
+          break;
+        }
+        const unsigned char *pk = pring + (size_t)ps * pb;
+        uint4 q[2];
+        uint32_t sc[2][GPK], zz[2][GPK];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = m0 + 64 * i;
+          q[i] = lds128(pk + m * 64 + c * 16);
+#pragma unroll
+          for (int g = 0; g < GPK; ++g) {
+            const uint16_t bits =
+                reinterpret_cast<const uint16_t *>(pk + kWords)[m * GPK + g];
+            const __half2 h = __float2half2_rn(W4Num<T>::scale(bits) * mul[i]);
+            sc[i][g] = *reinterpret_cast<const uint32_t *>(&h);
+            const uint32_t z = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
+            zz[i][g] = W4Num<__half>::kMagic | (z * 0x00010001u);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cta(&S.pempty[ps]);
+        if (++ps == a.packed) {
+          ps = 0;
+          pph ^= 1u;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (2 * kb + h >= a.nk) break;
+          if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
+            atomicOr(&S.s_err, kErrCopyTimeout);
+            ok = false;
+            break;
+          }
+          unsigned char *at = ring + (size_t)s * sb;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int m = m0 + 64 * i;
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+              const int j = 2 * h + jj, g = j * GPK / 4;
+              const uint32_t w = j == 0 ? q[i].x : j == 1 ? q[i].y : j == 2 ? q[i].z : q[i].w;
+              uint32_t x[4];
+              w4_unpack<__half>(w, zz[i][g], x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&x[e]),
+                                          *reinterpret_cast<const __half2 *>(&sc[i][g]));
+                x[e] = *reinterpret_cast<const uint32_t *>(&y);
+              }
+              *reinterpret_cast<uint4 *>(at + m * 128 + (((c + 4 * jj) ^ (m & 7)) << 4)) =
+                  make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          // generic-proxy writes of the tile become visible to the MMA
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cta(&S.conv[s]);
+          if (++s == a.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3;  // TMEM lane quadrant of this warp
+    const int et = tid - 32 * (2 + kW4tConvWarps);
+    grid_dep_wait();
+    for (int i = et; i < kW4tMaxN; i += 32 * kW4tEpiWarps)
+      S.fac[i] = a.row_fac && i < a.rows ? a.row_fac[i] : 1.f;
+    nbar_sync(1, 32 * kW4tEpiWarps);
+    bool ok = true;
+    for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
+      const int buf = i % a.n_acc, use = i / a.n_acc;
+      if (!mbar_wait(&S.acc_full[buf], (uint32_t)(use & 1), a.polls)) {
+        atomicOr(&S.s_err, kErrCopyTimeout);
+        ok = false;
+      }
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int v = t * kW4Tile + 32 * q + lane;
+      const float back = 1.f / __ldg(a.row_mul + v);  // a power of two
+      T *out = reinterpret_cast<T *>(a.out) + v;
+      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * a.n_pad);
+      for (int c = 0; c < a.n_pad; c += 32) {
+        uint32_t x[2][16];
+        tc_ld16(base + (uint32_t)c, x[0]);
+        if (c + 16 < a.n_pad) tc_ld16(base + (uint32_t)(c + 16), x[1]);
+        tc_wait_ld();
+        if (v < a.V) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int r = c + 16 * u + j;
+              if (r < a.rows)
+                out[(long long)r * a.ldo] =
+                    from_float<T>(__uint_as_float(x[u][j]) * back * S.fac[r]);
+            }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cta(&S.acc_empty[buf]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(a.tmem_cols)
+                 : "memory");
+  }
+  if (tid == 0 && S.s_err) atomicOr(a.err, S.s_err);
+}
+
+}  // namespace fh

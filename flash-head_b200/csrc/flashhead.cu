@@ -28,6 +28,7 @@
 #include "fh_spec.cuh"
 #include "fh_sample.cuh"
 #include "fh_w4.cuh"
+#include "fh_w4_tc.cuh"
 
 static_assert(fh::kS2MaskWords == 8, "the selection kernel writes 8 bit-map words per cluster");
 
@@ -1749,7 +1750,7 @@ static int check_w4(const fh_w4_desc *d, const void *hidden, int rows, const voi
   if (d->dtype != FH_BF16 && d->dtype != FH_FP16)
     return fail(FH_ERR_INVALID_ARGUMENT, "dtype must be FH_BF16 or FH_FP16");
   if (rows == 0) return FH_OK;
-  if (!d->qweight || !d->scales || !hidden || !out)
+  if (!d->qweight || !d->scales || !d->row_mul || !hidden || !out)
     return fail(FH_ERR_INVALID_ARGUMENT, "null pointer argument");
   if (!aligned16(d->qweight) || !aligned16(d->scales) || !aligned16(d->zeros) ||
       !aligned16(hidden))
@@ -1769,7 +1770,7 @@ static fh::W4Args w4_args(const fh_w4_desc *d, const void *hidden, int rows, voi
   a.V = d->vocab;
   a.D = d->hidden;
   a.nb = (d->hidden + fh::kW4Block - 1) / fh::kW4Block;
-  a.tiles = (d->vocab + 127) / 128 * 8;
+  a.tiles = (d->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
   a.hidden = hidden;
   a.rows = rows;
   a.out = out;
@@ -1789,18 +1790,22 @@ static cudaError_t launch_w4_mv_t(const fh::W4Args &a, int grid, cudaStream_t s)
 }
 
 template <typename T, int GPK, bool ZP>
-static cudaError_t launch_w4_mv_n(const fh::W4Args &a, int nt, int grid, cudaStream_t s) {
-  return nt == 1 ? launch_w4_mv_t<T, GPK, ZP, 1>(a, grid, s)
-                 : launch_w4_mv_t<T, GPK, ZP, 2>(a, grid, s);
-}
-
-template <typename T, int GPK, bool ZP>
 static cudaError_t launch_w4_probes_t(const fh::W4Args &a, unsigned grid, cudaStream_t s) {
   return launch(fh::k_w4_probes<T, GPK, ZP>, dim3(grid), dim3(32 * fh::kW4ProbeWarps), 0, s, false,
                 a);
 }
 
-// Calls f.template operator()<T, groups per block, zero points>() for a descriptor.
+template <typename T, int GPK, bool ZP>
+static cudaError_t launch_w4_tc_t(const CUtensorMap &tm, const fh::W4TcArgs &a, int grid,
+                                  size_t smem, bool pdl, cudaStream_t s) {
+  static bool done[128];
+  auto kern = fh::k_w4_tc<T, GPK, ZP>;
+  const cudaError_t e = raise_smem(kern, fh::kW4tSmemMax, done);
+  if (e != cudaSuccess) return e;
+  return launch(kern, dim3(grid), dim3(fh::kW4tThreads), smem, s, pdl, tm, a);
+}
+
+// Calls f(T *, groups per block, zero points) for a descriptor.
 template <typename F>
 static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
   const int gpk = fh::kW4Block / d->group_size;
@@ -1821,10 +1826,102 @@ static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
 
 extern "C" {
 
+// Rows of a call that go through k_w4_mv (mma.sync, 8 rows per pass of the
+// weight); more run on the tensor-core kernel.
+constexpr int kW4MvRows = 8;
+
 FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows) {
-  (void)desc;
-  (void)rows;
-  return 0;
+  if (!desc || rows <= kW4MvRows) return 0;
+  size_t n = 256;
+  if (desc->dtype == FH_BF16)  // factors and the f16 copy of the hidden rows
+    n += round_up((size_t)rows * sizeof(float), 256) + (size_t)rows * desc->hidden * 2;
+  return n;
+}
+
+static int run_w4_mv(const fh_w4_desc *desc, fh::W4Args a, int sms, cudaStream_t s) {
+  // few units: the 16 warps of a CTA share units so that every SM has work
+  const int units = a.tiles * (fh::kW4Tile / 32);
+  a.ksplit = 1;
+  while (a.ksplit < fh::kW4Warps && a.ksplit * 2 <= a.nb &&
+         (long long)units * a.ksplit < 2ll * sms * fh::kW4Warps)
+    a.ksplit *= 2;
+  const int teams = fh::kW4Warps / a.ksplit;
+  const int grid = std::min(sms, (units + teams - 1) / teams);
+  const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto gpk, auto zp) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return launch_w4_mv_t<T, decltype(gpk)::value, decltype(zp)::value, 1>(a, grid, s);
+  });
+  FH_CHECK_LAUNCH(e, "4-bit logits launch");
+  return FH_OK;
+}
+
+static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void *out,
+                     int64_t out_stride, void *workspace, size_t workspace_bytes, int sms,
+                     cudaStream_t s) {
+  if (!workspace || workspace_bytes < fh_w4_workspace_bytes(desc, rows))
+    return fail(FH_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu",
+                fh_w4_workspace_bytes(desc, rows), workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace))
+    return fail(FH_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+  unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
+  const int D = desc->hidden, gpk = fh::kW4Block / desc->group_size;
+  const bool zp = desc->zeros != nullptr;
+  fh::W4TcArgs a;
+  memset(&a, 0, sizeof(a));
+  a.qw = desc->qweight;
+  a.scales = desc->scales;
+  a.zeros = desc->zeros;
+  a.row_mul = desc->row_mul;
+  a.V = desc->vocab;
+  a.nb = (D + fh::kW4Block - 1) / fh::kW4Block;
+  a.nk = (D + 63) / 64;
+  a.tiles = (desc->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
+  a.ldo = out_stride;
+  a.err = reinterpret_cast<uint32_t *>(ws);
+  a.polls = 1u << 22;
+  const void *hop = hidden;
+  float *fac = nullptr;
+  bool pdl = false;
+  if (desc->dtype == FH_BF16) {
+    fac = reinterpret_cast<float *>(ws + 256);
+    uint4 *h16 = reinterpret_cast<uint4 *>(ws + 256 + round_up((size_t)rows * sizeof(float), 256));
+    FH_CHECK_LAUNCH(launch(fh::k_w4_hidden, dim3(rows), dim3(256), 0, s, false,
+                           reinterpret_cast<const uint4 *>(hidden), h16, fac, D / 8, a.err),
+                    "hidden f16 copy launch");
+    hop = h16;
+    pdl = true;
+  } else {
+    FH_CHECK_LAUNCH(cudaMemsetAsync(ws, 0, sizeof(uint32_t), s), "error word reset");
+  }
+  for (int r0 = 0; r0 < rows; r0 += fh::kW4tMaxN) {
+    const int n = std::min(fh::kW4tMaxN, rows - r0);
+    a.rows = n;
+    a.n_pad = (n + 15) / 16 * 16;
+    a.n_acc = 2;
+    a.tmem_cols = 32;
+    while (a.tmem_cols < 2 * a.n_pad) a.tmem_cols *= 2;
+    a.idesc = fh::s1tc_idesc(false, a.n_pad);
+    a.row_fac = fac ? fac + r0 : nullptr;
+    a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
+    // stages of 64 columns; the rest of shared memory is the packed ring
+    a.stages = a.n_pad <= 128 ? 4 : 3;
+    const size_t used = 1024 + sizeof(fh::W4TcCtrl) + a.stages * fh::w4t_stage_bytes(a.n_pad);
+    a.packed = (int)std::min<size_t>(fh::kW4tMaxPacked, ((size_t)fh::kW4tSmemMax - used) /
+                                                            fh::w4t_packed_bytes(gpk, zp));
+    const size_t smem = fh::w4t_smem_bytes(a.n_pad, a.stages, a.packed, gpk, zp);
+    CUtensorMap tm;
+    if (!encode_rows_map(&tm, reinterpret_cast<const char *>(hop) + (size_t)r0 * D * 2, FH_FP16, D,
+                         n, a.n_pad))
+      return fail(FH_ERR_UNSUPPORTED, "hidden-state tensor map");
+    const int grid = std::min(sms, a.tiles);
+    const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto g, auto z) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      return launch_w4_tc_t<T, decltype(g)::value, decltype(z)::value>(tm, a, grid, smem, pdl, s);
+    });
+    FH_CHECK_LAUNCH(e, "4-bit tensor-core launch");
+    pdl = false;
+  }
+  return FH_OK;
 }
 
 FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows, void *out,
@@ -1832,37 +1929,16 @@ FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows, vo
                         fh_stream_t stream) {
   const int st = check_w4(desc, hidden, rows, out);
   if (st != FH_OK || rows == 0) return st;
-  (void)workspace;
-  (void)workspace_bytes;
   if (out_stride < desc->vocab)
     return fail(FH_ERR_INVALID_ARGUMENT, "out_stride=%lld < vocab=%d", (long long)out_stride,
                 desc->vocab);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  if (rows > kW4MvRows)
+    return run_w4_tc(desc, hidden, rows, out, out_stride, workspace, workspace_bytes, sms, s);
   fh::W4Args a = w4_args(desc, hidden, rows, out);
   a.ldo = out_stride;
-  const int sms = sm_count() > 0 ? sm_count() : 148;
-  // few units: the 16 warps of a CTA share units so that every SM has work
-  const int units = a.tiles / 2;
-  a.ksplit = 1;
-  while (a.ksplit < fh::kW4Warps && a.ksplit * 2 <= a.nb &&
-         (long long)units * a.ksplit < 2ll * sms * fh::kW4Warps)
-    a.ksplit *= 2;
-  const int teams = fh::kW4Warps / a.ksplit;
-  const int grid = std::min(sms, (units + teams - 1) / teams);
-  for (int r0 = 0; r0 < rows;) {
-    int nt = rows - r0 > 8 ? 2 : 1;
-    if (fh::w4_mv_smem_bytes(a.nb, nt) > (size_t)kW4SmemMax) nt = 1;
-    a.hidden = reinterpret_cast<const char *>(hidden) + (size_t)r0 * a.D * 2;
-    a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
-    a.rows = std::min(8 * nt, rows - r0);
-    const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto gpk, auto zp) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      return launch_w4_mv_n<T, decltype(gpk)::value, decltype(zp)::value>(a, nt, grid, s);
-    });
-    FH_CHECK_LAUNCH(e, "4-bit logits launch");
-    r0 += 8 * nt;
-  }
-  return FH_OK;
+  return run_w4_mv(desc, a, sms, s);
 }
 
 FH_API int fh_w4_block_sparse_logits(const fh_w4_desc *desc, const void *hs, int T,

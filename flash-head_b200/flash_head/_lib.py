@@ -75,6 +75,7 @@ class W4Desc(ctypes.Structure):
         ("qweight", ctypes.c_void_p),
         ("scales", ctypes.c_void_p),
         ("zeros", ctypes.c_void_p),
+        ("row_mul", ctypes.c_void_p),
     ]
 
 
@@ -141,6 +142,8 @@ _lock = threading.Lock()
 def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load (once) and return the CUDA library; raises if it is not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -176,6 +179,43 @@ def dtype_code(dtype) -> int:
     if dtype not in codes:
         raise ValueError(f"unsupported dtype {dtype}")
     return codes[dtype]
+
+
+def bound(name: str):
+    """The fh_* function itself (a caller in a hot loop keeps it)."""
+    return getattr(load_library(), name)
+
+
+def check(name: str, status: int) -> None:
+    """Raise FlashHeadError for the non-zero status of a call of ``name``."""
+    if status != FH_OK:
+        raise FlashHeadError(name, status, last_error())
+
+
+class on_device:
+    """``with on_device(tensor.device) as stream:`` - that device is current in
+    the block, and ``stream`` is the raw handle of its current stream. Cheaper
+    than ``torch.cuda.device`` where the device is current already."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        import torch
+        self.before = torch.cuda.current_device()
+        if self.index is None:
+            self.index = self.before
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch.cuda.set_device(self.before)
+        return False
 
 
 def stream_ptr(stream=None) -> int:

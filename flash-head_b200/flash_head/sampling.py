@@ -23,25 +23,32 @@ import torch
 
 from . import _lib
 
-_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_DTYPES = {torch.bfloat16: _lib.FH_BF16, torch.float16: _lib.FH_FP16,
+           torch.float32: _lib.FH_FP32}
+_F32, _F64, _I32, _I64 = torch.float32, torch.float64, torch.int32, torch.int64
+_call = None  # fh_sample_logits
 
 
-def _per_row(name: str, value, B: int, dtype: torch.dtype, device, off):
-    """(tensor or None, scalar) of a setting given as None, a number or [B]."""
-    if value is None:
-        return None, off
-    if not isinstance(value, torch.Tensor):
-        value = float(value) if dtype.is_floating_point else int(value)
-        if value != value:
-            raise ValueError(f"{name} is NaN")
-        return None, value
-    if value.dim() > 1 or value.numel() not in (1, B) or (value.numel() == 1 and B != 1):
-        if value.numel() != 1:
-            raise ValueError(f"{name} must be a number or [{B}] values, got {tuple(value.shape)}")
-        value = value.reshape(1).expand(B)
-    if value.device != device:
-        raise ValueError(f"{name} on {value.device}, logits on {device}")
-    return value.reshape(B).to(dtype).contiguous(), off
+def _per_row(name: str, v: torch.Tensor, B: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """A setting's [B] values (a single one serves every row) as the kernel reads them."""
+    if v.device != device:
+        raise ValueError(f"{name} on {v.device}, logits on {device}")
+    if v.dtype is dtype and v.dim() == 1 and v.shape[0] == B and v.is_contiguous():
+        return v
+    if v.numel() == 1 and v.dim() <= 1:
+        v = v.reshape(1).expand(B)
+    elif v.shape != (B,):
+        raise ValueError(f"{name} must be a number or [{B}] values, got {tuple(v.shape)}")
+    return v.to(dtype).contiguous()
+
+
+def _number(name: str, v, low: float, high: float):
+    v = float(v)
+    if v != v:
+        raise ValueError(f"{name} is NaN")
+    if not low <= v <= high:
+        raise ValueError(f"{name} must be in [{low:g}, {high:g}], got {v}")
+    return v
 
 
 def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor,
@@ -70,43 +77,57 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor,
                          f"{tuple(logits.shape)} {logits.dtype}")
     B, n = logits.shape
     dev = logits.device
-    if (n > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < n):
+    stride = logits.stride(0)
+    if (n > 1 and logits.stride(1) != 1) or (B > 1 and stride < n):
         logits = logits.contiguous()
+        stride = n
     if uniforms.shape != (B,) or uniforms.device != dev or not uniforms.is_floating_point():
         raise ValueError(f"uniforms must be [{B}] float64 on {dev}, got "
                          f"{tuple(uniforms.shape)} {uniforms.dtype} on {uniforms.device}")
-    uniforms = uniforms.to(torch.float64).contiguous()
-    if not isinstance(temperature, torch.Tensor) and float(temperature) < 0:
-        raise ValueError(f"temperature must be >= 0, got {temperature}")
-    if not isinstance(top_k, torch.Tensor) and top_k is not None and int(top_k) < 0:
-        raise ValueError(f"top_k must be >= 0, got {top_k}")
-    for name, v in (("top_p", top_p), ("min_p", min_p)):
-        if not isinstance(v, torch.Tensor) and v is not None and not 0.0 <= float(v) <= 1.0:
-            raise ValueError(f"{name} must be in [0, 1], got {v}")
-    d = _lib.SampleParams()
-    f32 = torch.float32
-    t, d.temperature_all = _per_row("temperature", temperature, B, f32, dev, 1.0)
-    k, d.top_k_all = _per_row("top_k", top_k, B, torch.int32, dev, 0)
-    p, d.top_p_all = _per_row("top_p", top_p, B, f32, dev, 1.0)
-    m, d.min_p_all = _per_row("min_p", min_p, B, f32, dev, 0.0)
-    for name, v in (("temperature", t), ("top_k", k), ("top_p", p), ("min_p", m)):
-        setattr(d, name, None if v is None else v.data_ptr())
-    d.uniforms = uniforms.data_ptr()
+    if uniforms.dtype is not _F64 or not uniforms.is_contiguous():
+        uniforms = uniforms.to(_F64).contiguous()
+    tt = kt = pt = mt = None
+    t, k, p, m = 1.0, 0, 1.0, 0.0
+    if isinstance(temperature, torch.Tensor):
+        tt = _per_row("temperature", temperature, B, _F32, dev)
+    elif temperature is not None:
+        t = _number("temperature", temperature, 0.0, float("inf"))
+    if isinstance(top_k, torch.Tensor):
+        kt = _per_row("top_k", top_k, B, _I32, dev)
+    elif top_k is not None:
+        k = int(_number("top_k", top_k, 0, 2 ** 31 - 1))
+    if isinstance(top_p, torch.Tensor):
+        pt = _per_row("top_p", top_p, B, _F32, dev)
+    elif top_p is not None:
+        p = _number("top_p", top_p, 0.0, 1.0)
+    if isinstance(min_p, torch.Tensor):
+        mt = _per_row("min_p", min_p, B, _F32, dev)
+    elif min_p is not None:
+        m = _number("min_p", min_p, 0.0, 1.0)
+    ids_stride = 0
     if ids is not None:
-        if ids.dtype != torch.int32 or ids.device != dev or ids.shape not in ((n,), (B, n)):
+        if ids.dtype is not _I32 or ids.device != dev or ids.shape not in ((n,), (B, n)):
             raise ValueError(f"ids must be int32 [{n}] or [{B}, {n}] on {dev}, got "
                              f"{tuple(ids.shape)} {ids.dtype} on {ids.device}")
         ids = ids.contiguous()
-        d.ids, d.ids_stride = ids.data_ptr(), n if ids.dim() == 2 else 0
+        ids_stride = n if ids.dim() == 2 else 0
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=dev)
-    elif out.shape != (B,) or out.dtype != torch.int64 or out.device != dev \
+        out = torch.empty(B, dtype=_I64, device=dev)
+    elif out.shape != (B,) or out.dtype is not _I64 or out.device != dev \
             or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous [{B}] int64 tensor on {dev}")
-    prob = torch.empty(B, dtype=f32, device=dev) if return_prob else None
+    prob = torch.empty(B, dtype=_F32, device=dev) if return_prob else None
     if B:
-        with torch.cuda.device(dev):
-            _lib.call("fh_sample_logits", logits.data_ptr(), _lib.dtype_code(logits.dtype), B, n,
-                      max(logits.stride(0), n), ctypes.byref(d), out.data_ptr(),
-                      None if prob is None else prob.data_ptr(), _lib.stream_ptr())
+        global _call
+        if _call is None:
+            _call = _lib.bound("fh_sample_logits")
+        d = _lib.SampleParams(
+            None if tt is None else tt.data_ptr(), None if kt is None else kt.data_ptr(),
+            None if pt is None else pt.data_ptr(), None if mt is None else mt.data_ptr(),
+            uniforms.data_ptr(), None if ids is None else ids.data_ptr(), ids_stride, t, k, p, m)
+        with _lib.on_device(dev) as stream:
+            st = _call(logits.data_ptr(), _DTYPES[logits.dtype], B, n, max(stride, n),
+                       ctypes.byref(d), out.data_ptr(),
+                       None if prob is None else prob.data_ptr(), stream)
+        _lib.check("fh_sample_logits", st)
     return (out, prob) if return_prob else out

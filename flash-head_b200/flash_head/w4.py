@@ -10,7 +10,8 @@ w[v, k] = (q[v, k] - z[v, g]) * s[v, g], q in 0..15, one scale (and zero point;
 8 without zero points) per group g = k // group_size of a row. The kernels
 (``csrc/fh_w4.cuh``) sum exact products of q - z and the hidden states in fp32
 and scale each group's sum in fp32; results are rounded once, to the hidden
-states' dtype. ``w4_block_sparse_logits`` is the 4-bit form of
+states' dtype. ``w4_logits`` of more than 8 rows runs on the tensor cores with w
+rounded to 11 bits (``csrc/fh_w4_tc.cuh``). ``w4_block_sparse_logits`` is the 4-bit form of
 ``flash_head.fused.block_sparse_logits`` (reference
 ``src/flash_head/fused.py:82-93``).
 """
@@ -27,7 +28,7 @@ from . import _lib
 GROUP_SIZES = (32, 64, 128)
 MAX_HIDDEN = 12288
 _BLOCK = 128       # columns per layout block
-_ROWS = 128        # rows are padded to a multiple of this
+_ROWS = 128        # rows per layout tile (the last one is padded)
 _CHUNK = 1 << 27   # elements unpacked at a time while laying out
 
 
@@ -41,11 +42,12 @@ def _check_groups(D: int, group_size: int):
 
 
 def _pack_words(q: torch.Tensor, nb: int) -> torch.Tensor:
-    """[R, D] uint8 values (R a multiple of 16) -> int32 [R/16, nb, 16, 4, 4] words."""
+    """[R, D] uint8 values (R a multiple of 128) -> int32 [R/128, nb, 128, 4, 4] words."""
     R, D = q.shape
     if D < nb * _BLOCK:
         q = torch.nn.functional.pad(q, (0, nb * _BLOCK - D), value=8)
-    x = q.view(R // 16, 16, nb, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)  # tile, block, row, quad, word, e
+    # tile, block, row, quad, word, e
+    x = q.view(R // _ROWS, _ROWS, nb, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)
     w = torch.zeros(x.shape[:-1], dtype=torch.int32, device=q.device)
     for e in range(8):
         w |= x[..., e].to(torch.int32) << (4 * (e // 2) + 16 * (e % 2))
@@ -53,19 +55,19 @@ def _pack_words(q: torch.Tensor, nb: int) -> torch.Tensor:
 
 
 def _unpack_words(w: torch.Tensor, D: int) -> torch.Tensor:
-    """The inverse of ``_pack_words``: int32 [t, nb, 16, 4, 4] -> [16 t, D] uint8."""
+    """The inverse of ``_pack_words``: int32 [t, nb, 128, 4, 4] -> [128 t, D] uint8."""
     x = torch.stack([(w >> (4 * (e // 2) + 16 * (e % 2))) & 15 for e in range(8)], dim=-1)
     t, nb = w.shape[0], w.shape[1]
-    x = x.permute(0, 2, 1, 4, 3, 5).reshape(16 * t, nb * _BLOCK)
+    x = x.permute(0, 2, 1, 4, 3, 5).reshape(_ROWS * t, nb * _BLOCK)
     return x[:, :D].to(torch.uint8)
 
 
 def _pack_groups(x: torch.Tensor, V_pad: int, nb: int, gpk: int, fill) -> torch.Tensor:
-    """[V, G] per-group values -> [V_pad/16, nb, 16, gpk], padding = fill."""
+    """[V, G] per-group values -> [V_pad/128, nb, 128, gpk], padding = fill."""
     V, G = x.shape
     out = torch.full((V_pad, nb * gpk), fill, dtype=x.dtype, device=x.device)
     out[:V, :G] = x
-    return out.view(V_pad // 16, 16, nb, gpk).permute(0, 2, 1, 3).contiguous()
+    return out.view(V_pad // _ROWS, _ROWS, nb, gpk).permute(0, 2, 1, 3).contiguous()
 
 
 class W4Weight:
@@ -82,7 +84,13 @@ class W4Weight:
         d.dtype = _lib.dtype_code(scales.dtype)
         d.qweight, d.scales = qweight.data_ptr(), scales.data_ptr()
         d.zeros = None if zeros is None else zeros.data_ptr()
-        self.desc = d
+        # powers of two that bring a row's largest scale to [1, 2)
+        top = scales.float().abs().amax(dim=(1, 3)).view(-1)
+        fine = torch.isfinite(top) & (top > 0)
+        exp = torch.frexp(torch.where(fine, top, torch.ones_like(top))).exponent
+        self.row_mul = torch.ldexp(torch.ones_like(top), 1 - exp).contiguous()
+        d.row_mul = self.row_mul.data_ptr()
+        self.desc, self.ref = d, ctypes.byref(d)
 
     # -- making one ----------------------------------------------------------
     @classmethod
@@ -112,7 +120,7 @@ class W4Weight:
         nb, gpk = -(-D // _BLOCK), _BLOCK // group
         V_pad = -(-V // _ROWS) * _ROWS
         with torch.no_grad():
-            qw = torch.empty((V_pad // 16, nb, 16, 4, 4), dtype=torch.int32, device=q.device)
+            qw = torch.empty((V_pad // _ROWS, nb, _ROWS, 4, 4), dtype=torch.int32, device=q.device)
             step = max(_ROWS, _CHUNK // (nb * _BLOCK) // _ROWS * _ROWS)
             for lo in range(0, V_pad, step):
                 n = min(step, V_pad - lo)
@@ -120,7 +128,7 @@ class W4Weight:
                 x = torch.full((n, D), 8, dtype=torch.uint8, device=q.device)
                 x[:part.shape[0], 0::2] = part & 15
                 x[:part.shape[0], 1::2] = part >> 4
-                qw[lo // 16:(lo + n) // 16] = _pack_words(x, nb)
+                qw[lo // _ROWS:(lo + n) // _ROWS] = _pack_words(x, nb)
             s = _pack_groups(scales, V_pad, nb, gpk, 0.0)
             z = None if zeros is None else _pack_groups(zeros, V_pad, nb, gpk, 8)
         return cls(qw, s, z, V, D, group)
@@ -192,7 +200,7 @@ class W4Weight:
         """[V, D] fp32 (q - z) * s."""
         G = self.hidden // self.group_size
 
-        def rows(x):  # [tiles, nb, 16, gpk] -> [V, G]
+        def rows(x):  # [tiles, nb, 128, gpk] -> [V, G]
             return x.permute(0, 2, 1, 3).reshape(-1, x.shape[1] * x.shape[3])[:self.vocab, :G]
         q = _unpack_words(self.qweight, self.hidden)[:self.vocab].float()
         q = q.view(self.vocab, G, self.group_size)
@@ -232,12 +240,14 @@ def w4_logits(hs: torch.Tensor, w: W4Weight, out: Optional[torch.Tensor] = None)
                          "contiguous rows")
     if T == 0:
         return out
-    with torch.cuda.device(hs.device):
-        need = int(_lib.load_library().fh_w4_workspace_bytes(ctypes.byref(w.desc), T))
+    lib = _lib.load_library()
+    with _lib.on_device(hs.device) as stream:
+        need = lib.fh_w4_workspace_bytes(w.ref, T)
         ws = torch.empty(need, dtype=torch.uint8, device=hs.device) if need else None
-        _lib.call("fh_w4_logits", ctypes.byref(w.desc), hs.data_ptr(), T, out.data_ptr(),
-                  max(out.stride(0), w.vocab), None if ws is None else ws.data_ptr(), need,
-                  _lib.stream_ptr())
+        st = lib.fh_w4_logits(w.ref, hs.data_ptr(), T, out.data_ptr(),
+                              max(out.stride(0), w.vocab),
+                              None if ws is None else ws.data_ptr(), need, stream)
+    _lib.check("fh_w4_logits", st)
     return out
 
 
@@ -254,8 +264,10 @@ def w4_block_sparse_logits(hs: torch.Tensor, w: W4Weight, ci: torch.Tensor, n_cl
     T, P = ci.shape
     ci = ci.contiguous()
     out = torch.empty((T, P * int(cluster_size)), dtype=hs.dtype, device=hs.device)
-    with torch.cuda.device(hs.device):
-        _lib.call("fh_w4_block_sparse_logits", ctypes.byref(w.desc), hs.data_ptr(), T,
-                  ci.data_ptr(), P, int(n_clusters), int(cluster_size), out.data_ptr(),
-                  _lib.stream_ptr())
+    lib = _lib.load_library()
+    with _lib.on_device(hs.device) as stream:
+        st = lib.fh_w4_block_sparse_logits(w.ref, hs.data_ptr(), T, ci.data_ptr(), P,
+                                           int(n_clusters), int(cluster_size), out.data_ptr(),
+                                           stream)
+    _lib.check("fh_w4_block_sparse_logits", st)
     return out

@@ -375,12 +375,14 @@ FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
  *   hidden     D, columns: a multiple of group_size, at most FH_W4_MAX_HIDDEN
  *   group_size 32, 64 or 128
  *   dtype      FH_BF16 or FH_FP16: type of the scales, hidden states, outputs
- *   qweight    u32 [T][B][16][4][4], T = V / 16 rounded up to a multiple of 8
- *              (tiles of 16 rows), B = ceil(D / 128): word j of quad c of row r
- *              of block b holds the 8 columns 128 b + 32 j + 8 c + e, column
- *              e = 2i in bits 4i..4i+3, e = 2i + 1 in bits 16+4i..19+4i
- *   scales     [T][B][16][128 / group_size]; 0 in padded rows and groups
+ *   qweight    u32 [T][B][128][4][4], T = ceil(V / 128) tiles of 128 rows, B =
+ *              ceil(D / 128): word j of quad c of row r of block b holds the 8
+ *              columns 128 b + 32 j + 8 c + e, column e = 2i in bits
+ *              4i..4i+3, e = 2i + 1 in bits 16+4i..19+4i
+ *   scales     [T][B][128][128 / group_size]; 0 in padded rows and groups
  *   zeros      u8, the shape of scales; NULL: every zero point is 8
+ *   row_mul    fp32 [128 T], powers of two that bring the largest scale of each
+ *              row to [1, 2) (1 for a row without finite scales above 0)
  * The Python loader (flash_head/w4.py) makes this layout. Pointers 16-byte
  * aligned, device memory.
  */
@@ -393,12 +395,15 @@ typedef struct fh_w4_desc {
   const uint32_t *qweight;
   const void *scales;
   const uint8_t *zeros;
+  const float *row_mul;
 } fh_w4_desc;
 
 /* out[r * out_stride + v] = logit of weight row v for hidden row r: the dense
  * head's logits (the reference's F.linear over the head weight,
  * flash_head.py:292-301). out_stride >= V, in elements. The workspace
- * (fh_w4_workspace_bytes; it may be 0, then NULL is fine) needs no zeroing. */
+ * (fh_w4_workspace_bytes; where that is 0, NULL is fine) needs no zeroing; its
+ * first 32-bit word is 0 after a call, or has bit 1 set where a bounded wait
+ * inside the call ran out (the outputs are then meaningless). */
 FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows);
 FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows,
                         void *out, int64_t out_stride, void *workspace,

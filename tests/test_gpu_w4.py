@@ -7,6 +7,13 @@ of group/16 tensor-core steps, the groups' scaled sums another chain, and up to
 which rounds (or truncates) a partial sum of magnitude at most
 A = sum |w| |h| by 2^-22 relative at worst. Then one rounding to the output
 type: half a step, eps / 2 relative.
+
+Dense calls of more than 8 rows round each weight to f16: half a step, 2^-11
+relative. The hidden states are symmetric around 0 and independent, so the
+errors e_k w_k h_k, |e_k| <= 2^-11, are independent, have mean 0 and are bounded
+by b_k = 2^-11 |w_k h_k|: by Hoeffding's inequality their sum passes
+t = 7 sqrt(sum b_k^2) with a probability below 2 exp(-t^2 / (2 sum b_k^2)) =
+5e-11, 5e-4 over 10^7 outputs.
 """
 
 from __future__ import annotations
@@ -37,17 +44,21 @@ def make_hidden(T, D, dtype, seed):
     return (torch.randn(T, D, generator=g) * 0.5).to(dtype).cuda()
 
 
-def check(got, h, W, group, dtype):
-    """got [T, V] against h @ W^T in 64 bits (W [V, D] or [T, V, D])."""
+def check(got, h, W, group, dtype, rows=None):
+    """got [T, V] against h @ W^T in 64 bits (W [V, D] or [T, V, D]); rows: of
+    the call, when that is not T."""
     hd = h.double()
+    rounded = 0.0
     if W.dim() == 2:
         want, mag = hd @ W.t(), hd.abs() @ W.abs().t()
+        if (rows or h.shape[0]) > 8:
+            rounded = 7 * 2.0 ** -11 * (hd.square() @ W.square().t()).sqrt()
     else:
         want = (W * hd.unsqueeze(1)).sum(2)
         mag = (W.abs() * hd.abs().unsqueeze(1)).sum(2)
     D = h.shape[1]
     tol = (torch.finfo(dtype).eps / 2) * want.abs() \
-        + (group / 16 + D / group + 16) * 2.0 ** -22 * mag + torch.finfo(dtype).tiny
+        + (group / 16 + D / group + 16) * 2.0 ** -22 * mag + rounded + torch.finfo(dtype).tiny
     err = (got.double() - want).abs()
     bad = ~(err <= tol)
     assert not bad.any(), (bad.nonzero()[:4].tolist(), float((err / tol).max()))
@@ -113,7 +124,7 @@ def test_rows_do_not_touch_each_other(T):
     h[2, 7] = float("nan")
     got = w4_logits(h, w)
     keep = [r for r in range(T) if r not in (1, 2)]
-    check(got[keep], h[keep], W, 128, torch.float16)
+    check(got[keep], h[keep], W, 128, torch.float16, rows=T)
     assert got[2].isnan().all() and not got[1].isfinite().any()
 
 
@@ -194,6 +205,25 @@ def test_side_stream_and_graph(T):
         torch.cuda.synchronize()
         check(out, h, W, 128, torch.bfloat16)
         assert torch.equal(out, w4_logits(h, w))
+
+
+def test_workspace_word_is_clear():
+    """No bounded wait of the tensor-core kernel runs out."""
+    import ctypes
+
+    from flash_head import _lib
+    for dtype in (torch.bfloat16, torch.float16):
+        w, W = make_weight(40000, 1024, 64, True, dtype, seed=3)
+        h = make_hidden(100, 1024, dtype, 3)
+        lib = _lib.load_library()
+        need = lib.fh_w4_workspace_bytes(ctypes.byref(w.desc), 100)
+        ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        out = torch.empty(100, 40000, dtype=dtype, device="cuda")
+        _lib.call("fh_w4_logits", ctypes.byref(w.desc), h.data_ptr(), 100, out.data_ptr(), 40000,
+                  ws.data_ptr(), need, _lib.stream_ptr())
+        torch.cuda.synchronize()
+        assert int(ws[:4].view(torch.int32)) == 0
+        check(out, h, W, 64, dtype)
 
 
 @pytest.mark.parametrize("zeros,bound", [(False, 1 / 7), (True, 1 / 15)])

@@ -40,15 +40,15 @@ def test_layout_words():
     q, s, z = _quantized(V, D, group)
     w = W4Weight.from_quantized(q, s, z)
     v = torch.stack([q & 15, q >> 4], 2).view(V, D).tolist()
-    assert w.qweight.shape == (8, 2, 16, 4, 4)  # rows padded to 128
+    assert w.qweight.shape == (1, 2, 128, 4, 4)  # rows padded to 128
     words = w.qweight.tolist()
     for r, b, c, j in [(0, 0, 0, 0), (7, 1, 3, 2), (19, 0, 1, 3), (16, 1, 2, 1)]:
-        word = words[r // 16][b][r % 16][c][j] & 0xFFFFFFFF
+        word = words[r // 128][b][r % 128][c][j] & 0xFFFFFFFF
         for e in range(8):
             at = 4 * (e // 2) + 16 * (e % 2)
             assert (word >> at) & 15 == v[r][128 * b + 32 * j + 8 * c + e]
-    assert w.scales[1, 1, 3, 0] == s[19, 2] and w.zeros[1, 1, 3, 1] == z[19, 3]
-    assert (w.scales[1, :, 4:] == 0).all() and (w.scales[2:] == 0).all()
+    assert w.scales[0, 1, 19, 0] == s[19, 2] and w.zeros[0, 1, 19, 1] == z[19, 3]
+    assert (w.scales[0, :, 20:] == 0).all() and (w.zeros[0, :, 20:] == 8).all()
 
 
 @pytest.mark.parametrize("zeros", [False, True])
@@ -110,7 +110,7 @@ def _desc(**kw):
     d = _lib.W4Desc()
     fake = 1 << 20  # aligned, never dereferenced by validation
     d.vocab, d.hidden, d.group_size, d.dtype = 1000, 256, 64, _lib.FH_BF16
-    d.qweight, d.scales = fake, fake
+    d.qweight, d.scales, d.row_mul = fake, fake, fake
     for k, v in kw.items():
         setattr(d, k, v)
     return ctypes.byref(d)
@@ -120,6 +120,7 @@ def _desc(**kw):
     ("vocab", 0, "vocab"), ("hidden", 0, "hidden"), ("hidden", 96, "multiple of group_size"),
     ("hidden", 12288 + 64, "at most"), ("group_size", 48, "group_size"),
     ("dtype", _lib.FH_FP32, "dtype"), ("qweight", None, "null"), ("scales", None, "null"),
+    ("row_mul", None, "null"),
     ("qweight", (1 << 20) + 8, "aligned"), ("zeros", (1 << 20) + 1, "aligned")])
 def test_refused_descriptors(lib, field, value, msg):
     fake = 1 << 20
@@ -140,6 +141,13 @@ def test_refused_calls(lib):
     assert lib.fh_w4_logits(d, fake, 1, fake + 1, 1000, None, 0, None) == bad
     assert lib.fh_w4_logits(d, fake, 1, fake, 999, None, 0, None) == bad
     assert "out_stride" in _lib.last_error()
+    # more than 8 rows need a workspace
+    assert lib.fh_w4_workspace_bytes(d, 8) == 0 and lib.fh_w4_workspace_bytes(None, 99) == 0
+    need = lib.fh_w4_workspace_bytes(d, 20)
+    assert need == 256 + 256 + 20 * 256 * 2
+    assert lib.fh_w4_logits(d, fake, 20, fake, 1000, fake, need - 1, None) == _lib.FH_ERR_WORKSPACE
+    assert lib.fh_w4_logits(d, fake, 20, fake, 1000, None, 0, None) == _lib.FH_ERR_WORKSPACE
+    assert lib.fh_w4_logits(d, fake, 20, fake, 1000, fake + 4, need, None) == bad
     blk = lib.fh_w4_block_sparse_logits
     assert blk(d, None, 0, None, 4, 10, 16, None, None) == _lib.FH_OK
     assert blk(d, None, 3, None, 0, 10, 16, None, None) == _lib.FH_OK
