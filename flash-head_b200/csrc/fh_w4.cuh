@@ -8,13 +8,13 @@
 //
 // Layout (made once by the loader, flash_head/w4.py). Rows come in tiles of
 // 128, columns in blocks of 128 (both padded; padding has scale 0):
-//   qweight u32 [tile][block][128 rows][4 quads][4 words]: word j of quad c
+//   qweight u32 [tile][block][4 quads][128 rows][4 words]: word j of quad c
 //           holds columns 128 * block + 32 * j + 8 * c + e, e = 0..7, column
 //           e = 2i in bits 4i..4i+3 and e = 2i+1 in bits 16+4i..19+4i.
 //   scales  16-bit [tile][block][128 rows][groups per block]
 //   zeros   u8, same shape (absent: every zero point is 8)
-// One tile's block is 8 KB, contiguous (one bulk copy), and 16 of its rows are
-// 1 KB: lane (g, c) of a warp reads 16 bytes of row g and 16 of row g + 8.
+// One tile's block is 8 KB, contiguous (one bulk copy). Lane (g, c) of a warp
+// reads 16 bytes of row g and 16 of row g + 8 in quad c: 128-byte runs.
 // The nibble order makes (w >> 4i) & 0x000F000F a pair of neighbouring
 // columns, i.e. one operand register of mma.m16n8k16 (A: 16 weight rows), and
 // the 8 columns of a word are 16 contiguous bytes of a hidden row (B), so
@@ -26,6 +26,10 @@
 namespace fh {
 
 constexpr int kW4Warps = 16;
+#ifndef W4_AHEAD
+#define W4_AHEAD 2
+#endif
+constexpr int kW4Ahead = W4_AHEAD;  // blocks a warp loads ahead
 constexpr int kW4Block = 128;                   // columns per block
 constexpr int kW4Tile = 128;                     // rows per tile
 constexpr int kW4RowWords = kW4Block / 8;        // u32 of one row's block
@@ -130,6 +134,11 @@ struct W4Frag {
   typename W4Group<GPK>::Z z[2];
 };
 
+// First word of a row's quad; i counts rows in [tile][block][row] order.
+__device__ __forceinline__ long long w4_word(long long i, int c) {
+  return ((i >> 7) * (4 * kW4Tile) + c * kW4Tile + (i & (kW4Tile - 1))) * 4;
+}
+
 template <int GPK, bool ZP>
 __device__ __forceinline__ void w4_load(const W4Args &a, int kb, int r0, int r1, int c,
                                         W4Frag<GPK, ZP> &f) {
@@ -138,8 +147,8 @@ __device__ __forceinline__ void w4_load(const W4Args &a, int kb, int r0, int r1,
   // row of the [tile][block][row] order
   const long long i0 = ((long long)(r0 >> 7) * a.nb + kb) * kW4Tile + (r0 & 127);
   const long long i1 = ((long long)(r1 >> 7) * a.nb + kb) * kW4Tile + (r1 & 127);
-  f.q[0] = ldg_stream(a.qw + i0 * kW4RowWords + c * 4);
-  f.q[1] = ldg_stream(a.qw + i1 * kW4RowWords + c * 4);
+  f.q[0] = ldg_stream(a.qw + w4_word(i0, c));
+  f.q[1] = ldg_stream(a.qw + w4_word(i1, c));
   const S *s = reinterpret_cast<const S *>(a.scales);
   f.s[0] = __ldg(s + i0);
   f.s[1] = __ldg(s + i1);
@@ -244,29 +253,47 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
   const int rounds = (units + per_round - 1) / per_round;
   const int first = team * gridDim.x + blockIdx.x;
 
-  for (int round = 0; round < rounds; ++round) {
-    const int u = first + round * per_round;
-    const bool live = u < units;
-    float acc[2][NT][4];
+  // the warp's blocks, unit after unit, are loaded kW4Ahead steps ahead
+  W4Frag<GPK, ZP> f[kW4Ahead][2];
+  int l_round = 0, l_b = 0;
+  auto fetch = [&](W4Frag<GPK, ZP>(&x)[2]) {
+    if (l_round < rounds) {
+      const int u = min(first + l_round * per_round, units - 1), kb = kw + l_b * ks;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
-    if (live) {
-      for (int b = 0; b < my_nb; ++b) {
-        const int kb = kw + b * ks;
-        W4Frag<GPK, ZP> f[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          w4_load<GPK, ZP>(a, kb, 32 * u + 16 * t + g, 32 * u + 16 * t + g + 8, c, f[t]);
-        const unsigned char *hk = hl + kb * (kW4Block * 2);
-        auto load = [&](int n, int j) { return lds128(hk + (size_t)(8 * n) * rb + j * 64); };
-#pragma unroll
-        for (int t = 0; t < 2; ++t) w4_block<T, GPK, ZP, NT>(f[t], load, acc[t]);
+      for (int t = 0; t < 2; ++t)
+        w4_load<GPK, ZP>(a, kb, 32 * u + 16 * t + g, 32 * u + 16 * t + g + 8, c, x[t]);
+      if (++l_b == my_nb) {
+        l_b = 0;
+        ++l_round;
       }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kW4Ahead; ++i) fetch(f[i]);
+  float acc[2][NT][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
+
+  const int steps = rounds * my_nb;
+  for (int step0 = 0, b = 0, round = 0; step0 < steps; step0 += kW4Ahead) {
+#pragma unroll
+   for (int ahead = 0; ahead < kW4Ahead; ++ahead) {
+    if (step0 + ahead >= steps) break;
+    const int kb = kw + b * ks;
+    const unsigned char *hk = hl + kb * (kW4Block * 2);
+    auto load = [&](int n, int j) { return lds128(hk + (size_t)(8 * n) * rb + j * 64); };
+#pragma unroll
+    for (int t = 0; t < 2; ++t) w4_block<T, GPK, ZP, NT>(f[ahead][t], load, acc[t]);
+    fetch(f[ahead]);
+    if (++b < my_nb) continue;
+    b = 0;
+    const int u = first + round * per_round;
+    const bool live = u < units;
+    ++round;
     if (ks > 1) {
       // sum the team's partial sums, warp kw = 0 keeps them (fixed order)
       float *mine = red + (size_t)warp * NT * 32 * 8 + lane * (8 * NT);
@@ -309,6 +336,13 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
             if (v < a.V && r < a.rows) out[(long long)r * a.ldo + v] = from_float<T>(acc[t][n][i]);
           }
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
+   }
   }
 }
 

@@ -2,7 +2,7 @@
 // out[b, v] = sum_k w[v, k] h[b, k], M = 128 weight rows, N = up to 256 hidden
 // rows per launch.
 //
-// The weight's integers become f16 operands in shared memory: q - z is exact,
+// The weight's integers become f16 operands: q - z is exact,
 // and its product with the group's scale is rounded to f16 once, 2^-11 relative
 // (a bf16 scale times a 4-bit integer has at most one bit more than f16 holds).
 // That is an eighth of a bf16 output's own rounding; applying the scales to
@@ -12,20 +12,24 @@
 // hidden rows are copied to f16 first, each scaled by a power of two likewise
 // (k_w4_hidden); f16 ones are read as they are.
 //
-// One persistent CTA per SM, 14 warps:
+// The unpacked operand goes to tensor memory, not to shared memory: 16 KB
+// written and 16 KB read per 128 x 64 tile were most of the shared-memory
+// traffic that bound a first version (64 rows of a 1536 x 151936 head: 92 us).
+//
+// One persistent CTA per SM, 16 warps:
 //   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and
 //               zero points of 128 rows x 128 columns: two or three bulk copies)
-//               into a ring of their own, deep enough to keep HBM busy, and the
-//               hidden tile of every 64 columns (TMA, 128-byte swizzle) into
-//               the stages;
-//   warp 1      allocates TMEM; lane 0 issues tcgen05.mma (K = 16) per stage;
-//   warps 2-9   unpack: a thread takes 32 columns of two rows per block and
-//               writes 16-byte pieces of the swizzled A tile. Lanes cover rows
-//               p and p ^ 5 together: neither their reads (rows of 64 bytes)
-//               nor their writes (rows of 128, pieces exchanged by row) meet in
-//               a bank;
-//   warps 10-13 epilogue: a thread has one weight row and all hidden rows; the
-//               accumulators are double-buffered.
+//               into a ring of their own, deep enough to keep HBM busy;
+//   warp 2      lane 0 brings the hidden tile of every 64 columns (TMA, 128-byte
+//               swizzle) into the stages (a thread of its own: a wait that
+//               suspends the one for packed slots must not hold up these);
+//   warp 1      allocates TMEM; lane 0 issues tcgen05.mma (K = 16), A from
+//               tensor memory, B from shared memory;
+//   warps 4-11  unpack, in two groups of 4 on alternate blocks: a thread has one
+//               weight row, i.e. one TMEM lane, reads its 64 bytes of the block
+//               and stores 32 columns' pairs (16 TMEM columns) at a time;
+//   warps 12-15 epilogue: a thread has one weight row and all hidden rows; up to
+//               192 hidden rows the accumulators are double-buffered.
 // Bounds: HBM (the packed weight) up to about 64 rows, the tensor cores and
 // the hidden tiles' way from L2 at 256.
 // Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
@@ -37,13 +41,23 @@
 
 namespace fh {
 
-constexpr int kW4tThreads = 448;
-constexpr int kW4tConvWarps = 8;
+#ifndef W4_GROUPS
+#define W4_GROUPS 2
+#endif
+constexpr int kW4tConvWarps = 4;  // unpack one block together, a TMEM quadrant each
+constexpr int kW4tGroups = W4_GROUPS;      // of such warps, on successive blocks
 constexpr int kW4tEpiWarps = 4;
+constexpr int kW4tFirstConv = 4;  // warp
+constexpr int kW4tThreads = 32 * (kW4tFirstConv + kW4tGroups * kW4tConvWarps + kW4tEpiWarps);
+// A group skips the others' blocks; its parity waits are unambiguous while the
+// stage it comes to next was last used at most one use after those it knows to
+// be done (2 groups * 2 stages <= stages + 1), and likewise the packed slots.
+constexpr int kW4tMinStages = 2 * kW4tGroups - 1;
+constexpr int kW4tMinPacked = kW4tGroups + 2;
 constexpr int kW4tMaxN = 256;
-constexpr int kW4tMaxStages = 6;
+constexpr int kW4tMaxStages = 4;
+constexpr int kW4tACols = 32;  // TMEM columns of a stage's A tile: 64 f16 per row
 constexpr int kW4tMaxPacked = 12;
-constexpr int kW4tABytes = 128 * 128;  // 128 rows x 64 columns f16
 constexpr int kW4tSmemMax = 227 * 1024;
 
 struct W4TcArgs {
@@ -65,8 +79,7 @@ struct W4TcArgs {
 };
 
 struct W4TcCtrl {
-  uint64_t full[kW4tMaxStages];    // hidden tile landed
-  uint64_t conv[kW4tMaxStages];    // A tile written
+  uint64_t full[kW4tMaxStages];    // hidden tile landed and A tile written
   uint64_t empty[kW4tMaxStages];   // MMAs done
   uint64_t pfull[kW4tMaxPacked];   // packed block landed
   uint64_t pempty[kW4tMaxPacked];  // packed block unpacked
@@ -82,11 +95,50 @@ __host__ __device__ inline int w4t_packed_bytes(int gpk, bool zp) {
   return kW4Tile * kW4RowWords * 4 + kW4Tile * gpk * (zp ? 3 : 2);
 }
 __host__ __device__ inline size_t w4t_stage_bytes(int n_pad) {
-  return (size_t)kW4tABytes + (size_t)n_pad * 128;
+  return (size_t)n_pad * 128;
 }
 __host__ __device__ inline size_t w4t_smem_bytes(int n_pad, int stages, int packed, int gpk, bool zp) {
   return 1024 + stages * w4t_stage_bytes(n_pad) + (size_t)packed * w4t_packed_bytes(gpk, zp) +
          sizeof(W4TcCtrl);
+}
+
+// mbar_wait and tc_commit by shared-memory address.
+__device__ __forceinline__ bool w4t_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void w4t_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   bar)
+               : "memory");
+}
+
+// D += A . B with A in tensor memory: row m in lane m, two f16 per column.
+__device__ __forceinline__ void w4t_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 16 columns of this warp's 32 lanes, a register each.
+__device__ __forceinline__ void w4t_st16(uint32_t addr, const uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]),
+      "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+      : "memory");
 }
 
 // f16 copy of bf16 hidden rows, one CTA per row: the row's largest finite
@@ -158,8 +210,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&S.full[s], 1);
-      mbar_init(&S.conv[s], kW4tConvWarps);
+      mbar_init(&S.full[s], 1 + kW4tConvWarps);
       mbar_init(&S.empty[s], 1);
     }
     for (int s = 0; s < a.packed; ++s) {
@@ -185,78 +236,79 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = S.tmem_base;
+  const uint32_t a_col = (uint32_t)(a.n_acc * a.n_pad);  // first column of the A tiles
 
   if (warp == 0) {
     if (lane == 0) {
-      // packed blocks run ahead of the hidden tiles by the depth of their ring
-      int issued_s[kW4tMaxStages], issued_p[kW4tMaxPacked];  // parity of the last fill, -1: none
-      for (int j = 0; j < kW4tMaxStages; ++j) issued_s[j] = -1;
-      for (int j = 0; j < kW4tMaxPacked; ++j) issued_p[j] = -1;
-      int pt = t0, pkb = 0, ps = 0, s = 0;
-      uint32_t pph = 0u, ph = 0u;
-      bool ok = true, waited = false;
-      auto fill_packed = [&]() {  // false: its slot is not free yet
-        if (pt >= a.tiles) return true;
-        if (!mbar_try_wait(&S.pempty[ps], pph ^ 1u)) return false;
-        unsigned char *p = pring + (size_t)ps * pb;
-        const size_t blk = (size_t)pt * a.nb + pkb;
-        mbar_expect_tx(&S.pfull[ps], (uint32_t)pb);
-        bulk_g2s(p, reinterpret_cast<const unsigned char *>(a.qw) + blk * kWords, kWords,
-                 &S.pfull[ps]);
-        bulk_g2s(p + kWords, reinterpret_cast<const unsigned char *>(a.scales) + blk * kScales,
-                 kScales, &S.pfull[ps]);
-        if (ZP) bulk_g2s(p + kWords + kScales, a.zeros + blk * kZeros, kZeros, &S.pfull[ps]);
-        issued_p[ps] = (int)pph;
-        if (++ps == a.packed) {
-          ps = 0;
-          pph ^= 1u;
-        }
-        if (++pkb == a.nb) {
-          pkb = 0;
-          pt += G;
-        }
-        return true;
-      };
-      for (int i = 0; i < a.packed; ++i) fill_packed();
+      int issued[kW4tMaxPacked];  // parity of the last fill of each slot, -1: none
+      for (int j = 0; j < kW4tMaxPacked; ++j) issued[j] = -1;
+      int ps = 0;
+      uint32_t ph = 0u;
+      bool ok = true;
       for (int t = t0; t < a.tiles && ok; t += G) {
-        for (int k = 0; k < a.nk && ok; ++k) {
-          // the stage's hidden tile; meanwhile packed slots that come free
-          bool free = false;
-          for (uint32_t i = 0; i < a.polls && !free; ++i) {
-            fill_packed();
-            free = mbar_try_wait(&S.empty[s], ph ^ 1u);
-          }
-          if (!free) {
+        for (int kb = 0; kb < a.nb; ++kb) {
+          if (!mbar_wait(&S.pempty[ps], ph ^ 1u, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
             break;
           }
-          if (!waited) {  // the f16 copy of the hidden rows
-            grid_dep_wait();
-            waited = true;
+          unsigned char *p = pring + (size_t)ps * pb;
+          const size_t blk = (size_t)t * a.nb + kb;
+          mbar_expect_tx(&S.pfull[ps], (uint32_t)pb);
+          bulk_g2s(p, reinterpret_cast<const unsigned char *>(a.qw) + blk * kWords, kWords,
+                   &S.pfull[ps]);
+          bulk_g2s(p + kWords, reinterpret_cast<const unsigned char *>(a.scales) + blk * kScales,
+                   kScales, &S.pfull[ps]);
+          if (ZP) bulk_g2s(p + kWords + kScales, a.zeros + blk * kZeros, kZeros, &S.pfull[ps]);
+          issued[ps] = (int)ph;
+          if (++ps == a.packed) {
+            ps = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // every copy this thread issued has landed before the CTA may leave
+      for (int j = 0; j < a.packed; ++j)
+        if (issued[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued[j], a.polls))
+          atomicOr(&S.s_err, kErrCopyTimeout);
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      int issued[kW4tMaxStages];
+      for (int j = 0; j < kW4tMaxStages; ++j) issued[j] = -1;
+      int s = 0;
+      uint32_t ph = 0u;
+      bool ok = true;
+      grid_dep_wait();  // the f16 copy of the hidden rows
+      for (int t = t0; t < a.tiles && ok; t += G) {
+        for (int k = 0; k < a.nk; ++k) {
+          if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
+            atomicOr(&S.s_err, kErrCopyTimeout);
+            ok = false;
+            break;
           }
           mbar_expect_tx(&S.full[s], (uint32_t)(a.n_pad * 128));
-          tma_load_2d(ring + (size_t)s * sb + kW4tABytes, &tm_h, k * 64, 0, &S.full[s]);
-          issued_s[s] = (int)ph;
+          tma_load_2d(ring + (size_t)s * sb, &tm_h, k * 64, 0, &S.full[s]);
+          issued[s] = (int)ph;
           if (++s == a.stages) {
             s = 0;
             ph ^= 1u;
           }
         }
       }
-      // blocks whose slots were still taken
-      for (uint32_t i = 0; i < a.polls && ok && pt < a.tiles; ++i) fill_packed();
-      if (ok && pt < a.tiles) atomicOr(&S.s_err, kErrCopyTimeout);
-      // every copy this thread issued has landed before the CTA may leave
-      for (int j = 0; j < a.packed; ++j)
-        if (issued_p[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued_p[j], a.polls))
-          atomicOr(&S.s_err, kErrCopyTimeout);
       for (int j = 0; j < a.stages; ++j)
-        if (issued_s[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued_s[j], a.polls))
+        if (issued[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued[j], a.polls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 1) {
     if (lane == 0) {
+      // one thread feeds the tensor cores between busy warps: its loop has
+      // addresses and descriptors ready
+      const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]);
+      const uint64_t bd0 = umma_desc_k(smem_u32(ring)), step = sb >> 4;
+      const uint32_t idesc = a.idesc;
+      uint64_t bd = bd0;
+      uint32_t at = tmem + a_col;
       int s = 0;
       uint32_t ph = 0u;
       bool ok = true;
@@ -267,26 +319,29 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
             atomicOr(&S.s_err, kErrCopyTimeout);
             break;
           }
-          tc_fence_after();
         }
         const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
+        uint32_t more = 0u;
         for (int k = 0; k < a.nk; ++k) {
-          if (!mbar_wait(&S.full[s], ph, a.polls) || !mbar_wait(&S.conv[s], ph, a.polls)) {
+          if (!w4t_wait(full0 + 8u * s, ph, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(ring + (size_t)s * sb);
-          const uint64_t ad = umma_desc_k(st);
-          const uint64_t bd = umma_desc_k(st + (uint32_t)kW4tABytes);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            tc_mma_f16(acc, ad + 2u * q, bd + 2u * q, a.idesc, (k | q) != 0 ? 1u : 0u);
-          tc_commit(&S.empty[s]);
+          w4t_mma(acc, at, bd, idesc, more);
+          more = 1u;
+          w4t_mma(acc, at + 8u, bd + 2u, idesc, 1u);
+          w4t_mma(acc, at + 16u, bd + 4u, idesc, 1u);
+          w4t_mma(acc, at + 24u, bd + 6u, idesc, 1u);
+          w4t_commit(empty0 + 8u * s);
+          bd += step;
+          at += kW4tACols;
           if (++s == a.stages) {
             s = 0;
             ph ^= 1u;
+            bd = bd0;
+            at = tmem + a_col;
           }
         }
         if (ok) tc_commit(&S.acc_full[buf]);
@@ -294,37 +349,47 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
       tc_commit(&S.drain);
       if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
     }
-  } else if (warp < 2 + kW4tConvWarps) {
-    const int c = lane & 3, p = lane >> 3;
-    const int m0 = 8 * (warp - 2) + ((lane & 4) ? p ^ 5 : p);  // rows m0, m0 + 64
-    int s = 0, ps = 0;
+  } else if (warp >= kW4tFirstConv && warp < kW4tFirstConv + kW4tGroups * kW4tConvWarps) {
+    const int group = (warp - kW4tFirstConv) / kW4tConvWarps;
+    const int q4 = warp & 3, m = 32 * q4 + lane;  // this thread's row of the tile
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16) + a_col;
+    int s = 0, ps = 0, turn = 0;
     uint32_t ph = 0u, pph = 0u;
     bool ok = true;
     for (int t = t0; t < a.tiles && ok; t += G) {
-      const float mul[2] = {__ldg(a.row_mul + t * kW4Tile + m0),
-                            __ldg(a.row_mul + t * kW4Tile + m0 + 64)};
+      const float mul = __ldg(a.row_mul + t * kW4Tile + m);
       for (int kb = 0; kb < a.nb && ok; ++kb) {
+        const bool mine = turn == group;
+        if (++turn == kW4tGroups) turn = 0;
+        if (!mine) {  // another group's block: step over its slot and stages
+          if (++ps == a.packed) {
+            ps = 0;
+            pph ^= 1u;
+          }
+          s += min(2, a.nk - 2 * kb);
+          if (s >= a.stages) {
+            s -= a.stages;
+            ph ^= 1u;
+          }
+          continue;
+        }
         if (!mbar_wait(&S.pfull[ps], pph, a.polls)) {
           atomicOr(&S.s_err, kErrCopyTimeout);
           ok = false;
           break;
         }
         const unsigned char *pk = pring + (size_t)ps * pb;
-        uint4 q[2];
-        uint32_t sc[2][GPK], zz[2][GPK];
+        uint4 q[4];
+        uint32_t sc[GPK], zz[GPK];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int m = m0 + 64 * i;
-          q[i] = lds128(pk + m * 64 + c * 16);
+        for (int c = 0; c < 4; ++c) q[c] = lds128(pk + (c * kW4Tile + m) * 16);
 #pragma unroll
-          for (int g = 0; g < GPK; ++g) {
-            const uint16_t bits =
-                reinterpret_cast<const uint16_t *>(pk + kWords)[m * GPK + g];
-            const __half2 h = __float2half2_rn(W4Num<T>::scale(bits) * mul[i]);
-            sc[i][g] = *reinterpret_cast<const uint32_t *>(&h);
-            const uint32_t z = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
-            zz[i][g] = W4Num<__half>::kMagic | (z * 0x00010001u);
-          }
+        for (int g = 0; g < GPK; ++g) {
+          const uint16_t bits = reinterpret_cast<const uint16_t *>(pk + kWords)[m * GPK + g];
+          const __half2 h = __float2half2_rn(W4Num<T>::scale(bits) * mul);
+          sc[g] = *reinterpret_cast<const uint32_t *>(&h);
+          const uint32_t z = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
+          zz[g] = W4Num<__half>::kMagic | (z * 0x00010001u);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_cta(&S.pempty[ps]);
@@ -338,32 +403,32 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
           if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
-            break;
           }
-          unsigned char *at = ring + (size_t)s * sb;
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int m = m0 + 64 * i;
+          for (int jj = 0; jj < 2; ++jj) {
+            const int j = 2 * h + jj, g = j * GPK / 4;
+            uint32_t x[16];
 #pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-              const int j = 2 * h + jj, g = j * GPK / 4;
-              const uint32_t w = j == 0 ? q[i].x : j == 1 ? q[i].y : j == 2 ? q[i].z : q[i].w;
-              uint32_t x[4];
-              w4_unpack<__half>(w, zz[i][g], x);
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t w = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
+              uint32_t y[4];
+              w4_unpack<__half>(w, zz[g], y);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&x[e]),
-                                          *reinterpret_cast<const __half2 *>(&sc[i][g]));
-                x[e] = *reinterpret_cast<const uint32_t *>(&y);
+                const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&y[e]),
+                                          *reinterpret_cast<const __half2 *>(&sc[g]));
+                x[4 * c + e] = *reinterpret_cast<const uint32_t *>(&v);
               }
-              *reinterpret_cast<uint4 *>(at + m * 128 + (((c + 4 * jj) ^ (m & 7)) << 4)) =
-                  make_uint4(x[0], x[1], x[2], x[3]);
             }
+            w4t_st16(lane_base + (uint32_t)(s * kW4tACols + 16 * jj), x);
           }
-          // generic-proxy writes of the tile become visible to the MMA
-          fence_proxy_async_smem();
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cta(&S.conv[s]);
+          if (lane == 0) mbar_arrive_cta(&S.full[s]);
           if (++s == a.stages) {
             s = 0;
             ph ^= 1u;
@@ -371,9 +436,9 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
         }
       }
     }
-  } else {
+  } else if (warp > 3) {
     const int q = warp & 3;  // TMEM lane quadrant of this warp
-    const int et = tid - 32 * (2 + kW4tConvWarps);
+    const int et = tid - 32 * (kW4tFirstConv + kW4tGroups * kW4tConvWarps);
     grid_dep_wait();
     for (int i = et; i < kW4tMaxN; i += 32 * kW4tEpiWarps)
       S.fac[i] = a.row_fac && i < a.rows ? a.row_fac[i] : 1.f;

@@ -1897,17 +1897,20 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
     const int n = std::min(fh::kW4tMaxN, rows - r0);
     a.rows = n;
     a.n_pad = (n + 15) / 16 * 16;
-    a.n_acc = 2;
+    a.stages = 4;
+    // accumulators and A tiles share the 512 TMEM columns
+    a.n_acc = 2 * a.n_pad + a.stages * fh::kW4tACols <= 512 ? 2 : 1;
     a.tmem_cols = 32;
-    while (a.tmem_cols < 2 * a.n_pad) a.tmem_cols *= 2;
+    while (a.tmem_cols < a.n_acc * a.n_pad + a.stages * fh::kW4tACols) a.tmem_cols *= 2;
     a.idesc = fh::s1tc_idesc(false, a.n_pad);
     a.row_fac = fac ? fac + r0 : nullptr;
     a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
     // stages of 64 columns; the rest of shared memory is the packed ring
-    a.stages = a.n_pad <= 128 ? 4 : 3;
     const size_t used = 1024 + sizeof(fh::W4TcCtrl) + a.stages * fh::w4t_stage_bytes(a.n_pad);
     a.packed = (int)std::min<size_t>(fh::kW4tMaxPacked, ((size_t)fh::kW4tSmemMax - used) /
                                                             fh::w4t_packed_bytes(gpk, zp));
+    if (a.packed < fh::kW4tMinPacked || a.stages < fh::kW4tMinStages)
+      return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
     const size_t smem = fh::w4t_smem_bytes(a.n_pad, a.stages, a.packed, gpk, zp);
     CUtensorMap tm;
     if (!encode_rows_map(&tm, reinterpret_cast<const char *>(hop) + (size_t)r0 * D * 2, FH_FP16, D,

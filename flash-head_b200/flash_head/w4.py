@@ -42,12 +42,12 @@ def _check_groups(D: int, group_size: int):
 
 
 def _pack_words(q: torch.Tensor, nb: int) -> torch.Tensor:
-    """[R, D] uint8 values (R a multiple of 128) -> int32 [R/128, nb, 128, 4, 4] words."""
+    """[R, D] uint8 values (R a multiple of 128) -> int32 [R/128, nb, 4, 128, 4] words."""
     R, D = q.shape
     if D < nb * _BLOCK:
         q = torch.nn.functional.pad(q, (0, nb * _BLOCK - D), value=8)
-    # tile, block, row, quad, word, e
-    x = q.view(R // _ROWS, _ROWS, nb, 4, 4, 8).permute(0, 2, 1, 4, 3, 5)
+    # tile, block, quad, row, word, e
+    x = q.view(R // _ROWS, _ROWS, nb, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)
     w = torch.zeros(x.shape[:-1], dtype=torch.int32, device=q.device)
     for e in range(8):
         w |= x[..., e].to(torch.int32) << (4 * (e // 2) + 16 * (e % 2))
@@ -55,10 +55,10 @@ def _pack_words(q: torch.Tensor, nb: int) -> torch.Tensor:
 
 
 def _unpack_words(w: torch.Tensor, D: int) -> torch.Tensor:
-    """The inverse of ``_pack_words``: int32 [t, nb, 128, 4, 4] -> [128 t, D] uint8."""
+    """The inverse of ``_pack_words``: int32 [t, nb, 4, 128, 4] -> [128 t, D] uint8."""
     x = torch.stack([(w >> (4 * (e // 2) + 16 * (e % 2))) & 15 for e in range(8)], dim=-1)
     t, nb = w.shape[0], w.shape[1]
-    x = x.permute(0, 2, 1, 4, 3, 5).reshape(_ROWS * t, nb * _BLOCK)
+    x = x.permute(0, 3, 1, 4, 2, 5).reshape(_ROWS * t, nb * _BLOCK)
     return x[:, :D].to(torch.uint8)
 
 
@@ -120,7 +120,7 @@ class W4Weight:
         nb, gpk = -(-D // _BLOCK), _BLOCK // group
         V_pad = -(-V // _ROWS) * _ROWS
         with torch.no_grad():
-            qw = torch.empty((V_pad // _ROWS, nb, _ROWS, 4, 4), dtype=torch.int32, device=q.device)
+            qw = torch.empty((V_pad // _ROWS, nb, 4, _ROWS, 4), dtype=torch.int32, device=q.device)
             step = max(_ROWS, _CHUNK // (nb * _BLOCK) // _ROWS * _ROWS)
             for lo in range(0, V_pad, step):
                 n = min(step, V_pad - lo)

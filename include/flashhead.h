@@ -375,8 +375,8 @@ FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
  *   hidden     D, columns: a multiple of group_size, at most FH_W4_MAX_HIDDEN
  *   group_size 32, 64 or 128
  *   dtype      FH_BF16 or FH_FP16: type of the scales, hidden states, outputs
- *   qweight    u32 [T][B][128][4][4], T = ceil(V / 128) tiles of 128 rows, B =
- *              ceil(D / 128): word j of quad c of row r of block b holds the 8
+ *   qweight    u32 [T][B][4][128][4], T = ceil(V / 128) tiles of 128 rows, B =
+ *              ceil(D / 128): word j of row r in quad c of block b holds the 8
  *              columns 128 b + 32 j + 8 c + e, column e = 2i in bits
  *              4i..4i+3, e = 2i + 1 in bits 16+4i..19+4i
  *   scales     [T][B][128][128 / group_size]; 0 in padded rows and groups

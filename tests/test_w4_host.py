@@ -40,10 +40,10 @@ def test_layout_words():
     q, s, z = _quantized(V, D, group)
     w = W4Weight.from_quantized(q, s, z)
     v = torch.stack([q & 15, q >> 4], 2).view(V, D).tolist()
-    assert w.qweight.shape == (1, 2, 128, 4, 4)  # rows padded to 128
+    assert w.qweight.shape == (1, 2, 4, 128, 4)  # rows padded to 128
     words = w.qweight.tolist()
     for r, b, c, j in [(0, 0, 0, 0), (7, 1, 3, 2), (19, 0, 1, 3), (16, 1, 2, 1)]:
-        word = words[r // 128][b][r % 128][c][j] & 0xFFFFFFFF
+        word = words[r // 128][b][c][r % 128][j] & 0xFFFFFFFF
         for e in range(8):
             at = 4 * (e // 2) + 16 * (e % 2)
             assert (word >> at) & 15 == v[r][128 * b + 32 * j + 8 * c + e]
