@@ -16,20 +16,20 @@
 // written and 16 KB read per 128 x 64 tile were most of the shared-memory
 // traffic that bound a first version (64 rows of a 1536 x 151936 head: 92 us).
 //
-// One persistent CTA per SM, 16 warps:
+// One persistent CTA per SM, 20 warps:
 //   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and
 //               zero points of 128 rows x 128 columns: two or three bulk copies)
 //               into a ring of their own, deep enough to keep HBM busy;
-//   warp 2      lane 0 brings the hidden tile of every 64 columns (TMA, 128-byte
-//               swizzle) into the stages (a thread of its own: a wait that
+//   warp 2      lane 0 brings the hidden tiles of every 128 columns (TMA, two of 64
+//               with the 128-byte swizzle) into the stages (a thread of its own: a wait that
 //               suspends the one for packed slots must not hold up these);
-//   warp 1      allocates TMEM; lane 0 issues tcgen05.mma (K = 16), A from
-//               tensor memory, B from shared memory;
-//   warps 4-11  unpack, in two groups of 4 on alternate blocks: a thread has one
+//   warp 1      allocates TMEM; one lane issues tcgen05.mma (K = 16), 8 per
+//               stage, A from tensor memory, B from shared memory;
+//   warps 4-15  unpack, in three groups of 4 on successive blocks: a thread has one
 //               weight row, i.e. one TMEM lane, reads its 64 bytes of the block
 //               and stores 32 columns' pairs (16 TMEM columns) at a time;
-//   warps 12-15 epilogue: a thread has one weight row and all hidden rows; up to
-//               192 hidden rows the accumulators are double-buffered.
+//   warps 16-19 epilogue: a thread has one weight row and all hidden rows; up to
+//               128 hidden rows the accumulators are double-buffered.
 // Bounds: HBM (the packed weight) up to about 64 rows, the tensor cores and
 // the hidden tiles' way from L2 at 256.
 // Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
@@ -41,22 +41,15 @@
 
 namespace fh {
 
-#ifndef W4_GROUPS
-#define W4_GROUPS 2
-#endif
 constexpr int kW4tConvWarps = 4;  // unpack one block together, a TMEM quadrant each
-constexpr int kW4tGroups = W4_GROUPS;      // of such warps, on successive blocks
+constexpr int kW4tGroups = 3;     // of such warps, on successive blocks (a launch may use fewer)
 constexpr int kW4tEpiWarps = 4;
 constexpr int kW4tFirstConv = 4;  // warp
+constexpr int kW4tEpi = kW4tFirstConv + kW4tGroups * kW4tConvWarps;
 constexpr int kW4tThreads = 32 * (kW4tFirstConv + kW4tGroups * kW4tConvWarps + kW4tEpiWarps);
-// A group skips the others' blocks; its parity waits are unambiguous while the
-// stage it comes to next was last used at most one use after those it knows to
-// be done (2 groups * 2 stages <= stages + 1), and likewise the packed slots.
-constexpr int kW4tMinStages = 2 * kW4tGroups - 1;
-constexpr int kW4tMinPacked = kW4tGroups + 2;
 constexpr int kW4tMaxN = 256;
 constexpr int kW4tMaxStages = 4;
-constexpr int kW4tACols = 32;  // TMEM columns of a stage's A tile: 64 f16 per row
+constexpr int kW4tACols = 64;  // TMEM columns of a stage's A tile: 128 f16 per row
 constexpr int kW4tMaxPacked = 12;
 constexpr int kW4tSmemMax = 227 * 1024;
 
@@ -66,11 +59,12 @@ struct W4TcArgs {
   const uint8_t *zeros;
   const float *row_mul;   // [128 * tiles] powers of two
   const float *row_fac;   // [rows] factors of the hidden rows, or null
-  int V, nb, nk;          // nk: 64-column stages, ceil(D / 64)
+  int V, D, nb;
   int tiles;
   int rows, n_pad;
-  int stages, packed, n_acc;
+  int stages, packed, n_acc, groups;
   int tmem_cols;
+  int vec;                // outputs take 16-byte stores (V, ldo and out allow them)
   uint32_t idesc;
   void *out;
   long long ldo;
@@ -89,13 +83,27 @@ struct W4TcCtrl {
   uint32_t tmem_base;
   uint32_t s_err;
   float fac[kW4tMaxN];
+  uint4 out[kW4tEpiWarps][128];  // 32 hidden rows x 32 weight rows, 16-bit
 };
+
+// Groups that may run. A group steps over the others' blocks, so that it knows of
+// a barrier's progress only what the order of the work implies; a parity wait
+// is unambiguous while the phase before the awaited one is known to be
+// complete. Having written block n, a group knows the MMAs up to block
+// n - stages, and with them the packed blocks up to there, to be done. Its next
+// block n + groups needs the stage's use two rounds back, n + groups - 2 stages,
+// and the packed slot's fill one round back, n + groups - packed, among them.
+__host__ __device__ inline int w4t_groups(int stages, int packed) {
+  int g = kW4tGroups;
+  while (g > 0 && (g > stages || packed < g + stages)) --g;
+  return g;
+}
 
 __host__ __device__ inline int w4t_packed_bytes(int gpk, bool zp) {
   return kW4Tile * kW4RowWords * 4 + kW4Tile * gpk * (zp ? 3 : 2);
 }
 __host__ __device__ inline size_t w4t_stage_bytes(int n_pad) {
-  return (size_t)n_pad * 128;
+  return (size_t)n_pad * 256;  // two tiles of 64 hidden columns
 }
 __host__ __device__ inline size_t w4t_smem_bytes(int n_pad, int stages, int packed, int gpk, bool zp) {
   return 1024 + stages * w4t_stage_bytes(n_pad) + (size_t)packed * w4t_packed_bytes(gpk, zp) +
@@ -122,6 +130,12 @@ __device__ __forceinline__ void w4t_commit(uint32_t bar) {
                : "memory");
 }
 
+__device__ __forceinline__ bool w4t_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(p));
+  return p != 0;
+}
 // D += A . B with A in tensor memory: row m in lane m, two f16 per column.
 __device__ __forceinline__ void w4t_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -205,7 +219,8 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
   constexpr int kScales = kW4Tile * GPK * 2, kZeros = ZP ? kW4Tile * GPK : 0;
   constexpr int pb = kWords + kScales + kZeros;
   W4TcCtrl &S = *reinterpret_cast<W4TcCtrl *>(pring + (size_t)a.packed * pb);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);  // uniform
   const int G = gridDim.x, t0 = blockIdx.x;
 
   if (tid == 0) {
@@ -235,7 +250,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = S.tmem_base;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, S.tmem_base, 0);
   const uint32_t a_col = (uint32_t)(a.n_acc * a.n_pad);  // first column of the A tiles
 
   if (warp == 0) {
@@ -281,14 +296,17 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
       bool ok = true;
       grid_dep_wait();  // the f16 copy of the hidden rows
       for (int t = t0; t < a.tiles && ok; t += G) {
-        for (int k = 0; k < a.nk; ++k) {
+        for (int kb = 0; kb < a.nb; ++kb) {
           if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
             break;
           }
-          mbar_expect_tx(&S.full[s], (uint32_t)(a.n_pad * 128));
-          tma_load_2d(ring + (size_t)s * sb, &tm_h, k * 64, 0, &S.full[s]);
+          const bool two = 128 * kb + 64 < a.D;
+          unsigned char *at = ring + (size_t)s * sb;
+          mbar_expect_tx(&S.full[s], (uint32_t)(a.n_pad * (two ? 256 : 128)));
+          tma_load_2d(at, &tm_h, 128 * kb, 0, &S.full[s]);
+          if (two) tma_load_2d(at + a.n_pad * 128, &tm_h, 128 * kb + 64, 0, &S.full[s]);
           issued[s] = (int)ph;
           if (++s == a.stages) {
             s = 0;
@@ -301,51 +319,53 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // one thread feeds the tensor cores between busy warps: its loop has
-      // addresses and descriptors ready
-      const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]);
-      const uint64_t bd0 = umma_desc_k(smem_u32(ring)), step = sb >> 4;
-      const uint32_t idesc = a.idesc;
-      uint64_t bd = bd0;
-      uint32_t at = tmem + a_col;
-      int s = 0;
-      uint32_t ph = 0u;
-      bool ok = true;
-      for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
-        const int buf = i % a.n_acc, use = i / a.n_acc;
-        if (use > 0) {
-          if (!mbar_wait(&S.acc_empty[buf], (uint32_t)((use - 1) & 1), a.polls)) {
-            atomicOr(&S.s_err, kErrCopyTimeout);
-            break;
-          }
+    // the whole warp walks the loop, so that descriptors and addresses are
+    // uniform; one lane issues (by a single lane inside a branch, an MMA took
+    // 50 clocks to issue)
+    const bool leader = w4t_elect();
+    const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]);
+    const uint64_t bd0 = umma_desc_k(smem_u32(ring)), step = sb >> 4;
+    const uint64_t half = (uint64_t)(a.n_pad * 128) >> 4;
+    const uint32_t idesc = a.idesc;
+    int s = 0;
+    uint32_t ph = 0u;
+    bool ok = true;
+    for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
+      const int buf = i % a.n_acc, use = i / a.n_acc;
+      if (use > 0 && !mbar_wait(&S.acc_empty[buf], (uint32_t)((use - 1) & 1), a.polls)) ok = false;
+      const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
+      for (int kb = 0; kb < a.nb && ok; ++kb) {
+        if (!w4t_wait(full0 + 8u * s, ph, a.polls)) {
+          ok = false;
+          break;
         }
-        const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
-        uint32_t more = 0u;
-        for (int k = 0; k < a.nk; ++k) {
-          if (!w4t_wait(full0 + 8u * s, ph, a.polls)) {
-            atomicOr(&S.s_err, kErrCopyTimeout);
-            ok = false;
-            break;
+        tc_fence_after();
+        const uint64_t bd = bd0 + step * s;
+        const uint32_t at = tmem + a_col + (uint32_t)(s * kW4tACols);
+        const int steps = min(8, (a.D - 128 * kb + 15) >> 4);
+        if (leader) {
+          if (steps == 8) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
+                      (kb | q) != 0 ? 1u : 0u);
+          } else {
+            for (int q = 0; q < steps; ++q)
+              w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
+                      (kb | q) != 0 ? 1u : 0u);
           }
-          tc_fence_after();
-          w4t_mma(acc, at, bd, idesc, more);
-          more = 1u;
-          w4t_mma(acc, at + 8u, bd + 2u, idesc, 1u);
-          w4t_mma(acc, at + 16u, bd + 4u, idesc, 1u);
-          w4t_mma(acc, at + 24u, bd + 6u, idesc, 1u);
           w4t_commit(empty0 + 8u * s);
-          bd += step;
-          at += kW4tACols;
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1u;
-            bd = bd0;
-            at = tmem + a_col;
-          }
         }
-        if (ok) tc_commit(&S.acc_full[buf]);
+        __syncwarp();
+        if (++s == a.stages) {
+          s = 0;
+          ph ^= 1u;
+        }
       }
+      if (ok && leader) tc_commit(&S.acc_full[buf]);
+    }
+    if (leader) {
+      if (!ok) atomicOr(&S.s_err, kErrCopyTimeout);
       tc_commit(&S.drain);
       if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
     }
@@ -355,20 +375,19 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16) + a_col;
     int s = 0, ps = 0, turn = 0;
     uint32_t ph = 0u, pph = 0u;
-    bool ok = true;
+    bool ok = group < a.groups;
     for (int t = t0; t < a.tiles && ok; t += G) {
       const float mul = __ldg(a.row_mul + t * kW4Tile + m);
       for (int kb = 0; kb < a.nb && ok; ++kb) {
         const bool mine = turn == group;
-        if (++turn == kW4tGroups) turn = 0;
+        if (++turn == a.groups) turn = 0;
         if (!mine) {  // another group's block: step over its slot and stages
           if (++ps == a.packed) {
             ps = 0;
             pph ^= 1u;
           }
-          s += min(2, a.nk - 2 * kb);
-          if (s >= a.stages) {
-            s -= a.stages;
+          if (++s == a.stages) {
+            s = 0;
             ph ^= 1u;
           }
           continue;
@@ -397,42 +416,38 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
           ps = 0;
           pph ^= 1u;
         }
+        if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
+          atomicOr(&S.s_err, kErrCopyTimeout);
+          ok = false;
+        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (2 * kb + h >= a.nk) break;
-          if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
-            atomicOr(&S.s_err, kErrCopyTimeout);
-            ok = false;
-          }
-          ok = __all_sync(0xFFFFFFFFu, ok);
-          if (!ok) break;
-          tc_fence_after();
+        for (int j = 0; j < 4; ++j) {
+          const int g = j * GPK / 4;
+          uint32_t x[16];
 #pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int j = 2 * h + jj, g = j * GPK / 4;
-            uint32_t x[16];
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t w = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
+            uint32_t y[4];
+            w4_unpack<__half>(w, zz[g], y);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t w = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
-              uint32_t y[4];
-              w4_unpack<__half>(w, zz[g], y);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&y[e]),
-                                          *reinterpret_cast<const __half2 *>(&sc[g]));
-                x[4 * c + e] = *reinterpret_cast<const uint32_t *>(&v);
-              }
+            for (int e = 0; e < 4; ++e) {
+              const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&y[e]),
+                                        *reinterpret_cast<const __half2 *>(&sc[g]));
+              x[4 * c + e] = *reinterpret_cast<const uint32_t *>(&v);
             }
-            w4t_st16(lane_base + (uint32_t)(s * kW4tACols + 16 * jj), x);
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cta(&S.full[s]);
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1u;
-          }
+          w4t_st16(lane_base + (uint32_t)(s * kW4tACols + 16 * j), x);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cta(&S.full[s]);
+        if (++s == a.stages) {
+          s = 0;
+          ph ^= 1u;
         }
       }
     }
@@ -453,25 +468,36 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int v = t * kW4Tile + 32 * q + lane;
+      const int v0 = t * kW4Tile + 32 * q, v = v0 + lane;
       const float back = 1.f / __ldg(a.row_mul + v);  // a power of two
-      T *out = reinterpret_cast<T *>(a.out) + v;
+      T *out = reinterpret_cast<T *>(a.out);
+      T *stage = reinterpret_cast<T *>(S.out[warp - kW4tEpi]);
       const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * a.n_pad);
       for (int c = 0; c < a.n_pad; c += 32) {
         uint32_t x[2][16];
         tc_ld16(base + (uint32_t)c, x[0]);
         if (c + 16 < a.n_pad) tc_ld16(base + (uint32_t)(c + 16), x[1]);
         tc_wait_ld();
-        if (v < a.V) {
+        // through shared memory: 16-byte stores instead of 2-byte ones
+        __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int r = c + 16 * u + j;
-              if (r < a.rows)
-                out[(long long)r * a.ldo] =
-                    from_float<T>(__uint_as_float(x[u][j]) * back * S.fac[r]);
-            }
+          for (int j = 0; j < 16; ++j)
+            stage[32 * (16 * u + j) + lane] =
+                from_float<T>(__uint_as_float(x[u][j]) * back * S.fac[min(c, kW4tMaxN - 32) + 16 * u + j]);
+        __syncwarp();
+        if (a.vec) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = c + 8 * i + (lane >> 2), vv = v0 + 8 * (lane & 3);
+            if (r < a.rows && vv < a.V)
+              *reinterpret_cast<uint4 *>(out + (long long)r * a.ldo + vv) =
+                  S.out[warp - kW4tEpi][32 * i + lane];
+          }
+        } else if (v < a.V) {
+          for (int j = 0; j < 32 && c + j < a.rows; ++j)
+            out[(long long)(c + j) * a.ldo + v] = stage[32 * j + lane];
         }
       }
       tc_fence_before();

@@ -1874,7 +1874,7 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
   a.row_mul = desc->row_mul;
   a.V = desc->vocab;
   a.nb = (D + fh::kW4Block - 1) / fh::kW4Block;
-  a.nk = (D + 63) / 64;
+  a.D = D;
   a.tiles = (desc->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
   a.ldo = out_stride;
   a.err = reinterpret_cast<uint32_t *>(ws);
@@ -1897,7 +1897,8 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
     const int n = std::min(fh::kW4tMaxN, rows - r0);
     a.rows = n;
     a.n_pad = (n + 15) / 16 * 16;
-    a.stages = 4;
+    // stages of 128 columns; the rest of shared memory is the packed ring
+    a.stages = a.n_pad <= 64 ? 4 : a.n_pad <= 128 ? 3 : 2;
     // accumulators and A tiles share the 512 TMEM columns
     a.n_acc = 2 * a.n_pad + a.stages * fh::kW4tACols <= 512 ? 2 : 1;
     a.tmem_cols = 32;
@@ -1905,12 +1906,12 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
     a.idesc = fh::s1tc_idesc(false, a.n_pad);
     a.row_fac = fac ? fac + r0 : nullptr;
     a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
-    // stages of 64 columns; the rest of shared memory is the packed ring
     const size_t used = 1024 + sizeof(fh::W4TcCtrl) + a.stages * fh::w4t_stage_bytes(a.n_pad);
     a.packed = (int)std::min<size_t>(fh::kW4tMaxPacked, ((size_t)fh::kW4tSmemMax - used) /
                                                             fh::w4t_packed_bytes(gpk, zp));
-    if (a.packed < fh::kW4tMinPacked || a.stages < fh::kW4tMinStages)
-      return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
+    a.groups = fh::w4t_groups(a.stages, a.packed);
+    if (a.groups < 1) return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
+    a.vec = desc->vocab % 8 == 0 && out_stride % 8 == 0 && aligned16(a.out);
     const size_t smem = fh::w4t_smem_bytes(a.n_pad, a.stages, a.packed, gpk, zp);
     CUtensorMap tm;
     if (!encode_rows_map(&tm, reinterpret_cast<const char *>(hop) + (size_t)r0 * D * 2, FH_FP16, D,
