@@ -16,7 +16,7 @@
 // written and 16 KB read per 128 x 64 tile were most of the shared-memory
 // traffic that bound a first version (64 rows of a 1536 x 151936 head: 92 us).
 //
-// One persistent CTA per SM, 20 warps:
+// One persistent CTA per SM, 24 warps:
 //   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and
 //               zero points of 128 rows x 128 columns: two or three bulk copies)
 //               into a ring of their own, deep enough to keep HBM busy;
@@ -25,10 +25,10 @@
 //               suspends the one for packed slots must not hold up these);
 //   warp 1      allocates TMEM; one lane issues tcgen05.mma (K = 16), 8 per
 //               stage, A from tensor memory, B from shared memory;
-//   warps 4-15  unpack, in three groups of 4 on successive blocks: a thread has one
+//   warps 4-19  unpack, in four groups of 4 on successive blocks: a thread has one
 //               weight row, i.e. one TMEM lane, reads its 64 bytes of the block
 //               and stores 32 columns' pairs (16 TMEM columns) at a time;
-//   warps 16-19 epilogue: a thread has one weight row and all hidden rows; up to
+//   warps 20-23 epilogue: a thread has one weight row and all hidden rows; up to
 //               128 hidden rows the accumulators are double-buffered.
 // Bounds: HBM (the packed weight) up to about 64 rows, the tensor cores and
 // the hidden tiles' way from L2 at 256.
@@ -42,7 +42,7 @@
 namespace fh {
 
 constexpr int kW4tConvWarps = 4;  // unpack one block together, a TMEM quadrant each
-constexpr int kW4tGroups = 3;     // of such warps, on successive blocks (a launch may use fewer)
+constexpr int kW4tGroups = 4;     // of such warps, on successive blocks (a launch may use fewer)
 constexpr int kW4tEpiWarps = 4;
 constexpr int kW4tFirstConv = 4;  // warp
 constexpr int kW4tEpi = kW4tFirstConv + kW4tGroups * kW4tConvWarps;
@@ -82,7 +82,7 @@ struct W4TcCtrl {
   uint64_t drain;
   uint32_t tmem_base;
   uint32_t s_err;
-  float fac[kW4tMaxN];
+  alignas(16) float fac[kW4tMaxN];
   uint4 out[kW4tEpiWarps][128];  // 32 hidden rows x 32 weight rows, 16-bit
 };
 
@@ -342,17 +342,16 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
         tc_fence_after();
         const uint64_t bd = bd0 + step * s;
         const uint32_t at = tmem + a_col + (uint32_t)(s * kW4tACols);
-        const int steps = min(8, (a.D - 128 * kb + 15) >> 4);
         if (leader) {
-          if (steps == 8) {
+          if (128 * kb + 128 <= a.D) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
               w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
-                      (kb | q) != 0 ? 1u : 0u);
+                      q > 0 ? 1u : (uint32_t)kb);
           } else {
-            for (int q = 0; q < steps; ++q)
+            for (int q = 0; 128 * kb + 16 * q < a.D; ++q)
               w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
-                      (kb | q) != 0 ? 1u : 0u);
+                      (uint32_t)(kb | q));
           }
           w4t_commit(empty0 + 8u * s);
         }
@@ -477,15 +476,18 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
         uint32_t x[2][16];
         tc_ld16(base + (uint32_t)c, x[0]);
         if (c + 16 < a.n_pad) tc_ld16(base + (uint32_t)(c + 16), x[1]);
+        float4 fac[8];  // read before the stores below, which may alias them
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fac[j] = *reinterpret_cast<const float4 *>(&S.fac[c + 4 * j]);
         tc_wait_ld();
         // through shared memory: 16-byte stores instead of 2-byte ones
         __syncwarp();
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            stage[32 * (16 * u + j) + lane] =
-                from_float<T>(__uint_as_float(x[u][j]) * back * S.fac[min(c, kW4tMaxN - 32) + 16 * u + j]);
+        for (int j = 0; j < 32; ++j) {
+          const float4 f = fac[j >> 2];
+          const float fj = (j & 3) == 0 ? f.x : (j & 3) == 1 ? f.y : (j & 3) == 2 ? f.z : f.w;
+          stage[32 * j + lane] = from_float<T>(__uint_as_float(x[j >> 4][j & 15]) * back * fj);
+        }
         __syncwarp();
         if (a.vec) {
 #pragma unroll
