@@ -26,10 +26,7 @@
 namespace fh {
 
 constexpr int kW4Warps = 16;
-#ifndef W4_AHEAD
-#define W4_AHEAD 2
-#endif
-constexpr int kW4Ahead = W4_AHEAD;  // blocks a warp loads ahead
+constexpr int kW4Ahead = 2;  // blocks a warp loads ahead
 constexpr int kW4Block = 128;                   // columns per block
 constexpr int kW4Tile = 128;                     // rows per tile
 constexpr int kW4RowWords = kW4Block / 8;        // u32 of one row's block
@@ -47,6 +44,7 @@ struct W4Args {
   void *out;    // [rows, ldo]
   long long ldo;
   int ksplit;   // warps that share a unit, each with every ksplit-th block
+  uint32_t mask, magic;  // kW4Mask and W4Num<T>::kMagic (see W4Bits)
   // probed clusters (k_w4_probes)
   const int64_t *ci;  // [rows, P]
   int P, K, cap;
@@ -96,9 +94,9 @@ template <>
 struct W4Num<__nv_bfloat16> {
   static constexpr uint32_t kMagic = 0x43004300u;
   __device__ __forceinline__ static uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
-                                     *reinterpret_cast<const __nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
+    uint32_t r;  // a * 1 - b, with b's signs set by the caller
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x3F803F80u), "r"(b));
+    return r;
   }
   __device__ __forceinline__ static float scale(uint32_t bits) {
     return __uint_as_float(bits << 16);
@@ -108,21 +106,71 @@ template <>
 struct W4Num<__half> {
   static constexpr uint32_t kMagic = 0x64006400u;
   __device__ __forceinline__ static uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&a),
-                              *reinterpret_cast<const __half2 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
   }
   __device__ __forceinline__ static float scale(uint32_t bits) {
     return __half2float(__ushort_as_half((unsigned short)bits));
   }
 };
 
-// The four pairs of a word as T x 2 of q - z; zz = magic + z in both halves.
+// The mask of a word's nibble pairs and the magic number, as values that the
+// compiler cannot know: with both in registers (x & mask) | magic is one
+// instruction, with literals it became two, and integer instructions are what
+// the unpacking has most of.
+constexpr uint32_t kW4Mask = 0x000F000Fu;
+struct W4Bits {
+  uint32_t mask, magic;
+  __device__ __forceinline__ uint32_t low(uint32_t x) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(magic));
+    return r;
+  }
+  __device__ __forceinline__ uint32_t high(uint32_t x, uint32_t mask16) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask16), "r"(magic));
+    return r;
+  }
+};
+
+// What turns a group's integers into q - z: -(magic + z) in both halves, and for
+// fp16 also -(64 + z).
 template <typename T>
-__device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t zz, uint32_t (&p)[4]) {
+struct W4Zero {
+  uint32_t z, z16;
+  __device__ __forceinline__ explicit W4Zero(uint32_t zero) {
+    z = (W4Num<T>::kMagic | (zero * 0x00010001u)) ^ 0x80008000u;
+    // 64 + z in fp16: 0x5400 is 64, a step 1/16
+    z16 = (0x54005400u | (zero * 0x00100010u)) ^ 0x80008000u;
+  }
+};
+
+// The four pairs of a word as T x 2 of q - z. (Integer operations bound the
+// unpacking: fp16 takes the odd pairs where they stand, as 1024 + 16 q, and an
+// exact fma, (1024 + 16 q) / 16 - (64 + z), so that a word is shifted once
+// instead of three times; bf16 has no bits for it.)
+template <typename T>
+__device__ __forceinline__ void w4_unpack(uint32_t w, const W4Bits &b, const W4Zero<T> &zero,
+                                          uint32_t (&p)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = W4Num<T>::sub(((w >> (4 * i)) & 0x000F000Fu) | W4Num<T>::kMagic, zz);
+  for (int i = 0; i < 4; ++i) p[i] = W4Num<T>::sub(b.low(w >> (4 * i)), zero.z);
+}
+template <>
+__device__ __forceinline__ void w4_unpack<__half>(uint32_t w, const W4Bits &b,
+                                                  const W4Zero<__half> &zero, uint32_t (&p)[4]) {
+  const uint32_t mask16 = b.mask << 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i ? w >> 8 : w;
+    p[2 * i] = W4Num<__half>::sub(b.low(x), zero.z);
+    p[2 * i + 1] = W4Num<__half>::fma(b.high(x, mask16), 0x2C002C00u, zero.z16);
+  }
 }
 
 // One warp's share of a 16-row block: the words, scales and zero points of
@@ -159,56 +207,67 @@ __device__ __forceinline__ void w4_load(const W4Args &a, int kb, int r0, int r1,
   }
 }
 
-// acc += the block's products; hb points at the lane's 16 bytes of hidden
-// column n = lane / 4 (this block, quad c) and hstride is the distance, in
-// bytes, of the next 8 columns of B. LOAD reads 16 bytes of hidden states.
-template <typename T, int GPK, bool ZP, int NT, typename Load>
-__device__ __forceinline__ void w4_block(const W4Frag<GPK, ZP> &f, Load load, float (&acc)[NT][4]) {
+// acc += the products of a block of TILES 16-row tiles; load(n, j) gives the 16
+// bytes of hidden column 8 n + lane / 4 that belong to word j of the lane's quad.
+template <typename T, int GPK, bool ZP, int NT, int TILES, typename Load>
+__device__ __forceinline__ void w4_block(const W4Frag<GPK, ZP> (&f)[TILES], const W4Bits &bits, Load load,
+                                         float (&acc)[TILES][NT][4]) {
   constexpr int JG = 4 / GPK;  // words per group
 #pragma unroll
   for (int gi = 0; gi < GPK; ++gi) {
-    uint32_t zz0, zz1;
-    if (ZP) {
-      const uint32_t z0 = ((uint32_t)f.z[0] >> (8 * gi)) & 0xFFu;
-      const uint32_t z1 = ((uint32_t)f.z[1] >> (8 * gi)) & 0xFFu;
-      zz0 = W4Num<T>::kMagic | (z0 * 0x00010001u);
-      zz1 = W4Num<T>::kMagic | (z1 * 0x00010001u);
-    } else {
-      zz0 = zz1 = W4Num<T>::kMagic | 0x00080008u;
-    }
-    float part[NT][4];
+    float part[TILES][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[n][i] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[t][n][i] = 0.f;
 #pragma unroll
     for (int jj = 0; jj < JG; ++jj) {
       const int j = gi * JG + jj;
-      const uint32_t w0 = j == 0 ? f.q[0].x : j == 1 ? f.q[0].y : j == 2 ? f.q[0].z : f.q[0].w;
-      const uint32_t w1 = j == 0 ? f.q[1].x : j == 1 ? f.q[1].y : j == 2 ? f.q[1].z : f.q[1].w;
-      uint32_t p0[4], p1[4];
-      w4_unpack<T>(w0, zz0, p0);
-      w4_unpack<T>(w1, zz1, p1);
-      const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]};
-      const uint32_t a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+      uint4 h[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 h = load(n, j);
-        const uint32_t b0[2] = {h.x, h.y}, b1[2] = {h.z, h.w};
-        mma16816<T>(part[n], a0, b0);
-        mma16816<T>(part[n], a1, b1);
+      for (int n = 0; n < NT; ++n) h[n] = load(n, j);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const uint32_t w0 = j == 0 ? f[t].q[0].x : j == 1 ? f[t].q[0].y : j == 2 ? f[t].q[0].z : f[t].q[0].w;
+        const uint32_t w1 = j == 0 ? f[t].q[1].x : j == 1 ? f[t].q[1].y : j == 2 ? f[t].q[1].z : f[t].q[1].w;
+        uint32_t p0[4], p1[4];
+        const W4Zero<T> z0(ZP ? ((uint32_t)f[t].z[0] >> (8 * gi)) & 0xFFu : 8u);
+        const W4Zero<T> z1(ZP ? ((uint32_t)f[t].z[1] >> (8 * gi)) & 0xFFu : 8u);
+        w4_unpack<T>(w0, bits, z0, p0);
+        w4_unpack<T>(w1, bits, z1, p1);
+        const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]};
+        const uint32_t a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint32_t b0[2] = {h[n].x, h[n].y}, b1[2] = {h[n].z, h[n].w};
+          mma16816<T>(part[t][n], a0, b0);
+          mma16816<T>(part[t][n], a1, b1);
+        }
       }
     }
-    const float s0 = W4Num<T>::scale(w4_scale_bits<GPK>(f.s[0], gi));
-    const float s1 = W4Num<T>::scale(w4_scale_bits<GPK>(f.s[1], gi));
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
-      acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
-      acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
-      acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+    for (int t = 0; t < TILES; ++t) {
+      const float s0 = W4Num<T>::scale(w4_scale_bits<GPK>(f[t].s[0], gi));
+      const float s1 = W4Num<T>::scale(w4_scale_bits<GPK>(f[t].s[1], gi));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[t][n][0] = fmaf(s0, part[t][n][0], acc[t][n][0]);
+        acc[t][n][1] = fmaf(s0, part[t][n][1], acc[t][n][1]);
+        acc[t][n][2] = fmaf(s1, part[t][n][2], acc[t][n][2]);
+        acc[t][n][3] = fmaf(s1, part[t][n][3], acc[t][n][3]);
+      }
     }
   }
+}
+
+__device__ __forceinline__ uint4 w4_lds(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at));
+  return v;
 }
 
 // Hidden rows in shared memory, 64 bytes of padding per row: the 8 lanes of a
@@ -243,25 +302,46 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
   }
   __syncthreads();
   float *red = reinterpret_cast<float *>(w4_sm + (size_t)(8 * NT) * rb);
-  const unsigned char *hl = w4_sm + (size_t)g * rb + c * 16;
+  const W4Bits bits{a.mask, a.magic};
+  const uint32_t hl = smem_u32(w4_sm) + (uint32_t)(g * rb + c * 16);
 
   const int ks = a.ksplit, kw = warp % ks;
   const int team = warp / ks, teams = kW4Warps / ks;
   const int units = a.tiles * (kW4Tile / 32);
   const int per_round = teams * gridDim.x;
   const int my_nb = (a.nb - kw + ks - 1) / ks;  // blocks of this warp
-  const int rounds = (units + per_round - 1) / per_round;
   const int first = team * gridDim.x + blockIdx.x;
+  const int rounds = first < units ? (units - 1 - first) / per_round + 1 : 0;  // of this team
 
   // the warp's blocks, unit after unit, are loaded kW4Ahead steps ahead
   W4Frag<GPK, ZP> f[kW4Ahead][2];
   int l_round = 0, l_b = 0;
+  using ST = typename W4Group<GPK>::S;
+  using ZT = typename W4Group<GPK>::Z;
+  const uint32_t *lq = nullptr;  // this lane's words, scales, zero points of the next block
+  const ST *ls = nullptr;
+  const ZT *lz = nullptr;
   auto fetch = [&](W4Frag<GPK, ZP>(&x)[2]) {
     if (l_round < rounds) {
-      const int u = min(first + l_round * per_round, units - 1), kb = kw + l_b * ks;
+      if (l_b == 0) {  // a new unit: 32 rows of a tile
+        const int u = first + l_round * per_round;  // below units
+        const long long blk = (long long)(u >> 2) * a.nb + kw;
+        const int row = 32 * (u & 3) + g;
+        lq = a.qw + blk * (kW4Tile * kW4RowWords) + (c * kW4Tile + row) * 4;
+        ls = reinterpret_cast<const ST *>(a.scales) + blk * kW4Tile + row;
+        if (ZP) lz = reinterpret_cast<const ZT *>(a.zeros) + blk * kW4Tile + row;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        w4_load<GPK, ZP>(a, kb, 32 * u + 16 * t + g, 32 * u + 16 * t + g + 8, c, x[t]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[t].q[i] = ldg_stream(lq + (16 * t + 8 * i) * 4);
+          x[t].s[i] = __ldg(ls + 16 * t + 8 * i);
+          if (ZP) x[t].z[i] = __ldg(lz + 16 * t + 8 * i);
+        }
+      lq += ks * (kW4Tile * kW4RowWords);
+      ls += ks * kW4Tile;
+      if (ZP) lz += ks * kW4Tile;
       if (++l_b == my_nb) {
         l_b = 0;
         ++l_round;
@@ -284,36 +364,34 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
    for (int ahead = 0; ahead < kW4Ahead; ++ahead) {
     if (step0 + ahead >= steps) break;
     const int kb = kw + b * ks;
-    const unsigned char *hk = hl + kb * (kW4Block * 2);
-    auto load = [&](int n, int j) { return lds128(hk + (size_t)(8 * n) * rb + j * 64); };
-#pragma unroll
-    for (int t = 0; t < 2; ++t) w4_block<T, GPK, ZP, NT>(f[ahead][t], load, acc[t]);
+    const uint32_t hk = hl + (uint32_t)(kb * (kW4Block * 2));
+    auto load = [&](int n, int j) { return w4_lds(hk + (uint32_t)(8 * n * rb + j * 64)); };
+    w4_block<T, GPK, ZP, NT, 2>(f[ahead], bits, load, acc);
     fetch(f[ahead]);
     if (++b < my_nb) continue;
     b = 0;
     const int u = first + round * per_round;
-    const bool live = u < units;
     ++round;
     if (ks > 1) {
       // sum the team's partial sums, warp kw = 0 keeps them (fixed order)
-      float *mine = red + (size_t)warp * NT * 32 * 8 + lane * (8 * NT);
-      if (live && kw > 0) {
+      float *mine = red + (size_t)warp * NT * 32 * 8 + lane * 4;
+      if (kw > 0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float4 *>(mine + (t * NT + n) * 4) =
+            *reinterpret_cast<float4 *>(mine + (t * NT + n) * 128) =
                 make_float4(acc[t][n][0], acc[t][n][1], acc[t][n][2], acc[t][n][3]);
       }
-      __syncthreads();
-      if (live && kw == 0) {
+      nbar_sync(1 + team, 32 * ks);
+      if (kw == 0) {
         for (int o = 1; o < ks; ++o) {
           const float *other = mine + (size_t)o * NT * 32 * 8;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const float4 v = *reinterpret_cast<const float4 *>(other + (t * NT + n) * 4);
+              const float4 v = *reinterpret_cast<const float4 *>(other + (t * NT + n) * 128);
               acc[t][n][0] += v.x;
               acc[t][n][1] += v.y;
               acc[t][n][2] += v.z;
@@ -321,9 +399,9 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
             }
         }
       }
-      __syncthreads();
+      nbar_sync(1 + team, 32 * ks);
     }
-    if (live && kw == 0) {
+    if (kw == 0) {
       T *out = reinterpret_cast<T *>(a.out);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -373,20 +451,20 @@ __global__ void __launch_bounds__(32 * kW4ProbeWarps) k_w4_probes(W4Args a) {
     }
   }
   const uint4 *h = reinterpret_cast<const uint4 *>(a.hidden) + (size_t)row * (a.D / 8);
-  float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+  float acc[1][1][4] = {{{0.f, 0.f, 0.f, 0.f}}};
   for (int kb = warp; kb < a.nb; kb += kW4ProbeWarps) {
-    W4Frag<GPK, ZP> f;
-    w4_load<GPK, ZP>(a, kb, wr[0], wr[1], c, f);
+    W4Frag<GPK, ZP> f[1];
+    w4_load<GPK, ZP>(a, kb, wr[0], wr[1], c, f[0]);
     // one hidden row: column n = 0 of B, the other 7 are zero
     auto load = [&](int, int j) {
       const int x = kb * 16 + j * 4 + c;
       return g == 0 && x < a.D / 8 ? ldg_keep(h + x) : make_uint4(0u, 0u, 0u, 0u);
     };
-    w4_block<T, GPK, ZP, 1>(f, load, acc);
+    w4_block<T, GPK, ZP, 1, 1>(f, W4Bits{a.mask, a.magic}, load, acc);
   }
   if (c == 0) {
-    red[warp][g] = acc[0][0];
-    red[warp][g + 8] = acc[0][2];
+    red[warp][g] = acc[0][0][0];
+    red[warp][g + 8] = acc[0][0][2];
   }
   __syncthreads();
   if (tid < 16 && s0 + tid < n) {

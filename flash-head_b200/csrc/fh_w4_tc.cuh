@@ -66,6 +66,7 @@ struct W4TcArgs {
   int tmem_cols;
   int vec;                // outputs take 16-byte stores (V, ldo and out allow them)
   uint32_t idesc;
+  uint32_t mask, magic;   // kW4Mask, W4Num<__half>::kMagic
   void *out;
   long long ldo;
   uint32_t *err;
@@ -371,6 +372,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
   } else if (warp >= kW4tFirstConv && warp < kW4tFirstConv + kW4tGroups * kW4tConvWarps) {
     const int group = (warp - kW4tFirstConv) / kW4tConvWarps;
     const int q4 = warp & 3, m = 32 * q4 + lane;  // this thread's row of the tile
+    const W4Bits bits{a.mask, a.magic};
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16) + a_col;
     int s = 0, ps = 0, turn = 0;
     uint32_t ph = 0u, pph = 0u;
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
         }
         const unsigned char *pk = pring + (size_t)ps * pb;
         uint4 q[4];
-        uint32_t sc[GPK], zz[GPK];
+        uint32_t sc[GPK], zz[GPK];  // scales (f16 pairs), zero points
 #pragma unroll
         for (int c = 0; c < 4; ++c) q[c] = lds128(pk + (c * kW4Tile + m) * 16);
 #pragma unroll
@@ -406,8 +408,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
           const uint16_t bits = reinterpret_cast<const uint16_t *>(pk + kWords)[m * GPK + g];
           const __half2 h = __float2half2_rn(W4Num<T>::scale(bits) * mul);
           sc[g] = *reinterpret_cast<const uint32_t *>(&h);
-          const uint32_t z = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
-          zz[g] = W4Num<__half>::kMagic | (z * 0x00010001u);
+          zz[g] = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_cta(&S.pempty[ps]);
@@ -425,12 +426,13 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int g = j * GPK / 4;
+          const W4Zero<__half> zero(zz[g]);
           uint32_t x[16];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t w = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
             uint32_t y[4];
-            w4_unpack<__half>(w, zz[g], y);
+            w4_unpack<__half>(w, bits, zero, y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&y[e]),
