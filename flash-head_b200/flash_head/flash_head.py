@@ -26,7 +26,10 @@ Differences from the reference, all deliberate:
     and a multinomial over the candidates) without its sequential kernel;
   * ``get_next_token_batched`` serves any number of decode rows (greedy or
     sampled) in one call; the reference-named methods keep the reference's
-    shape rules and NotImplementedError cases.
+    shape rules and NotImplementedError cases;
+  * ``get_next_token_filtered`` samples with per-row temperature, min-p, top-k
+    and top-p from given uniform numbers, and ``quantize_head`` gives the head
+    a 4-bit weight whose logits it then draws from.
 """
 
 from __future__ import annotations
@@ -142,6 +145,7 @@ class FlashHead(nn.Module):
         self.register_buffer("special_token_ids_tensor", torch.tensor(st, dtype=torch.int64),
                              persistent=False)
         self._native = None  # (buffer key, NativeHead)
+        self._w4 = None  # (buffer key, W4Weight of w_perm)
 
     # ------------------------------------------------------------------
     # Native head (device buffers + C handle)
@@ -212,6 +216,89 @@ class FlashHead(nn.Module):
         if do_sample and seed is None:
             seed, offset = self._next_seed()
         return self.native().dense_next_token(hidden, do_sample, temperature, seed or 0, offset)
+
+    # ------------------------------------------------------------------
+    # Filtered sampling and the 4-bit head
+    # ------------------------------------------------------------------
+    def quantize_head(self, group_size: int = 128, zeros: bool = False):
+        """Quantise ``w_perm`` to 4 bits (``flash_head.w4.W4Weight.from_dense``)
+        for ``candidate_logits``, ``head_logits`` and ``get_next_token_filtered``,
+        which use it from then on; returns the weight. Greedy and
+        temperature-only steps keep the 16-bit weight. A head moved or cast
+        afterwards has to be quantised again."""
+        from .w4 import W4Weight
+        w = W4Weight.from_dense(self.w_perm.view(-1, self._D), group_size, zeros)
+        self._w4 = ((self.w_perm.data_ptr(), self.w_perm.dtype, self.w_perm.device), w)
+        return w
+
+    def quantized(self):
+        """The 4-bit weight of the current ``w_perm``, or None."""
+        key = (self.w_perm.data_ptr(), self.w_perm.dtype, self.w_perm.device)
+        return self._w4[1] if self._w4 is not None and self._w4[0] == key else None
+
+    def candidate_logits(self, hidden: torch.Tensor, probes: Optional[torch.Tensor] = None):
+        """(logits [N, C], ids [N, C] int32) of a step's candidates: the tokens
+        of each row's probed clusters (``probes`` [N, p] int64; default: the
+        greedy stage 1), then the special tokens, -inf where a probed cluster
+        holds them already. Logits are in the head's dtype, from the 4-bit
+        weight after ``quantize_head``."""
+        from .fused import block_sparse_logits
+        from .w4 import w4_block_sparse_logits
+        nh = self.native()
+        h = nh._h(hidden)
+        N, cap, K = h.shape[0], self._cap, self._K
+        if probes is None:
+            probes = nh.top_clusters(h)
+        probes = probes.to(torch.int64)
+        w4 = self.quantized()
+
+        def product(ci, n, size):
+            if w4 is not None:
+                return w4_block_sparse_logits(h, w4, ci, n, size)
+            return block_sparse_logits(h, self.w_perm.view(-1), ci, n, size)
+        logits = product(probes, K, cap)
+        vocab = nh.bufs["vocab_map"]
+        ids = vocab.view(K, cap).index_select(0, probes.view(-1)).view(N, -1)
+        slots = nh.bufs["special_slots"]
+        if slots is not None:
+            at = slots.to(torch.int64).unsqueeze(0).expand(N, -1)
+            extra = product(at.contiguous(), K * cap, 1)
+            dup = ((at // cap).unsqueeze(2) == probes.unsqueeze(1)).any(dim=2)
+            logits = torch.cat([logits, extra.masked_fill(dup, float("-inf"))], dim=1)
+            ids = torch.cat([ids, vocab.index_select(0, slots).expand(N, -1)], dim=1)
+        return logits, ids
+
+    def head_logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        """[N, V] logits of the whole 4-bit head in ``w_perm`` order (the id of
+        column i is ``vocab_maps.view(-1)[i]``); needs ``quantize_head``."""
+        from .w4 import w4_logits
+        w4 = self.quantized()
+        if w4 is None:
+            raise RuntimeError("head_logits needs the 4-bit weight: call quantize_head() first")
+        return w4_logits(self.native()._h(hidden), w4)
+
+    def get_next_token_filtered(self, hidden: torch.Tensor,
+                                uniforms: Optional[torch.Tensor] = None, temperature=1.0,
+                                top_k=None, top_p=None, min_p=None, dense: bool = False,
+                                return_prob: bool = False):
+        """[N, D] hidden states -> [N] int64 ids sampled with temperature, min-p,
+        top-k and top-p (numbers or [N] tensors; temperature 0 is greedy) from
+        one uniform number per row (``flash_head.sampling.sample_logits``;
+        default: drawn from torch's generator of the device).
+
+        A row's candidates are those of ``candidate_logits``; ``dense``: the
+        whole vocabulary, through the 4-bit head. Ties go to the earlier
+        candidate: clusters by rising id, their tokens by rising vocab id.
+        ``return_prob``: also the drawn token's share of the kept mass [N]."""
+        from .sampling import sample_logits
+        if dense:
+            logits, ids = self.head_logits(hidden), self.native().bufs["vocab_map"]
+        else:
+            logits, ids = self.candidate_logits(hidden)
+        if uniforms is None:
+            uniforms = torch.rand(logits.shape[0], dtype=torch.float64, device=logits.device)
+        return sample_logits(logits, uniforms, temperature, top_k, top_p, min_p, ids=ids,
+                             return_prob=return_prob)
 
     def candidate_logprobs(self, hidden: torch.Tensor, token_ids: torch.Tensor,
                            num_logprobs: int):

@@ -82,13 +82,6 @@ def step_candidate_logprobs(token_ids: torch.Tensor, num_logprobs: int):
 
 # below this temperature a request is greedy (vLLM's sampler uses the same bound)
 _SAMPLING_EPS = 1e-5
-_warned = set()
-
-
-def _warn_once(key, msg):
-    if key not in _warned:
-        _warned.add(key)
-        logger.warning(msg)
 
 
 def _row_seed(rows, generators):
@@ -101,13 +94,35 @@ def _row_seed(rows, generators):
     return int(torch.randint(0, 2**62, (1,)).item())
 
 
+def _row_uniforms(rows, generators, device):
+    """One float64 uniform per row: from the row's own generator where its
+    request has one (so seeded requests repeat), else from torch's default."""
+    u = torch.rand(len(rows), dtype=torch.float64)
+    for i, r in enumerate(rows):
+        g = generators.get(int(r)) if generators else None
+        if g is not None:
+            u[i] = torch.rand((), generator=g, device=g.device, dtype=torch.float64).cpu()
+    return u.to(device)
+
+
+def _step_min_p(md, n: int):
+    """vLLM keeps min-p in a logits processor of the step; [n] or None."""
+    for proc in getattr(getattr(md, "logitsprocs", None), "argmax_invariant", None) or ():
+        v = getattr(proc, "min_p", None)
+        if isinstance(v, torch.Tensor) and getattr(proc, "min_p_count", 0):
+            v = v.reshape(-1)
+            return v[:n] if v.numel() >= n else None
+    return None
+
+
 def step_sampled_ids(greedy_ids: torch.Tensor, sampling_metadata):
     """The last FlashHead step's ids with each non-greedy request sampled at its
-    own temperature (FlashHead.get_next_token_batched(do_sample=True), one call
-    per distinct temperature); greedy rows keep greedy_ids. Where the reference
-    hook decodes every request greedily (patches/logits_processor.py:38), this
-    routes vLLM's per-request temperature to the sampling kernels. top-k / top-p
-    / min-p are not applied on this path (a warning says so once)."""
+    own settings; greedy rows keep greedy_ids. Where the reference hook decodes
+    every request greedily (patches/logits_processor.py:38), this routes vLLM's
+    per-request settings to the sampling kernels: with top-k, top-p or min-p in
+    the step, all its random rows in one call over the step's candidates
+    (FlashHead.get_next_token_filtered); with temperatures alone, one call per
+    distinct temperature (FlashHead.get_next_token_batched(do_sample=True))."""
     md = sampling_metadata
     if md is None or getattr(md, "all_greedy", True) or getattr(md, "temperature", None) is None:
         return greedy_ids
@@ -116,12 +131,21 @@ def step_sampled_ids(greedy_ids: torch.Tensor, sampling_metadata):
     n = greedy_ids.numel()
     if fh is _FLASH_HEAD_NOT_LOADED or fh is None or h is None or h.shape[0] != n:
         return greedy_ids
-    if getattr(md, "top_k", None) is not None or getattr(md, "top_p", None) is not None:
-        _warn_once("topkp", "[FlashHead] top-k / top-p are not applied on the FlashHead "
-                            "path: requests sample from the candidate set at their temperature")
     temps = md.temperature.detach().float().view(-1)[:n].cpu()
     out = greedy_ids.clone()
     random_rows = torch.nonzero(temps >= _SAMPLING_EPS).view(-1)
+    filters = {"top_k": getattr(md, "top_k", None), "top_p": getattr(md, "top_p", None),
+               "min_p": _step_min_p(md, n)}
+    if any(f is not None for f in filters.values()) and random_rows.numel():
+        idx = random_rows.to(h.device)
+        per_row = {k: None if f is None else f.reshape(-1)[:n].to(h.device).index_select(0, idx)
+                   for k, f in filters.items()}
+        ids = fh.get_next_token_filtered(
+            h.index_select(0, idx),
+            _row_uniforms(random_rows.tolist(), getattr(md, "generators", None), h.device),
+            temperature=temps[random_rows].to(h.device), **per_row)
+        out.view(-1).index_copy_(0, idx.to(out.device), ids.to(out.dtype).view(-1))
+        return out
     for t in torch.unique(temps[random_rows]).tolist():
         rows = random_rows[temps[random_rows] == t]
         idx = rows.to(h.device)

@@ -2,8 +2,8 @@
 patches/sampler.py:16-29): 1-D or [N, 1] input is treated as sampled ids and
 returned as ``SamplerOutput(sampled_token_ids=[N, 1] int32, ...)``. Requests
 with a temperature are sampled by FlashHead's sampling kernels at that
-temperature (``logits_processor.step_sampled_ids``) instead of decoded
-greedily.
+temperature, and with their top-k, top-p and min-p
+(``logits_processor.step_sampled_ids``), instead of decoded greedily.
 
 Where the reference always returns ``logprobs_tensors=None``, requests that
 ask for k logprobs get them over the step's candidate set
