@@ -17,19 +17,27 @@
 //
 // A row is read by a cluster of 1..8 CTAs; warp w of the cluster owns the
 // w-th contiguous segment of the row. Passes over the row:
-//   1  its largest logit (and every thread's own);
-//   2  where a filter keeps few entries (top-k up to 1024, min-p, or a top-p
-//      cut near the top), the candidates above a threshold that is known to
-//      hold the cut are collected (at most 2048), sorted in shared memory by
-//      one CTA, cut, and drawn from there. The threshold of a top-k is an
-//      order statistic of the threads' maxima; that of a top-p comes from the
-//      masses of 16 bands of logits (each thread sums bands of its own in
-//      shared memory: no atomics, a fixed order);
-//   3  otherwise (deep cuts) the band that holds the cut is split again until
-//      its entries fit the list; the kept mass is summed per segment, and the
-//      segment of the draw is scanned.
+//   1  its largest logit. Without a filter, the masses too. A row that does not
+//      fit in shared memory also yields its candidates, the entries above a
+//      threshold that a sample of the row gives, and under a top-p its mass in
+//      fp32, whose error is bounded;
+//   2  the candidates (at most 2048, in column order) are joined, sorted in
+//      shared memory by one CTA, cut, and drawn from there. A mass known to a
+//      factor is enough unless the cut differs between its two ends;
+//   3  a top-p whose cut lies deeper: fp32 masses of 46 bands of logits say where
+//      it lies (each thread sums bands of its own in shared memory: no atomics,
+//      a fixed order), then one pass collects the entries of the band as
+//      candidates and sums the exact masses above it. The segment of the draw is
+//      scanned.
 // Rows that resist (thousands of equal logits at a cut, top-k beyond 1024)
 // descend through 16 bands of keys per pass, exact for every input.
+//
+// Bound: a pass in fp64 is the cost, not the bytes: an exponential is 14 fp64
+// instructions, about 9 clocks of an SM per 32 entries, 33 us for 256 rows of
+// 128256 entries against 10 us of reading. Measured, bf16 rows of 128256 unless
+// said otherwise: one row with top-k and top-p 17.4 us; 64 rows of mixed filters
+// 54 us; 256 rows without a filter 66 us (1.0 TB/s); 256 fp32 rows of 151936
+// with top-p 208 us, 114 us where the cut lies among the first candidates.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -39,10 +47,14 @@
 namespace fh {
 
 constexpr int kSmpThreads = 256;
-// CTAs per SM: fp64 chains are long, and 32 warps cover them (16: 30 % slower)
+// CTAs per SM, of 64 registers a thread (rows in shared memory: half as many).
+// Two of 128 registers are better for fp64 chains alone (256 unfiltered rows: 60
+// us against 66), four for everything with candidates (64 rows of mixed filters:
+// 91 us against 77; 256 fp32 rows with top-p: 281 against 245).
 constexpr int kSmpResident = 4;
 constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBands = 16;
+constexpr int kSmpWin = 48;  // bands of a window, the parts above and below it among them
 constexpr int kSmpMaxCluster = 8;
 constexpr int kSmpChunk = 2048;  // vectors of the segment of the draw looked at together
 constexpr int kSmpList = 2048;   // candidates one CTA sorts
@@ -74,6 +86,7 @@ struct __align__(16) SmpShared {
       double mass[kSmpBands][kSmpThreads];
       uint32_t cnt[kSmpBands][kSmpThreads];
     } band;
+    float win[kSmpWin][kSmpThreads];
     struct {
       // the warps' candidates, key << 32 | column, by column; later the sorted
       // keys of the whole list
@@ -87,9 +100,9 @@ struct __align__(16) SmpShared {
   };
   // values exchanged between the CTAs of a cluster, double-buffered so that
   // one cluster barrier per exchange is enough
-  double x_mass[2][kSmpBands];
+  double x_mass[2][kSmpWin];
   unsigned long long x_cnt[2][kSmpBands];
-  double sum_mass[kSmpBands];
+  double sum_mass[kSmpWin];
   unsigned long long sum_cnt[kSmpBands];
   // per warp: kept mass of its segment in units of 2^warp_k, and ties; of the
   // first pass: largest logit, whether the mass has to be summed again
@@ -103,8 +116,7 @@ struct __align__(16) SmpShared {
   double scan_d[kSmpWarps];
   int scan_i[33];
   int part_n[kSmpWarps];  // candidates a warp found
-  ulonglong2 sample[kSmpThreads / 2];
-  float lo;
+  uint32_t warp_key[kSmpWarps];
   int verdict;
   int best, last;
   unsigned long long cut_key;
@@ -250,6 +262,7 @@ struct SmpCut {
 template <typename E, bool CACHED>
 struct SmpSpan {
   static constexpr int kVec = SmpElem<E>::kVec;
+  static constexpr bool kCached = CACHED;
   SmpRow<E> row;
   int v0, v1;
   int lane;
@@ -258,7 +271,7 @@ struct SmpSpan {
   // f(vector, kVec values), a lane every 32 vectors, by whole warps: lanes past
   // the segment get -inf. FIRST: the row is read for the first time; a CACHED
   // row then stays in shared memory.
-  template <bool FIRST, typename F>
+  template <bool FIRST, int kAhead = 4, typename F>
   __device__ __forceinline__ void walk(F f) const {
     constexpr uint32_t no = SmpElem<E>::kNone;
     float x[kVec];
@@ -277,12 +290,12 @@ struct SmpSpan {
       }
     } else {
       int v = v0;
-      for (; v + 128 <= v1; v += 128) {
-        uint4 u[4];
+      for (; v + 32 * kAhead <= v1; v += 32 * kAhead) {
+        uint4 u[kAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = row.raw(v + lane + 32 * i);
+        for (int i = 0; i < kAhead; ++i) u[i] = row.raw(v + lane + 32 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
           row.unpack(u[i], x);
           f(v + lane + 32 * i, x);
         }
@@ -321,10 +334,10 @@ __device__ __forceinline__ void smp_exchange(Ctx &C, int n) {
     for (int r = 0; r < C.size; ++r) {
       const SmpShared *R = cl.map_shared_rank(&C.S, r);
       d += R->x_mass[b][C.tid];
-      k += R->x_cnt[b][C.tid];
+      if (C.tid < kSmpBands) k += R->x_cnt[b][C.tid];
     }
     C.S.sum_mass[C.tid] = d;
-    C.S.sum_cnt[C.tid] = k;
+    if (C.tid < kSmpBands) C.S.sum_cnt[C.tid] = k;
   }
   __syncthreads();
 }
@@ -522,51 +535,20 @@ __device__ __noinline__ uint32_t smp_min_key(float m, float T, float min_p) {
   return hi;
 }
 
-// Bands of a top-p descent: a run of the order, logits in (lo, hi], split in
-// 16 by depth; the last band also takes what lies deeper. Any rounding of the
-// depth keeps the bands runs of the order, since it is monotone.
-struct SmpBands {
-  float lo, hi;        // logits
-  float from, scale;   // depth of the first band, bands per unit of depth
-  __device__ __forceinline__ int band(float d) const {
-    return (int)fmaxf(0.f, fminf(__fmul_rn(d - from, scale), (float)(kSmpBands - 1)));
-  }
-  __device__ __forceinline__ float begin(int j) const { return from + (float)j / scale; }
-};
-
-// Largest logit in (b.lo, b.hi] that lies in band j or behind (b.lo if none):
-// each round of 32 probes by a warp's lanes narrows its key 32-fold.
-__device__ __noinline__ float smp_band_top(const SmpMass &w, const SmpBands &b, int j) {
-  const int lane = threadIdx.x & 31;
-  uint32_t lo = smp_key(b.lo), hi = smp_key(b.hi);  // lo holds, keys above hi do not
-  while (lo < hi) {
-    const uint32_t step = (hi - lo + 31u) / 32u;
-    const uint32_t k = (hi - lo) / step > (uint32_t)lane ? lo + step * (uint32_t)(lane + 1) : hi;
-    const unsigned in = __ballot_sync(0xFFFFFFFFu, b.band(w.depth(unmono(k))) >= j);
-    const int n = in == 0xFFFFFFFFu ? 32 : __ffs(~in) - 1;  // probes that hold
-    const uint32_t l = n ? __shfl_sync(0xFFFFFFFFu, k, n - 1) : lo;
-    const uint32_t h = n < 32 ? __shfl_sync(0xFFFFFFFFu, k, n) - 1u : l;
-    lo = l;
-    hi = max(l, h);
-  }
-  return unmono(lo);
-}
-
 // The entries that `hit` marks of a warp's vectors (a lane's first column c0)
 // into the warp's part of the list, in column order; n counts on past its end.
 template <int kVec>
 __device__ __forceinline__ void smp_append(const float *f, int c0, uint32_t hit,
                                            unsigned long long *part, int &n) {
   if (__any_sync(0xFFFFFFFFu, hit)) {
-    const int mine = __popc(hit);
-    int incl = mine;
+    const unsigned below = (1u << (threadIdx.x & 31)) - 1u;
+    int at = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-      if ((int)(threadIdx.x & 31) >= o) incl += t;
+    for (int i = 0; i < kVec; ++i) {
+      const unsigned in = __ballot_sync(0xFFFFFFFFu, (hit >> i) & 1u);
+      at += __popc(in & below);
+      n += __popc(in);
     }
-    int at = n + incl - mine;
-    n += __shfl_sync(0xFFFFFFFFu, incl, 31);
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
       if ((hit >> i) & 1u) {
@@ -577,11 +559,11 @@ __device__ __forceinline__ void smp_append(const float *f, int c0, uint32_t hit,
   }
 }
 
-// Exchanges the number of candidates (and x_mass[0] of the caller): the
+// Exchanges the number of candidates (and x_mass[0..n) of the caller): the
 // cluster's total in sum_cnt[0], beyond kSmpList also where one warp found
 // more than its part holds.
 template <typename Ctx>
-__device__ __forceinline__ void smp_count_list(Ctx &C) {
+__device__ __forceinline__ void smp_count_list(Ctx &C, int masses = 1) {
   SmpShared &S = C.S;
   __syncthreads();
   if (C.warp == 0) {
@@ -590,7 +572,7 @@ __device__ __forceinline__ void smp_count_list(Ctx &C) {
     n = __reduce_add_sync(0xFFFFFFFFu, n);
     if (C.lane == 0) S.x_cnt[C.phase & 1][0] = over ? (unsigned long long)kSmpList + 1ull : n;
   }
-  smp_exchange(C, 1);
+  smp_exchange(C, masses);
 }
 
 // Rank 0 joins the warps' parts into its list, in column order (a cluster
@@ -775,7 +757,7 @@ __device__ __noinline__ SmpPick smp_pick(SmpShared &S, SmpMass w, int n, uint32_
     }
     (void)smp_count_scan(S, reach | (reach_most << 16), &all);
     // the cut is the same for the least and the most that the target can be
-    if (sure) *sure = (all & 0xFFFF) == (all >> 16) && most < z;
+    if (sure) *sure = (all & 0xFFFF) == (all >> 16) && most < above + z;
     keep = max(1, all & 0xFFFF);
   }
   SmpPick pick;
@@ -1039,36 +1021,6 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   }
 }
 
-// Masses of the 16 bands of the logits in (b.lo, b.hi], per thread. WIDE: most
-// of the row lies there.
-constexpr float kSmpBand0 = 1.5f;  // depth of a first band: 15 hold all but 2^-22
-template <bool WIDE, typename Span>
-__device__ __noinline__ void smp_bands(Span span, SmpMass w, SmpBands b, double *mine) {
-  constexpr int kVec = Span::kVec;
-#pragma unroll
-  for (int i = 0; i < kSmpBands; ++i) mine[i * kSmpThreads] = 0.0;
-  const float least = fmaxf(b.lo, w.xlo), hi = b.hi;
-  span.template walk<false>([&](int, const float *f) {
-    if (WIDE) {
-#pragma unroll
-      for (int h = 0; h < kVec; h += 4) {
-        double x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = w.raw(f[h + i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = b.band(w.depth(f[h + i]));
-          if (f[h + i] > least) mine[j * kSmpThreads] += x[i];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (f[i] > least && f[i] <= hi) mine[b.band(w.depth(f[i])) * kSmpThreads] += w.raw(f[i]);
-    }
-  });
-}
-
 // The first pass of the list path: the thread's largest logit, the entries
 // above `lo` into the CTA's list and, MASS, the row's mass relative to `ref` in
 // fp32, kSmpSlack of it off at most: with t = (x - ref) c, the difference is
@@ -1081,6 +1033,17 @@ __device__ __forceinline__ float smp_ex2(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
   return y;
 }
+struct SmpFloat {
+  float ref, c_hi, c_lo, xcut;
+  __device__ __forceinline__ SmpFloat(float ref_, double c)
+      : ref(ref_), c_hi((float)c), c_lo((float)(c - (double)(float)c)),
+        xcut(ref_ - 100.f / (float)c) {}
+  __device__ __forceinline__ float operator()(float f) const {
+    const float x = f - ref, t = x * c_hi;
+    const float e = smp_ex2(t), d = fmaf(x, c_lo, fmaf(x, c_hi, -t));
+    return fmaf(e, d * 0.69314718f, e);
+  }
+};
 struct SmpFirst {
   double z;
   float top;
@@ -1089,7 +1052,7 @@ template <bool MASS, typename Span>
 __device__ __noinline__ SmpFirst smp_first(Span span, float lo, float ref, double c,
                                            unsigned long long *part, int *part_n) {
   constexpr int kVec = Span::kVec;
-  const float c_hi = (float)c, c_lo = (float)(c - (double)c_hi), xcut = ref - 100.f / c_hi;
+  const SmpFloat e2(ref, c);
   SmpFirst r{0.0, -INFINITY};
   int n = 0;
   span.template walk<true>([&](int v, const float *f) {
@@ -1099,10 +1062,8 @@ __device__ __noinline__ SmpFirst smp_first(Span span, float lo, float ref, doubl
     for (int i = 0; i < kVec; ++i) {
       if (i) top = fmaxf(top, f[i]);
       if (MASS) {
-        const float x = f[i] - ref, t = x * c_hi;
-        const float e = smp_ex2(t), d = fmaf(x, c_lo, fmaf(x, c_hi, -t));
-        const float y = fmaf(e, d * 0.69314718f, e);
-        if (f[i] > xcut) sum += y;
+        const float y = e2(f[i]);
+        if (f[i] > e2.xcut) sum += y;
       }
     }
     r.top = fmaxf(r.top, top);
@@ -1132,23 +1093,295 @@ __device__ __forceinline__ void smp_sample(Ctx &C, float want, float &lo, float 
 #pragma unroll
   for (int i = 1; i < kVec; ++i) x = fmaxf(x, f[i]);
   x = fmaxf(x, -INFINITY);  // all NaN
-  // every thread counts the larger ones (equal ones by thread)
-  const unsigned long long key = ((unsigned long long)smp_key(x) << 32) | (uint32_t)~C.tid;
-  reinterpret_cast<unsigned long long *>(S.sample)[C.tid] = key;
-  __syncthreads();
-  int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < kSmpThreads / 2; ++i) {
-    const ulonglong2 k = S.sample[i];
-    above += (int)(k.x > key) + (int)(k.y > key);
-  }
+  // its key's upper bits, by halving: a threshold slightly below
+  const uint32_t key = smp_key(x);
   const int r = min(kSmpThreads, max(4, (int)(want * (kSmpThreads * kVec) / (float)C.span.row.n)));
-  if (above == r - 1) S.lo = x;
-  if (above == 0) S.warp_f[0] = x;
+  const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, key);
+  if (C.lane == 0) S.warp_key[C.warp] = top;
+  uint32_t pre = 0u;
+#pragma unroll 1
+  for (int bit = 31; bit >= 12; --bit) {
+    const uint32_t t = pre | (1u << bit);
+    if (__syncthreads_count(key >= t) >= r) pre = t;
+  }
+  uint32_t most = 0u;
+#pragma unroll
+  for (int i = 0; i < kSmpWarps; ++i) most = max(most, S.warp_key[i]);
+  ref = unmono(most);
+  // (at most what the r-th largest is, and -inf for -inf)
+  lo = pre > smp_key(-INFINITY) ? smp_float(pre) : -INFINITY;
+}
+
+// The window of a deep top-p cut: logits up to `hi` in 46 bands of equal width,
+// band 0 above it, band 47 below. Band j is (edge(j), edge(j - 1)].
+struct SmpWindow {
+  float hi, scale;  // scale: bands per logit
+  __device__ __forceinline__ int band(float x) const {
+    const float y = fminf(fmaxf(fmaf(hi - x, scale, 0.5f), 0.f), (float)(kSmpWin - 1));
+    return __float_as_int(y + 8388608.f) & 63;  // the nearest integer
+  }
+  __device__ __forceinline__ float edge(int j) const { return hi - (float)j / scale; }
+};
+
+// Per-thread masses of a window's bands, of the logits above `base`, in fp32
+// relative to `ref`; returns the thread's largest logit. (Bands of the thread's
+// own: no atomics, a fixed order.) The row's mass is off by kSmpSlack, and 2^-24
+// for every addition: the thread's entries, and 16 more.
+template <typename Span>
+__device__ __noinline__ float smp_window(Span span, SmpWindow win, float base, float ref, double c,
+                                         float *mine) {
+  constexpr int kVec = Span::kVec;
+  const SmpFloat e2(ref, c);
+  const float xcut = fmaxf(base, e2.xcut);
+  float top = -INFINITY;
+#pragma unroll 8
+  for (int i = 0; i < kSmpWin; ++i) mine[i * kSmpThreads] = 0.f;
+  span.template walk<false>([&](int, const float *f) {
+#pragma unroll
+    for (int h = 0; h < kVec; h += 4) {
+      float e[4];
+      int j[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = f[h + i];
+        top = fmaxf(top, x);
+        e[i] = e2(x);
+        e[i] = x > xcut ? e[i] : 0.f;
+        j[i] = win.band(x) * kSmpThreads;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[j[i]] += e[i];
+    }
+  });
+  return top;
+}
+
+// Sums the threads' window bands over the CTA, in a fixed order.
+template <typename Ctx>
+__device__ __forceinline__ void smp_window_sums(Ctx &C, double *out) {
+  static_assert(kSmpWin % kSmpWarps == 0, "as many bands to every warp");
   __syncthreads();
-  lo = S.lo;
-  ref = S.warp_f[0];
+  float d[kSmpWin / kSmpWarps];
+#pragma unroll
+  for (int b = 0; b < kSmpWin / kSmpWarps; ++b) {
+    d[b] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSmpThreads; i += 32)
+      d[b] += C.S.win[b * kSmpWarps + C.warp][i + C.lane];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int b = 0; b < kSmpWin / kSmpWarps; ++b) d[b] += __shfl_xor_sync(0xFFFFFFFFu, d[b], o);
+  if (C.lane < kSmpWin / kSmpWarps) {
+    float mine = d[0];
+#pragma unroll
+    for (int b = 1; b < kSmpWin / kSmpWarps; ++b) mine = C.lane == b ? d[b] : mine;
+    out[C.lane * kSmpWarps + C.warp] = (double)mine;
+  }
+}
+
+// One pass: exact masses of the logits above `hi` and above `base`, per thread, and
+// the entries in (lo, hi] into the warp's part of the list.
+struct SmpExact {
+  double above, all;
+};
+template <typename Span>
+__device__ __noinline__ SmpExact smp_exact(Span span, SmpMass w, float base, float lo, float hi,
+                                           unsigned long long *part, int *part_n) {
+  constexpr int kVec = Span::kVec;
+  double all0 = 0.0, all1 = 0.0, above0 = 0.0, above1 = 0.0;
+  int n = 0;
+  span.template walk<false, kVec == 4 ? 2 : 1>([&](int v, const float *f) {
+    uint32_t hit = 0u;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) hit |= f[i] > lo && f[i] <= hi ? 1u << i : 0u;
+#pragma unroll
+    for (int h = 0; h < kVec; h += 4) {
+      double x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w.raw(f[h + i]);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        if (f[h + i] > base) all0 += x[i];
+        if (f[h + i + 1] > base) all1 += x[i + 1];
+        if (f[h + i] > hi) above0 += x[i];
+        if (f[h + i + 1] > hi) above1 += x[i + 1];
+      }
+    }
+    smp_append<kVec>(f, span.row.column(v), hit, part, n);
+  });
+  if (span.lane == 0) *part_n = n;
+  return SmpExact{above0 + above1, all0 + all1};
+}
+
+// A deep top-p cut of the logits above `base`: the window's masses, relative to
+// `ref`, are in sum_mass; m is the row's largest logit. Finds the bands that hold
+// the cut (a window of their own if they hold too many entries). Where that is
+// near the top, the candidates are the whole prefix, and a mass known to a
+// factor may do (a row in shared memory is summed at once); otherwise one pass gives the exact masses and the candidates,
+// then come the cut and the segments' masses for the draw. kDrawn: it has been
+// drawn. kLost: nothing but the passes.
+enum SmpDeep { kLost, kCut, kDrawn };
+template <typename E, typename Ctx>
+__device__ __forceinline__ SmpDeep smp_deep(Ctx &C, const SampleArgs &a, const SmpMass &w,
+                                            SmpWindow win, float base, float m, float ref,
+                                            double c, float p, int r, double u, SmpCut &cut) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cl = cg::this_cluster();
+  SmpShared &S = C.S;
+  const int lane = C.lane;
+  const float cf = (float)c;
+  float lo = 0.f, hi = 0.f;
+  bool whole = false;  // (lo, m] is short enough
+  double z;
+#pragma unroll 1
+  for (int level = 0;; ++level) {
+    // lane i has bands 2 i and 2 i + 1
+    const bool mine = lane < kSmpWin / 2;
+    const double a0 = mine ? S.sum_mass[2 * lane] : 0.0, a1 = mine ? S.sum_mass[2 * lane + 1] : 0.0;
+    double incl = a0 + a1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    z = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    // the band that reaches a mass
+    const auto reach = [&](double need) {
+      const unsigned b0 = __ballot_sync(0xFFFFFFFFu, mine && incl - a1 >= need);
+      const unsigned b1 = __ballot_sync(0xFFFFFFFFu, mine && incl >= need);
+      const int l = __ffs(b0 | b1) - 1;
+      return b0 | b1 ? 2 * l + ((b0 >> l) & 1u ? 0 : 1) : kSmpWin - 1;
+    };
+    // 2^-12 of room each way
+    const int j0 = reach((double)p * z * (1.0 - 0x1p-12));
+    const int j1 = reach((double)p * z * (1.0 + 0x1p-12));
+    // entries of a band: at most its mass over the least of theirs
+    const float n0 = a0 > 0.0 ? (float)a0 * smp_ex2((ref - win.edge(2 * lane)) * cf) : 0.f;
+    const float n1 = a1 > 0.0 ? (float)a1 * smp_ex2((ref - win.edge(2 * lane + 1)) * cf) : 0.f;
+    float prefix = (2 * lane <= j1 ? n0 : 0.f) + (2 * lane + 1 <= j1 ? n1 : 0.f);
+    float in = (2 * lane >= j0 && 2 * lane <= j1 ? n0 : 0.f) +
+               (2 * lane + 1 >= j0 && 2 * lane + 1 <= j1 ? n1 : 0.f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      prefix += __shfl_xor_sync(0xFFFFFFFFu, prefix, o);
+      in += __shfl_xor_sync(0xFFFFFFFFu, in, o);
+    }
+    __syncthreads();
+    if (!(z > 0.0)) return kLost;
+    const bool last = j1 == kSmpWin - 1;  // (it has no lower edge)
+    // (a logit on an edge may be in either band: 1 % of one more each way)
+    hi = j0 > 0 ? fminf(win.edge(j0 - 1) + 0.01f / win.scale, m) : m;
+    lo = last ? win.edge(kSmpWin - 2) - 24.f / cf : win.edge(j1) - 0.01f / win.scale;
+    lo = fmaxf(fminf(lo, nextafterf(hi, -INFINITY)), base);
+    const bool fits = !last || lo == base;
+    whole = fits && prefix <= (float)kSmpList;
+    if (whole || (fits && in <= (float)kSmpList)) break;
+    if (level == 3) return kLost;
+    win.hi = hi;
+    win.scale = (float)(kSmpWin - 2) / (hi - lo);
+    if (!(win.scale > 0.f && win.scale < 1e30f)) return kLost;
+    smp_window(C.span, win, base, ref, c, &S.win[0][C.tid]);
+    smp_window_sums(C, S.x_mass[C.phase & 1]);
+    smp_exchange(C, kSmpWin);
+  }
+  const uint32_t least = cut.key;
+  if (whole && decltype(C.span)::kCached) {
+    hi = m;
+  } else if (whole) {
+    const int got = smp_collect(C, lo, m);
+    if (got > 0 && got <= kSmpList) {
+      hi = m;
+      if (C.rank == 0) {
+        const double slack = kSmpSlack + 0x1p-24 * (16.0 + (double)C.span.row.n /
+                                                               (double)(kSmpThreads * C.size));
+        const double target = (double)p * z * exp2((double)ref * w.c - w.k0);
+        bool sure = false;
+        const SmpPick pick = smp_pick(S, w, got, least, 0, (double)p, target * (1.0 - slack), 0.0,
+                                      target * (1.0 + slack), &sure);
+        sure = sure && !w.held && target > 0.0;
+        if (C.tid == 0) S.verdict = sure;
+        if (sure) smp_draw_list<E>(S, a, w, r, got, pick, u);
+      }
+      cl.sync();
+      const int ok = cl.map_shared_rank(&S, 0)->verdict;
+      cl.sync();
+      if (ok) return kDrawn;
+    }
+  }
+  hi = fmaxf(hi, w.xlo);  // masses below are none
+  SmpExact e = smp_exact(C.span, w, fmaxf(base, w.xlo), lo, hi, S.list.part[C.warp], &S.part_n[C.warp]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    e.above += __shfl_xor_sync(0xFFFFFFFFu, e.above, o);
+    e.all += __shfl_xor_sync(0xFFFFFFFFu, e.all, o);
+  }
+  if (C.lane == 0) {
+    S.warp_d[C.warp] = e.above;
+    S.warp_k[C.warp] = w.k0;
+    S.scan_d[C.warp] = e.all;
+  }
   __syncthreads();
+  if (C.tid == 0) {
+    double above = 0.0, all = 0.0;
+    for (int i = 0; i < kSmpWarps; ++i) {
+      above += S.warp_d[i];
+      all += S.scan_d[i];
+    }
+    S.x_mass[C.phase & 1][0] = above;
+    S.x_mass[C.phase & 1][1] = all;
+  }
+  smp_count_list(C, 2);
+  const double above = S.sum_mass[0], target = (double)p * S.sum_mass[1];
+  const unsigned long long listed = S.sum_cnt[0];
+  if (listed == 0 || listed > (unsigned long long)kSmpList || !(above < target)) return kLost;
+  smp_gather(C);
+  if (C.rank == 0) {
+    bool sure = false;
+    const SmpPick pick = smp_pick(S, w, (int)listed, least, 0, (double)p, target, above, target, &sure);
+    if (C.tid == 0) {
+      S.cut_key = pick.key;
+      S.cut_ties = pick.ties;
+      S.verdict = sure;
+    }
+    if (sure && hi == m) smp_draw_list<E>(S, a, w, r, (int)listed, pick, u);
+  }
+  cl.sync();
+  const SmpShared *R = cl.map_shared_rank(&S, 0);
+  if (!R->verdict) {
+    cl.sync();
+    return kLost;
+  }
+  if (hi == m) {
+    cl.sync();
+    return kDrawn;
+  }
+  cut.key = (uint32_t)R->cut_key;
+  cut.ties = R->cut_ties;
+  // the segment's kept candidates (rank 0 sorted over its parts: its own lead
+  // its list)
+  int first = 0;
+  for (int i = 0; i < C.warp; ++i) first += S.part_n[i];
+  double kept = 0.0;
+  int ties = 0;
+  for (int i = C.lane; i < S.part_n[C.warp]; i += 32) {
+    const uint32_t key = C.rank == 0 ? S.list.key[first + i]
+                                     : (uint32_t)(S.list.part[C.warp][i] >> 32);
+    if (key > cut.key) kept += w(unmono(key));
+    ties += key == cut.key;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    kept += __shfl_xor_sync(0xFFFFFFFFu, kept, o);
+    ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
+  }
+  if (C.lane == 0) {
+    S.warp_d[C.warp] += kept;
+    S.warp_i[C.warp] = ties;
+  }
+  cl.sync();
+  return kCut;
 }
 
 // CACHED: every lane's share of the row is at most kSmpCache vectors, kept in
@@ -1195,6 +1428,7 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
   int first = 0x7FFFFFFF;
   SmpMass w(0.f, T);
   int bad = 1;
+  const double c = 1.4426950408889634 / (double)T;
   if (all) {
     float f[kVec];
     ref = -INFINITY;
@@ -1216,7 +1450,7 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
     SmpFirst f;
     unsigned long long *part = S.list.part[warp];
     if (nucleus && a.n > kSmpList)
-      f = smp_first<true>(C.span, fast_lo, ref, 1.4426950408889634 / (double)T, part,
+      f = smp_first<true>(C.span, fast_lo, ref, c, part,
                           &S.part_n[warp]);
     else
       f = smp_first<false>(C.span, fast_lo, ref, 1.0, part, &S.part_n[warp]);
@@ -1345,14 +1579,10 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
       if (ok) return;
     }
     // What is tried next: the list of the candidates of a top-k or min-p, a
-    // split of the band with the cut, the list of a band's whole prefix, the
-    // list of a band, the cut key by key; kRow: the cut is known.
-    enum { kList, kSplit, kPrefix, kBand, kKeys, kRow } next;
-    float lo = xb, hi = m;
-    SmpBands bands{xb, m, 0.f, 1.f / kSmpBand0};
-    int level = 0;
-    double target = 0.0, above = 0.0, in_band = 0.0;
-    float band_lo = xb, band_hi = m, band_d0 = 0.f, band_d1 = 0.f;
+    // deep cut, the cut key by key; kRow: the cut is known.
+    enum { kList, kDeep, kKeys, kRow } next;
+    float lo = xb;
+    bad = 1;
     if (!nucleus && (!use_k || k <= kSmpMaxK)) {
       next = kList;
       if (use_k) {
@@ -1381,51 +1611,23 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
         lo = smp_float(max(cut.key, pre - 1u));
       }
     } else {
-      next = use_k ? kKeys : kSplit;
+      next = use_k ? kKeys : kDeep;
     }
 #pragma unroll 1
     while (next != kRow) {
-      if (next == kSplit) {
-        if (level == 4) {
-          next = kKeys;
-          continue;
+      if (next == kDeep) {
+        const SmpWindow win{m, 2.f * (float)c};
+        SmpDeep d = kLost;
+        if (win.scale < 1e30f) {
+          smp_window(C.span, win, xb, m, c, &S.win[0][tid]);
+          smp_window_sums(C, S.x_mass[C.phase & 1]);
+          smp_exchange(C, kSmpWin);
+          d = smp_deep<E>(C, a, w, win, xb, m, m, c, p, r, u, cut);
         }
-        if (level == 0)
-          smp_bands<true>(C.span, w, bands, &S.band.mass[0][tid]);
-        else
-          smp_bands<false>(C.span, w, bands, &S.band.mass[0][tid]);
-        smp_band_sums<true, false>(C);
-        if (level == 0) {
-          for (int i = 0; i < kSmpBands; ++i) target += S.sum_mass[i];
-          target *= (double)p;
-        }
-        // the band of the cut; entries in a band are at least its mass over
-        // its largest mass
-        int j = 0;
-        double entries = 0.0;
-#pragma unroll 1
-        for (; j < kSmpBands; ++j) {
-          band_d0 = j == 0 ? fminf(w.depth(m), bands.from) : bands.begin(j);
-          in_band = S.sum_mass[j] * (double)exp2f(band_d0);
-          entries += in_band;
-          if (above + S.sum_mass[j] >= target || j == kSmpBands - 1) break;
-          above += S.sum_mass[j];
-        }
-        band_d1 = level == 0 && j == kSmpBands - 1 ? 72.f : bands.begin(j + 1);
-        __syncthreads();
-        band_hi = j == 0 ? bands.hi : smp_band_top(w, bands, j);
-        band_lo = j == kSmpBands - 1 ? bands.lo : smp_band_top(w, bands, j + 1);
-        next = level == 0 && entries <= (double)kSmpList ? kPrefix
-               : in_band <= (double)kSmpList             ? kBand
-                                                         : kSplit;
-        lo = band_lo;
-        hi = next == kPrefix ? m : band_hi;
-        if (next == kSplit) {
-          ++level;
-          bands = SmpBands{band_lo, band_hi, band_d0,
-                           (float)kSmpBands / fmaxf(band_d1 - band_d0, 1e-6f)};
-          continue;
-        }
+        if (d == kDrawn) return;
+        if (d == kCut) bad = 0;
+        next = d == kCut ? kRow : kKeys;
+        continue;
       }
       if (next == kKeys) {
         if (use_k) smp_top_k(C, w, cut.key + 1u, key_max, k, cut);
@@ -1435,47 +1637,18 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
         }
         break;
       }
-      const int got = smp_collect(C, lo, hi);
-      const bool fits = got > 0 && got <= kSmpList &&
-                        (next != kList || lo == xb || (long long)got >= k);
-      if (!fits) {
-        if (next == kList) {
-          // min-p alone keeps a long prefix: its threshold is the cut
-          next = use_k ? kKeys : use_p ? kSplit : kRow;
-        } else if (next == kPrefix && in_band <= (double)kSmpList) {
-          next = kBand;
-          hi = band_hi;
-        } else {
-          next = kSplit;
-          ++level;
-          bands = SmpBands{band_lo, band_hi, band_d0,
-                           (float)kSmpBands / fmaxf(band_d1 - band_d0, 1e-6f)};
-        }
-        continue;
-      }
-      if (rank == 0) {
-        const SmpPick pick =
-            smp_pick(S, w, got, cut.key, use_k ? k : 0, use_p ? (double)p : 1.0,
-                     next == kList ? -1.0 : target, next == kBand ? above : 0.0, 0.0, nullptr);
-        if (next != kBand) {
+      const int got = smp_collect(C, lo, m);
+      if (got > 0 && got <= kSmpList && (lo == xb || (long long)got >= k)) {
+        if (rank == 0) {
+          const SmpPick pick = smp_pick(S, w, got, cut.key, use_k ? k : 0,
+                                        use_p ? (double)p : 1.0, -1.0, 0.0, 0.0, nullptr);
           smp_draw_list<E>(S, a, w, r, got, pick, u);
-        } else if (tid == 0) {
-          // the cut lies among these
-          S.cut_key = pick.key;
-          S.cut_ties = pick.ties;
         }
-      }
-      if (next == kBand) {
-        cl.sync();
-        const SmpShared *R = cl.map_shared_rank(&S, 0);
-        cut.key = (uint32_t)R->cut_key;
-        cut.ties = R->cut_ties;
-      } else {
         return;  // drawn; nothing of another CTA is read any more
       }
-      next = kRow;
+      // min-p alone keeps a long prefix: its threshold is the cut
+      next = use_k ? kKeys : use_p ? kDeep : kRow;
     }
-    bad = 1;
     if (cut.ties > 0) tie_w = w(unmono(cut.key));
   }
   if (bad) {  // the segments' masses are not known yet

@@ -297,3 +297,37 @@ def test_repeated_calls_agree():
     first = check(x, u, **s)
     for _ in range(5):
         assert torch.equal(first, sample_logits(x, u, *(s[c] for c in "Tkpm")))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,B", [(4111, 60), (50003, 60), (151936, 6)])
+def test_cuts_at_every_depth(n, B, dtype):
+    """Top-p alone, from the first entry to the last, on rows from flat to sharp."""
+    for s, sigma in enumerate((1e-3, 0.3, 1.0, 3.0)):
+        x = logits(B, n, dtype, 300 + s, sigma, peak=s % 2 == 1)
+        p = torch.linspace(1e-4, 0.99999, B).cuda()
+        check(x, uniforms(B, s), T=0.9, p=p)
+        check(x, uniforms(B, s + 9), T=0.9, p=p, m=1e-7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_heavy_entries_side_by_side(dtype):
+    """The entries above the cut fill one stretch of the row, and few values."""
+    B, n = 12, 60013
+    x = logits(B, n, dtype, 41, 1.0, peak=False)
+    p = torch.tensor([0.3, 0.6, 0.9, 0.99] * 3).cuda()
+    for first, count in ((0, 1500), (30001, 700), (58000, 2013), (100, 5000)):
+        y = x.clone()
+        y[:, first:first + count] += 9.0
+        check(y, uniforms(B, first), p=p)
+        check((y * 4).round() / 4, uniforms(B, first + 1), T=1.3, p=p)
+
+
+@pytest.mark.parametrize("shift", [0.0, 1e4, -1e4, 3e37])
+def test_cuts_far_from_zero(shift):
+    """Logits whose spread is a few steps of their type, and large ones."""
+    B, n = 16, 40000
+    p = torch.linspace(0.05, 0.999, B).cuda()
+    x = logits(B, n, torch.float32, 51, 2.0) + shift
+    check(x, uniforms(B, 3), p=p)
+    check(x, uniforms(B, 4), T=max(1.0, abs(shift) / 1e4), p=p)
