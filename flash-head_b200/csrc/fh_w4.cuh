@@ -207,27 +207,24 @@ __device__ __forceinline__ void w4_load(const W4Args &a, int kb, int r0, int r1,
   }
 }
 
-// acc += the products of a block of TILES 16-row tiles; load(n, j) gives the 16
-// bytes of hidden column 8 n + lane / 4 that belong to word j of the lane's quad.
-template <typename T, int GPK, bool ZP, int NT, int TILES, typename Load>
+// acc += the products of a block of TILES 16-row tiles; load(j) gives the 16
+// bytes of hidden column lane / 4 that belong to word j of the lane's quad.
+template <typename T, int GPK, bool ZP, int TILES, typename Load>
 __device__ __forceinline__ void w4_block(const W4Frag<GPK, ZP> (&f)[TILES], const W4Bits &bits, Load load,
-                                         float (&acc)[TILES][NT][4]) {
+                                         float (&acc)[TILES][4]) {
   constexpr int JG = 4 / GPK;  // words per group
 #pragma unroll
   for (int gi = 0; gi < GPK; ++gi) {
-    float part[TILES][NT][4];
+    float part[TILES][4];
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[t][n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) part[t][i] = 0.f;
 #pragma unroll
     for (int jj = 0; jj < JG; ++jj) {
       const int j = gi * JG + jj;
-      uint4 h[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) h[n] = load(n, j);
+      const uint4 h = load(j);
+      const uint32_t b0[2] = {h.x, h.y}, b1[2] = {h.z, h.w};
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         const uint32_t w0 = j == 0 ? f[t].q[0].x : j == 1 ? f[t].q[0].y : j == 2 ? f[t].q[0].z : f[t].q[0].w;
@@ -239,25 +236,18 @@ __device__ __forceinline__ void w4_block(const W4Frag<GPK, ZP> (&f)[TILES], cons
         w4_unpack<T>(w1, bits, z1, p1);
         const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]};
         const uint32_t a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t b0[2] = {h[n].x, h[n].y}, b1[2] = {h[n].z, h[n].w};
-          mma16816<T>(part[t][n], a0, b0);
-          mma16816<T>(part[t][n], a1, b1);
-        }
+        mma16816<T>(part[t], a0, b0);
+        mma16816<T>(part[t], a1, b1);
       }
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const float s0 = W4Num<T>::scale(w4_scale_bits<GPK>(f[t].s[0], gi));
       const float s1 = W4Num<T>::scale(w4_scale_bits<GPK>(f[t].s[1], gi));
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc[t][n][0] = fmaf(s0, part[t][n][0], acc[t][n][0]);
-        acc[t][n][1] = fmaf(s0, part[t][n][1], acc[t][n][1]);
-        acc[t][n][2] = fmaf(s1, part[t][n][2], acc[t][n][2]);
-        acc[t][n][3] = fmaf(s1, part[t][n][3], acc[t][n][3]);
-      }
+      acc[t][0] = fmaf(s0, part[t][0], acc[t][0]);
+      acc[t][1] = fmaf(s0, part[t][1], acc[t][1]);
+      acc[t][2] = fmaf(s1, part[t][2], acc[t][2]);
+      acc[t][3] = fmaf(s1, part[t][3], acc[t][3]);
     }
   }
 }
@@ -273,16 +263,21 @@ __device__ __forceinline__ uint4 w4_lds(uint32_t at) {
 // Hidden rows in shared memory, 64 bytes of padding per row: the 8 lanes of a
 // 128-byte phase of a 16-byte load (2 rows x 4 quads) then hit all 32 banks.
 __host__ __device__ inline int w4_row_bytes(int nb) { return nb * kW4Block * 2 + 64; }
-__host__ __device__ inline size_t w4_mv_smem_bytes(int nb, int nt) {
+__host__ __device__ inline size_t w4_mv_smem_bytes(int nb) {
   // hidden rows, then the partial sums of the warps that share a unit
-  return (size_t)(8 * nt) * w4_row_bytes(nb) + (size_t)kW4Warps * nt * 32 * 8 * sizeof(float);
+  return (size_t)8 * w4_row_bytes(nb) + (size_t)kW4Warps * 32 * 8 * sizeof(float);
 }
 
-// Dense form for up to 8 * NT hidden rows: one persistent CTA per SM, 16
+// Dense form for up to 8 hidden rows: one persistent CTA per SM, 16
 // warps; a unit is 32 weight rows, taken by ksplit warps (each every
 // ksplit-th block of 128 columns). Units go to CTAs round-robin, so every SM
 // reads the same share of the weight.
-template <typename T, int GPK, bool ZP, int NT>
+// Bound: turning nibbles into operands, about 5 integer instructions a word
+// against 1/2 mma, next to HBM: one row of a 2048 x 128256 head, groups of 128
+// in bf16 and no zero points, 35 us (3.8 TB/s), 8 rows of 4096 x 128256 69 us.
+// mma.sync, not tcgen05: its operand is made in registers, where the words
+// arrive, and a tcgen05 tile of 8 columns would wait for the same words.
+template <typename T, int GPK, bool ZP>
 __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
   extern __shared__ __align__(16) unsigned char w4_sm[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -292,7 +287,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
   {
     const int chunks = a.nb * 16;  // 16-byte chunks of a row
     const int valid = a.D / 8;     // D is a multiple of 32
-    for (int i = tid; i < 8 * NT * chunks; i += 32 * kW4Warps) {
+    for (int i = tid; i < 8 * chunks; i += 32 * kW4Warps) {
       const int r = i / chunks, x = i - r * chunks;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (r < a.rows && x < valid)
@@ -301,7 +296,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
     }
   }
   __syncthreads();
-  float *red = reinterpret_cast<float *>(w4_sm + (size_t)(8 * NT) * rb);
+  float *red = reinterpret_cast<float *>(w4_sm + (size_t)8 * rb);
   const W4Bits bits{a.mask, a.magic};
   const uint32_t hl = smem_u32(w4_sm) + (uint32_t)(g * rb + c * 16);
 
@@ -350,13 +345,11 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
   };
 #pragma unroll
   for (int i = 0; i < kW4Ahead; ++i) fetch(f[i]);
-  float acc[2][NT][4];
+  float acc[2][4];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
 
   const int steps = rounds * my_nb;
   for (int step0 = 0, b = 0, round = 0; step0 < steps; step0 += kW4Ahead) {
@@ -365,8 +358,8 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
     if (step0 + ahead >= steps) break;
     const int kb = kw + b * ks;
     const uint32_t hk = hl + (uint32_t)(kb * (kW4Block * 2));
-    auto load = [&](int n, int j) { return w4_lds(hk + (uint32_t)(8 * n * rb + j * 64)); };
-    w4_block<T, GPK, ZP, NT, 2>(f[ahead], bits, load, acc);
+    auto load = [&](int j) { return w4_lds(hk + (uint32_t)(j * 64)); };
+    w4_block<T, GPK, ZP, 2>(f[ahead], bits, load, acc);
     fetch(f[ahead]);
     if (++b < my_nb) continue;
     b = 0;
@@ -374,29 +367,25 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
     ++round;
     if (ks > 1) {
       // sum the team's partial sums, warp kw = 0 keeps them (fixed order)
-      float *mine = red + (size_t)warp * NT * 32 * 8 + lane * 4;
+      float *mine = red + (size_t)warp * 32 * 8 + lane * 4;
       if (kw > 0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float4 *>(mine + (t * NT + n) * 128) =
-                make_float4(acc[t][n][0], acc[t][n][1], acc[t][n][2], acc[t][n][3]);
+          *reinterpret_cast<float4 *>(mine + t * 128) =
+              make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
       }
       nbar_sync(1 + team, 32 * ks);
       if (kw == 0) {
         for (int o = 1; o < ks; ++o) {
-          const float *other = mine + (size_t)o * NT * 32 * 8;
+          const float *other = mine + (size_t)o * 32 * 8;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float4 v = *reinterpret_cast<const float4 *>(other + (t * NT + n) * 128);
-              acc[t][n][0] += v.x;
-              acc[t][n][1] += v.y;
-              acc[t][n][2] += v.z;
-              acc[t][n][3] += v.w;
-            }
+          for (int t = 0; t < 2; ++t) {
+            const float4 v = *reinterpret_cast<const float4 *>(other + t * 128);
+            acc[t][0] += v.x;
+            acc[t][1] += v.y;
+            acc[t][2] += v.z;
+            acc[t][3] += v.w;
+          }
         }
       }
       nbar_sync(1 + team, 32 * ks);
@@ -406,20 +395,16 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int v = (2 * u + t) * 16 + g + (i >> 1) * 8;
-            const int r = 8 * n + 2 * c + (i & 1);
-            if (v < a.V && r < a.rows) out[(long long)r * a.ldo + v] = from_float<T>(acc[t][n][i]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int v = (2 * u + t) * 16 + g + (i >> 1) * 8;
+          const int r = 2 * c + (i & 1);
+          if (v < a.V && r < a.rows) out[(long long)r * a.ldo + v] = from_float<T>(acc[t][i]);
+        }
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
    }
   }
 }
@@ -427,6 +412,10 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
 // Probed clusters: out[r, i * cap + s] = logit of weight row ci[r, i] * cap + s
 // for hidden row r. A CTA takes 16 candidate slots of one row and its 8 warps
 // share the columns. Cluster ids outside [0, K) give -inf.
+// Bound: latency for one row, then HBM sectors: a cluster of 16 neighbouring
+// rows is 256 bytes in each quad of a block. 256 clusters of 16, 2048 columns,
+// one row 4.7 us; 4096 columns with zero points, 12 rows 40 us (2.7 TB/s of the
+// words, scales and zero points of every row's own clusters).
 constexpr int kW4ProbeWarps = 8;
 
 template <typename T, int GPK, bool ZP>
@@ -451,20 +440,20 @@ __global__ void __launch_bounds__(32 * kW4ProbeWarps) k_w4_probes(W4Args a) {
     }
   }
   const uint4 *h = reinterpret_cast<const uint4 *>(a.hidden) + (size_t)row * (a.D / 8);
-  float acc[1][1][4] = {{{0.f, 0.f, 0.f, 0.f}}};
+  float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
   for (int kb = warp; kb < a.nb; kb += kW4ProbeWarps) {
     W4Frag<GPK, ZP> f[1];
     w4_load<GPK, ZP>(a, kb, wr[0], wr[1], c, f[0]);
     // one hidden row: column n = 0 of B, the other 7 are zero
-    auto load = [&](int, int j) {
+    auto load = [&](int j) {
       const int x = kb * 16 + j * 4 + c;
       return g == 0 && x < a.D / 8 ? ldg_keep(h + x) : make_uint4(0u, 0u, 0u, 0u);
     };
-    w4_block<T, GPK, ZP, 1, 1>(f, W4Bits{a.mask, a.magic}, load, acc);
+    w4_block<T, GPK, ZP, 1>(f, W4Bits{a.mask, a.magic}, load, acc);
   }
   if (c == 0) {
-    red[warp][g] = acc[0][0][0];
-    red[warp][g + 8] = acc[0][0][2];
+    red[warp][g] = acc[0][0];
+    red[warp][g + 8] = acc[0][2];
   }
   __syncthreads();
   if (tid < 16 && s0 + tid < n) {

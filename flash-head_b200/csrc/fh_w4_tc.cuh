@@ -30,8 +30,9 @@
 //               and stores 32 columns' pairs (16 TMEM columns) at a time;
 //   warps 20-23 epilogue: a thread has one weight row and all hidden rows; up to
 //               128 hidden rows the accumulators are double-buffered.
-// Bounds: HBM (the packed weight) up to about 64 rows, the tensor cores and
-// the hidden tiles' way from L2 at 256.
+// Bounds: unpacking next to HBM (the packed weight) up to about 64 rows: 64 rows
+// of a 1536 x 151936 head 43 us (2.8 TB/s); the tensor cores and the hidden
+// tiles' way from L2 at 256: 2048 x 128256 112 us (1.2 PFLOP/s).
 // Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
 // drains its own copies and MMAs (bounded) and frees TMEM before it returns.
 #pragma once

@@ -1781,14 +1781,14 @@ static fh::W4Args w4_args(const fh_w4_desc *d, const void *hidden, int rows, voi
 
 constexpr int kW4SmemMax = 227 * 1024;
 
-template <typename T, int GPK, bool ZP, int NT>
+template <typename T, int GPK, bool ZP>
 static cudaError_t launch_w4_mv_t(const fh::W4Args &a, int grid, cudaStream_t s) {
   static bool done[128];
-  auto kern = fh::k_w4_mv<T, GPK, ZP, NT>;
+  auto kern = fh::k_w4_mv<T, GPK, ZP>;
   const cudaError_t e = raise_smem(kern, kW4SmemMax, done);
   if (e != cudaSuccess) return e;
-  return launch(kern, dim3(grid), dim3(32 * fh::kW4Warps), fh::w4_mv_smem_bytes(a.nb, NT), s,
-                false, a);
+  return launch(kern, dim3(grid), dim3(32 * fh::kW4Warps), fh::w4_mv_smem_bytes(a.nb), s, false,
+                a);
 }
 
 template <typename T, int GPK, bool ZP>
@@ -1828,8 +1828,9 @@ static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
 
 extern "C" {
 
-// Rows of a call that go through k_w4_mv (mma.sync, 8 rows per pass of the
-// weight); more run on the tensor-core kernel.
+// Rows of a call that go through k_w4_mv (8 rows per pass of the weight); more
+// run on the tensor-core kernel. 2048 x 128256: 35 us for up to 8 rows against
+// 45..50 us there; 9..16 rows would be two passes, 70 us.
 constexpr int kW4MvRows = 8;
 
 FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows) {
@@ -1859,7 +1860,7 @@ static int run_w4_mv(const fh_w4_desc *desc, fh::W4Args a, int sms, cudaStream_t
   const int grid = std::min(sms, (units + teams - 1) / teams);
   const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto gpk, auto zp) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_w4_mv_t<T, decltype(gpk)::value, decltype(zp)::value, 1>(a, grid, s);
+    return launch_w4_mv_t<T, decltype(gpk)::value, decltype(zp)::value>(a, grid, s);
   });
   FH_CHECK_LAUNCH(e, "4-bit logits launch");
   return FH_OK;
@@ -1890,7 +1891,7 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
   a.tiles = (desc->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
   a.ldo = out_stride;
   a.err = reinterpret_cast<uint32_t *>(ws);
-  a.polls = 1u << 22;
+  a.polls = 1u << 18;  // a wait is for one block: microseconds
   const void *hop = hidden;
   float *fac = nullptr;
   bool pdl = false;
