@@ -145,7 +145,7 @@ class FlashHead(nn.Module):
         self.register_buffer("special_token_ids_tensor", torch.tensor(st, dtype=torch.int64),
                              persistent=False)
         self._native = None  # (buffer key, NativeHead)
-        self._w4 = None  # (buffer key, W4Weight of w_perm)
+        self._w4 = None  # (_w4_key, W4Weight of w_perm)
 
     # ------------------------------------------------------------------
     # Native head (device buffers + C handle)
@@ -224,17 +224,30 @@ class FlashHead(nn.Module):
         """Quantise ``w_perm`` to 4 bits (``flash_head.w4.W4Weight.from_dense``)
         for ``candidate_logits``, ``head_logits`` and ``get_next_token_filtered``,
         which use it from then on; returns the weight. Greedy and
-        temperature-only steps keep the 16-bit weight. A head moved or cast
-        afterwards has to be quantised again."""
+        temperature-only steps keep the 16-bit weight. A head moved, cast or
+        written to afterwards has to be quantised again: until then the 16-bit
+        weight serves (and ``head_logits`` refuses)."""
         from .w4 import W4Weight
         w = W4Weight.from_dense(self.w_perm.view(-1, self._D), group_size, zeros)
-        self._w4 = ((self.w_perm.data_ptr(), self.w_perm.dtype, self.w_perm.device), w)
+        self._w4 = (self._w4_key(), w)
         return w
+
+    def _w4_key(self):
+        # the tensor itself (held: its address is not reused) and its writes
+        # (not counted for a tensor made in inference mode)
+        t = self.w_perm
+        return t, t.data_ptr(), t.dtype, t.device, 0 if t.is_inference() else t._version
 
     def quantized(self):
         """The 4-bit weight of the current ``w_perm``, or None."""
-        key = (self.w_perm.data_ptr(), self.w_perm.dtype, self.w_perm.device)
-        return self._w4[1] if self._w4 is not None and self._w4[0] == key else None
+        if self._w4 is None:
+            return None
+        (t, *was), w = self._w4
+        now, *is_ = self._w4_key()
+        if t is not now or was != is_:
+            self._w4 = None
+            return None
+        return w
 
     def candidate_logits(self, hidden: torch.Tensor, probes: Optional[torch.Tensor] = None):
         """(logits [N, C], ids [N, C] int32) of a step's candidates: the tokens

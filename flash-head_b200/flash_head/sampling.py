@@ -39,6 +39,11 @@ def _per_row(name: str, v: torch.Tensor, B: int, dtype: torch.dtype, device) -> 
         v = v.reshape(1).expand(B)
     elif v.shape != (B,):
         raise ValueError(f"{name} must be a number or [{B}] values, got {tuple(v.shape)}")
+    if dtype is _I32:
+        if v.is_floating_point() or v.is_complex():
+            raise ValueError(f"{name} must hold integers, got {v.dtype}")
+        if v.dtype is _I64:  # beyond 32 bits: every k from n on is the same
+            v = v.clamp(-1, 2 ** 31 - 1)
     return v.to(dtype).contiguous()
 
 

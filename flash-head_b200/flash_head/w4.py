@@ -92,6 +92,10 @@ class W4Weight:
         d.row_mul = self.row_mul.data_ptr()
         self.desc, self.ref = d, ctypes.byref(d)
 
+    def __reduce__(self):  # copies and pickles hold no addresses
+        return W4Weight, (self.qweight, self.scales, self.zeros, self.vocab, self.hidden,
+                          self.group_size)
+
     # -- making one ----------------------------------------------------------
     @classmethod
     def from_quantized(cls, q: torch.Tensor, scales: torch.Tensor,

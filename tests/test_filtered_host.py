@@ -88,3 +88,40 @@ def test_head_logits_need_a_quantised_head():
     assert fh.quantized() is w and w.shape == (32, 64)
     fh.to(torch.float16)  # another weight
     assert fh.quantized() is None
+
+
+def test_a_4_bit_weight_is_of_the_weight_as_it_is():
+    """Written to, replaced or copied: the old 4-bit weight no longer serves."""
+    import copy
+
+    from torch import nn
+
+    from flash_head.flash_head import FlashHead
+    lm = nn.Linear(64, 32, bias=False).to(torch.bfloat16)
+    fh = FlashHead(lm, torch.randn(64, 4), torch.arange(32).view(4, 8), n_probes=2)
+    w = fh.quantize_head(group_size=32)
+    assert fh.quantized() is w
+    with torch.no_grad():
+        fh.w_perm.mul_(2)
+    assert fh.quantized() is None
+    w = fh.quantize_head(group_size=32)
+    state = {k: v * 3 for k, v in fh.state_dict().items()}
+    if "w_perm" in state:
+        fh.load_state_dict(state)
+        assert fh.quantized() is None
+        w = fh.quantize_head(group_size=32)
+    twin = copy.deepcopy(fh)
+    assert fh.quantized() is w and twin.quantized() is None
+    assert torch.equal(copy.deepcopy(w).dequantize(), w.dequantize())
+    fh.w_perm = fh.w_perm.clone()
+    assert fh.quantized() is None
+
+
+def test_copies_of_vllms_top_k():
+    """int64 values beyond 32 bits keep their meaning; numbers that are none are refused."""
+    from flash_head.sampling import _per_row
+    v = torch.tensor([2 ** 40, -2 ** 40, 7, -1, 2 ** 32 + 1])
+    got = _per_row("top_k", v, 5, torch.int32, v.device)
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, -1, 7, -1, 2 ** 31 - 1]
+    with pytest.raises(ValueError, match="integers"):
+        _per_row("top_k", v.double(), 5, torch.int32, v.device)
