@@ -1126,7 +1126,8 @@ struct SmpWindow {
 // Per-thread masses of a window's bands, of the logits above `base`, in fp32
 // relative to `ref`; returns the thread's largest logit. (Bands of the thread's
 // own: no atomics, a fixed order.) The row's mass is off by kSmpSlack, and 2^-24
-// for every addition: the thread's entries, and 16 more.
+// for every addition: the thread's entries (at most 16 more than an equal
+// share of the row), and 13 that join the threads' bands.
 template <typename Span>
 __device__ __noinline__ float smp_window(Span span, SmpWindow win, float base, float ref, double c,
                                          float *mine) {
@@ -1294,7 +1295,7 @@ __device__ __forceinline__ SmpDeep smp_deep(Ctx &C, const SampleArgs &a, const S
     if (got > 0 && got <= kSmpList) {
       hi = m;
       if (C.rank == 0) {
-        const double slack = kSmpSlack + 0x1p-24 * (16.0 + (double)C.span.row.n /
+        const double slack = kSmpSlack + 0x1p-24 * (32.0 + (double)C.span.row.n /
                                                                (double)(kSmpThreads * C.size));
         const double target = (double)p * z * exp2((double)ref * w.c - w.k0);
         bool sure = false;

@@ -367,9 +367,10 @@ FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
 /*
  * Products with a head weight held in 4 bits (no counterpart in the
  * reference): w[v, k] = (q[v, k] - z[v, g]) * s[v, g] with q in 0..15 and one
- * scale s (and zero point z) per group g = k / group_size of a row. The group
- * sums are exact products summed in fp32 and scaled in fp32; results are
- * rounded once, to the hidden states' type.
+ * scale s (and zero point z) per group g = k / group_size of a row. Up to 8
+ * rows, and for probed clusters, the products (q - z) * h are exact, summed in
+ * fp32 and scaled in fp32 by group; beyond, (q - z) * s is rounded to 11 bits
+ * once. Results are rounded once, to the hidden states' type.
  *
  *   vocab      V, weight rows
  *   hidden     D, columns: a multiple of group_size, at most FH_W4_MAX_HIDDEN
