@@ -1713,13 +1713,17 @@ extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, 
   a.out = out_ids;
   a.prob = out_prob;
   // Several CTAs per row while the grid stays within a number of CTAs per SM
-  // and each keeps 4096 entries: 8, which evens out rows that need more passes
-  // than others (256 rows of 151936 with top-p: 247 us, with at most 2 per SM
-  // 455); 2 where no row has a filter and all are alike (256 rows of 128256: 60
-  // us, with 8 per SM 71).
-  const bool plain = !params->top_k && !params->top_p && !params->min_p && params->top_k_all <= 0 &&
-                     !(params->top_p_all < 1.f) && !(params->min_p_all > 0.f);
-  const long long per_sm = plain ? 2 : 8;
+  // and each keeps 4096 entries. A top-p may need more passes for some rows than
+  // for others, which shorter CTAs in two waves even out: 8 (256 fp32 rows of
+  // 151936, top-p 0.9 at temperature 0.8: 207 us, with 4 per SM 223, with 16
+  // 257). Rows that the first candidates settle run in one wave: 4 (256 bf16 rows
+  // of 128256, top-k 50: 52 us, with 8 per SM 68). 2 where no row has a filter
+  // and all are alike (the same rows: 60 us, with 8 per SM 71).
+  const bool some_p = params->top_p || params->top_p_all < 1.f;
+  const bool plain = !params->top_k && !some_p && !params->min_p && params->top_k_all <= 0 &&
+                     !(params->min_p_all > 0.f);
+  const bool listed = !params->top_k && params->top_k_all > 0 && params->top_k_all <= fh::kSmpMaxK;
+  const long long per_sm = plain ? 2 : some_p && !listed ? 8 : 4;
   const int sms = sm_count() > 0 ? sm_count() : 148;
   int cluster = 1;
   while (cluster < fh::kSmpMaxCluster && (long long)rows * cluster * 2 <= per_sm * sms &&
