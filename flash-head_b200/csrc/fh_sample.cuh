@@ -32,12 +32,15 @@
 // Rows that resist (thousands of equal logits at a cut, top-k beyond 1024)
 // descend through 16 bands of keys per pass, exact for every input.
 //
-// Bound: a pass in fp64 is the cost, not the bytes: an exponential is 14 fp64
-// instructions, about 9 clocks of an SM per 32 entries, 33 us for 256 rows of
-// 128256 entries against 10 us of reading. Measured, bf16 rows of 128256 unless
-// said otherwise: one row with top-k and top-p 17.4 us; 64 rows of mixed filters
-// 54 us; 256 rows without a filter 66 us (1.0 TB/s); 256 fp32 rows of 151936
-// with top-p 208 us, 114 us where the cut lies among the first candidates.
+// Bound: an unfiltered row costs a pass in fp64, not its bytes: an exponential
+// is 14 fp64 instructions, about 9 clocks of an SM per 32 entries, 33 us for 256
+// rows of 128256 entries against 10 us of reading. Filtered rows are bound by
+// latency: a chain of passes, exchanges, a sort and scans, which the rows of
+// other clusters cover in part. Measured, bf16 rows of 128256 unless said
+// otherwise: one row with top-k and top-p 17.4 us; 64 rows of mixed filters 54
+// us; 256 rows without a filter 66 us (1.0 TB/s), with top-k 50 52 us (1.3
+// TB/s); 256 fp32 rows of 151936 with top-p 208 us, 114 us where the cut lies
+// among the first candidates.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -1718,7 +1718,7 @@ extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, 
   // 151936, top-p 0.9 at temperature 0.8: 207 us, with 4 per SM 223, with 16
   // 257). Rows that the first candidates settle run in one wave: 4 (256 bf16 rows
   // of 128256, top-k 50: 52 us, with 8 per SM 68). 2 where no row has a filter
-  // and all are alike (the same rows: 60 us, with 8 per SM 71).
+  // and all are alike (the same rows: 66 us, with 8 per SM 72).
   const bool some_p = params->top_p || params->top_p_all < 1.f;
   const bool plain = !params->top_k && !some_p && !params->min_p && params->top_k_all <= 0 &&
                      !(params->min_p_all > 0.f);
