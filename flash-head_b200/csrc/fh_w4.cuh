@@ -4,7 +4,7 @@
 // are formed group by group: q - z is a small integer, exact in the 16-bit
 // type of the hidden states, so the tensor cores sum exact products in fp32,
 // and the scale multiplies the group's fp32 sum. No weight is ever rounded to
-// 16 bits.
+// 16 bits. (More than 8 rows: fh_w4_tc.cuh, fh_w4_split.cuh.)
 //
 // Layout (made once by the loader, flash_head/w4.py). Rows come in tiles of
 // 128, columns in blocks of 128 (both padded; padding has scale 0):

@@ -1,38 +1,48 @@
-// Logits of a 4-bit head for many rows on the 5th-generation tensor cores:
-// out[b, v] = sum_k w[v, k] h[b, k], M = 128 weight rows, N = up to 256 hidden
-// rows per launch.
+// Logits of a 4-bit head with scale groups of 128 columns for many rows, on the
+// 5th-generation tensor cores:
+// out[b, v] = sum_g s[v, g] sum_{k in g} (q[v, k] - z[v, g]) h[b, k], M = 128
+// weight rows, N = up to 128 hidden rows per launch. (Smaller groups:
+// fh_w4_split.cuh.)
 //
-// The weight's integers become f16 operands: q - z is exact,
-// and its product with the group's scale is rounded to f16 once, 2^-11 relative
-// (a bf16 scale times a 4-bit integer has at most one bit more than f16 holds).
-// That is an eighth of a bf16 output's own rounding; applying the scales to
-// fp32 sums instead, as k_w4_mv does, would read every accumulator back once
-// per group. Rows of scales are brought to [1, 2) by an exact power of two
-// (row_mul), undone in the epilogue, so that no weight leaves f16's range. bf16
-// hidden rows are copied to f16 first, each scaled by a power of two likewise
-// (k_w4_hidden); f16 ones are read as they are.
+// The products are k_w4_mv's: the operands are the integers q - z, exact in
+// the hidden states' own 16-bit type, and those hidden states as they are; a
+// group's products are summed in fp32 in an accumulator of their own, and the
+// group's scale multiplies that sum in fp32. No weight and no hidden state is
+// rounded, however far apart scales or hidden states lie. (Scales multiplied
+// into one f16 operand need no accumulator per group and take 45 us where this
+// takes 54, but round weights to 11 bits and lose scales 2^-14 below their row's
+// largest.)
 //
 // The unpacked operand goes to tensor memory, not to shared memory: 16 KB
 // written and 16 KB read per 128 x 64 tile were most of the shared-memory
-// traffic that bound a first version (64 rows of a 1536 x 151936 head: 92 us).
+// traffic that bound a first version.
 //
-// One persistent CTA per SM, 24 warps:
-//   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and
-//               zero points of 128 rows x 128 columns: two or three bulk copies)
-//               into a ring of their own, deep enough to keep HBM busy;
-//   warp 2      lane 0 brings the hidden tiles of every 128 columns (TMA, two of 64
+// One persistent CTA per SM, 28 warps; its blocks (128 columns, one scale group, of
+// a tile of 128 weight rows) are numbered in the order of the work:
+//   warp 0      lane 0 brings the packed blocks (8 KB of words, the scales and zero
+//               points: two or three bulk copies) into a ring of their own, deep
+//               enough to keep HBM busy;
+//   warp 2      lane 0 brings the hidden tiles of every block (TMA, two of 64 columns
 //               with the 128-byte swizzle) into the stages (a thread of its own: a wait that
 //               suspends the one for packed slots must not hold up these);
-//   warp 1      allocates TMEM; one lane issues tcgen05.mma (K = 16), 8 per
-//               stage, A from tensor memory, B from shared memory;
-//   warps 4-19  unpack, in four groups of 4 on successive blocks: a thread has one
-//               weight row, i.e. one TMEM lane, reads its 64 bytes of the block
-//               and stores 32 columns' pairs (16 TMEM columns) at a time;
-//   warps 20-23 epilogue: a thread has one weight row and all hidden rows; up to
-//               128 hidden rows the accumulators are double-buffered.
-// Bounds: unpacking next to HBM (the packed weight) up to about 64 rows: 64 rows
-// of a 1536 x 151936 head 43 us (2.8 TB/s); the tensor cores and the hidden
-// tiles' way from L2 at 256: 2048 x 128256 112 us (1.2 PFLOP/s).
+//   warps 1, 3  issue tcgen05.mma (K = 16), 8 a block, A from tensor memory, B
+//               from shared memory: warp 1 the even blocks, warp 3 the odd ones, each
+//               into accumulators of its own. Warp 1 also allocates TMEM;
+//   warps 4-27  six groups of 4 (a TMEM quadrant each). The last one to four, one
+//               for every 32 hidden rows, sum and store: a thread has one weight
+//               row and 32 hidden rows, whose logits it keeps in registers. The
+//               first ones (4 or 2) unpack, on successive blocks: a thread has one
+//               weight row, reads its 64 bytes of the block and stores 32
+//               columns' pairs (16 TMEM columns) at a time; it also hands the
+//               scale on, in shared memory.
+// More than 128 rows take several launches: two more sets of accumulators would
+// not fit beside the operand, nor their sums in the registers.
+// Bound: the chain of barriers that every block passes (a wait costs some 130
+// clocks, met or not) and the issue slots (72 %): 9 rows of a 2048 x 128256 head
+// 49 us, 64 of a 1536 x 151936 one 54 us (2.2 TB/s), 128 and 256 of 2048 x 128256
+// 75 and 148 us (0.9 PFLOP/s). Tried and slower: polls with a time hint, fp32x2
+// multiply-adds, half as many warps that sum 64 rows each, and twice as many that
+// take every other block.
 // Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
 // drains its own copies and MMAs (bounded) and frees TMEM before it returns.
 #pragma once
@@ -44,30 +54,39 @@ namespace fh {
 
 constexpr int kW4tConvWarps = 4;  // unpack one block together, a TMEM quadrant each
 constexpr int kW4tGroups = 4;     // of such warps, on successive blocks (a launch may use fewer)
-constexpr int kW4tEpiWarps = 4;
-constexpr int kW4tFirstConv = 4;  // warp
-constexpr int kW4tEpi = kW4tFirstConv + kW4tGroups * kW4tConvWarps;
-constexpr int kW4tThreads = 32 * (kW4tFirstConv + kW4tGroups * kW4tConvWarps + kW4tEpiWarps);
-constexpr int kW4tMaxN = 256;
-constexpr int kW4tMaxStages = 4;
-constexpr int kW4tACols = 64;  // TMEM columns of a stage's A tile: 128 f16 per row
+constexpr int kW4tTeams = 6;      // groups of 4 warps that unpack, or sum and store
+constexpr int kW4tFirst = 4;      // their first warp
+constexpr int kW4tThreads = 32 * (kW4tFirst + 4 * kW4tTeams);
+constexpr int kW4tCols = 32;      // hidden rows of a group that sums
+constexpr int kW4tMaxN = 128;
+constexpr int kW4tStages = 4;     // blocks of hidden columns and unpacked weights
+constexpr int kW4tMaxAcc = 2;     // accumulators of an issuing warp
+constexpr int kW4tACols = 64;  // TMEM columns of a stage's A tile: 128 16-bit numbers per row
 constexpr int kW4tMaxPacked = 12;
-constexpr int kW4tSmemMax = 227 * 1024;
+// Blocks of scales handed on. Block n's are written when the MMAs of block
+// n - stages are done, which were issued when the block 2 * n_acc before had been
+// summed (n_acc accumulators in each of two warps): the slot's last use, 8 blocks
+// before, is over.
+constexpr int kW4tScaleSlots = 8;
+static_assert(kW4tScaleSlots >= kW4tStages + 2 * kW4tMaxAcc, "a slot may still be read");
+constexpr int kW4tOutBytes = 32 * 16 * 2;  // a warp's outputs, 16 hidden rows at a time
+constexpr int kW4SmemMax = 227 * 1024;
 
 struct W4TcArgs {
   const uint32_t *qw;
   const void *scales;
   const uint8_t *zeros;
-  const float *row_mul;   // [128 * tiles] powers of two
-  const float *row_fac;   // [rows] factors of the hidden rows, or null
   int V, D, nb;
   int tiles;
   int rows, n_pad;
-  int stages, packed, n_acc, groups;
+  int packed;  // slots of packed blocks
+  int n_acc;   // accumulators of an issuing warp (1 or 2)
+  int groups;  // groups that unpack
+  int sums;    // groups that sum and store
   int tmem_cols;
   int vec;                // outputs take 16-byte stores (V, ldo and out allow them)
   uint32_t idesc;
-  uint32_t mask, magic;   // kW4Mask, W4Num<__half>::kMagic
+  uint32_t mask, magic;   // kW4Mask, W4Num<T>::kMagic
   void *out;
   long long ldo;
   uint32_t *err;
@@ -75,44 +94,41 @@ struct W4TcArgs {
 };
 
 struct W4TcCtrl {
-  uint64_t full[kW4tMaxStages];    // hidden tile landed and A tile written
-  uint64_t empty[kW4tMaxStages];   // MMAs done
+  uint64_t hfull[kW4tStages];   // hidden tile landed
+  uint64_t full[kW4tStages];    // A tile written
+  uint64_t empty[kW4tStages];   // MMAs done
   uint64_t pfull[kW4tMaxPacked];   // packed block landed
   uint64_t pempty[kW4tMaxPacked];  // packed block unpacked
-  uint64_t acc_full[2];
-  uint64_t acc_empty[2];
+  uint64_t acc_full[2][kW4tMaxAcc];
+  uint64_t acc_empty[2][kW4tMaxAcc];
   uint64_t drain;
   uint32_t tmem_base;
   uint32_t s_err;
-  alignas(16) float fac[kW4tMaxN];
-  uint4 out[kW4tEpiWarps][128];  // 32 hidden rows x 32 weight rows, 16-bit
 };
 
-// Groups that may run. A group steps over the others' blocks, so that it knows of
-// a barrier's progress only what the order of the work implies; a parity wait
-// is unambiguous while the phase before the awaited one is known to be
-// complete. Having written block n, a group knows the MMAs up to block
-// n - stages, and with them the packed blocks up to there, to be done. Its next
-// block n + groups needs the stage's use two rounds back, n + groups - 2 stages,
-// and the packed slot's fill one round back, n + groups - packed, among them.
+// Groups that may unpack: as many as divide the stages and the packed slots, so
+// that a stage and a slot are always the same group's. A parity wait cannot tell
+// a phase from the one two before it: a group that did not see every phase of
+// a barrier might pass one early.
 __host__ __device__ inline int w4t_groups(int stages, int packed) {
   int g = kW4tGroups;
-  while (g > 0 && (g > stages || packed < g + stages)) --g;
+  while (g > 0 && (g > stages || packed < g + stages || stages % g || packed % g)) --g;
   return g;
 }
 
-__host__ __device__ inline int w4t_packed_bytes(int gpk, bool zp) {
+__host__ __device__ inline int w4_packed_bytes(int gpk, bool zp) {
   return kW4Tile * kW4RowWords * 4 + kW4Tile * gpk * (zp ? 3 : 2);
 }
-__host__ __device__ inline size_t w4t_stage_bytes(int n_pad) {
+__host__ __device__ inline size_t w4_stage_bytes(int n_pad) {
   return (size_t)n_pad * 256;  // two tiles of 64 hidden columns
 }
-__host__ __device__ inline size_t w4t_smem_bytes(int n_pad, int stages, int packed, int gpk, bool zp) {
-  return 1024 + stages * w4t_stage_bytes(n_pad) + (size_t)packed * w4t_packed_bytes(gpk, zp) +
-         sizeof(W4TcCtrl);
+// Everything but the packed ring.
+__host__ __device__ inline size_t w4t_other_bytes(int n_pad, int sums) {
+  return 1024 + kW4tStages * w4_stage_bytes(n_pad) + (size_t)kW4tScaleSlots * kW4Tile * 2 +
+         (size_t)sums * 4 * kW4tOutBytes + sizeof(W4TcCtrl);
 }
 
-// mbar_wait and tc_commit by shared-memory address.
+// mbar_wait by shared-memory address.
 __device__ __forceinline__ bool w4t_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
   for (uint32_t i = 0; i < polls; ++i) {
     uint32_t ok;
@@ -126,10 +142,32 @@ __device__ __forceinline__ bool w4t_wait(uint32_t bar, uint32_t parity, uint32_t
   }
   return false;
 }
+// The same by a whole warp, with one outcome for all its lanes.
+__device__ __forceinline__ bool w4t_wait_all(uint32_t bar, uint32_t parity, uint32_t polls) {
+  return __all_sync(0xFFFFFFFFu, w4t_wait(bar, parity, polls));
+}
+// The same by a group of 4 warps (named barrier `id`): its first warp polls, the
+// others are held by the barrier, which brings them the outcome. (28 warps that
+// poll took a third of the issue slots.)
+__device__ __forceinline__ bool w4t_wait_group(uint32_t bar, uint32_t parity, uint32_t polls,
+                                               int id, bool first) {
+  const uint32_t failed = first && !w4t_wait(bar, parity, polls);
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
+      " barrier.cta.red.or.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(any)
+      : "r"(failed), "r"(id)
+      : "memory");
+  return any == 0u;
+}
 __device__ __forceinline__ void w4t_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    bar)
                : "memory");
+}
+__device__ __forceinline__ void w4t_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ bool w4t_elect() {
@@ -138,7 +176,7 @@ __device__ __forceinline__ bool w4t_elect() {
                : "=r"(p));
   return p != 0;
 }
-// D += A . B with A in tensor memory: row m in lane m, two f16 per column.
+// D += A . B with A in tensor memory: row m in lane m, two 16-bit numbers per column.
 __device__ __forceinline__ void w4t_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
@@ -157,88 +195,64 @@ __device__ __forceinline__ void w4t_st16(uint32_t addr, const uint32_t (&x)[16])
       : "memory");
 }
 
-// f16 copy of bf16 hidden rows, one CTA per row: the row's largest finite
-// magnitude is brought to [2^14, 2^15) by a power of two whose inverse goes to
-// fac. Infinities and NaN stay. Also clears the error word.
-__global__ void __launch_bounds__(256)
-    k_w4_hidden(const uint4 *h, uint4 *out, float *fac, int chunks, uint32_t *err) {
-  __shared__ uint32_t top[8];
-  grid_dep_launch();
-  const uint4 *src = h + (size_t)blockIdx.x * chunks;
-  uint32_t m = 0u;  // largest finite magnitude, bf16 bits
-  for (int i = threadIdx.x; i < chunks; i += 256) {
-    const uint4 v = src[i];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = w[j] & 0x7FFFu, hi = (w[j] >> 16) & 0x7FFFu;
-      if (lo < 0x7F80u) m = max(m, lo);
-      if (hi < 0x7F80u) m = max(m, hi);
+// A position in a ring of n barriers and the parity of its current round.
+struct W4tRing {
+  int at = 0;
+  uint32_t phase = 0u;
+  __device__ __forceinline__ void next(int n) {
+    if (++at == n) {
+      at = 0;
+      phase ^= 1u;
     }
   }
-  m = __reduce_max_sync(0xFFFFFFFFu, m);
-  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, top[i]);
-  // exponent of the largest value (a zero or subnormal row counts as 2^-126)
-  const int e = max((int)(m >> 7), 1) - 127;
-  // 2^(14 - e) in two factors: it may pass the largest fp32
-  const int s0 = (14 - e) / 2, s1 = 14 - e - s0;
-  const float f0 = __uint_as_float((uint32_t)(127 + s0) << 23);
-  const float f1 = __uint_as_float((uint32_t)(127 + s1) << 23);
-  uint4 *dst = out + (size_t)blockIdx.x * chunks;
-  for (int i = threadIdx.x; i < chunks; i += 256) {
-    const uint4 v = src[i];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float lo = __uint_as_float(w[j] << 16) * f0 * f1;
-      const float hi = __uint_as_float(w[j] & 0xFFFF0000u) * f0 * f1;
-      const __half2 x = __floats2half2_rn(lo, hi);
-      o[j] = *reinterpret_cast<const uint32_t *>(&x);
-    }
-    dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-  if (threadIdx.x == 0) {
-    // the inverse, 2^(e - 14): may be subnormal as one factor, never zero
-    fac[blockIdx.x] = ldexpf(1.f, e - 14);
-    if (blockIdx.x == 0) *err = 0u;
-  }
-}
+};
 
-// T: type of the scales and outputs. GPK, ZP as in k_w4_mv.
-template <typename T, int GPK, bool ZP>
+// A block's accumulator among the n_acc (1 or 2) of the warp that issues its MMAs.
+struct W4tUse {
+  uint32_t at, phase;
+  __device__ __forceinline__ W4tUse(uint32_t block, uint32_t n_acc) {
+    const uint32_t use = block >> 1;
+    at = use & (n_acc - 1u);
+    phase = (n_acc == 2u ? use >> 1 : use) & 1u;
+  }
+};
+
+// T: type of the hidden states, scales and outputs. ZP: with zero points.
+template <typename T, bool ZP>
 __global__ void __launch_bounds__(kW4tThreads, 1)
     k_w4_tc(const __grid_constant__ CUtensorMap tm_h, W4TcArgs a) {
   extern __shared__ __align__(1024) unsigned char w4t_sm[];
   const uint32_t raw = smem_u32(w4t_sm);
   unsigned char *ring = w4t_sm + (((raw + 1023u) & ~1023u) - raw);
-  const size_t sb = w4t_stage_bytes(a.n_pad);
-  unsigned char *pring = ring + (size_t)a.stages * sb;
+  const size_t sb = w4_stage_bytes(a.n_pad);
   constexpr int kWords = kW4Tile * kW4RowWords * 4;  // bytes of packed words
-  constexpr int kScales = kW4Tile * GPK * 2, kZeros = ZP ? kW4Tile * GPK : 0;
+  constexpr int kScales = kW4Tile * 2, kZeros = ZP ? kW4Tile : 0;
   constexpr int pb = kWords + kScales + kZeros;
-  W4TcCtrl &S = *reinterpret_cast<W4TcCtrl *>(pring + (size_t)a.packed * pb);
+  unsigned char *pring = ring + (size_t)kW4tStages * sb;
+  unsigned char *sring = pring + (size_t)a.packed * pb;
+  unsigned char *oring = sring + kW4tScaleSlots * kScales;
+  W4TcCtrl &S = *reinterpret_cast<W4TcCtrl *>(oring + (size_t)a.sums * 4 * kW4tOutBytes);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);  // uniform
   const int G = gridDim.x, t0 = blockIdx.x;
+  const int team = (warp - kW4tFirst) >> 2;
 
   if (tid == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&S.full[s], 1 + kW4tConvWarps);
+    for (int s = 0; s < kW4tStages; ++s) {
+      mbar_init(&S.hfull[s], 1);
+      mbar_init(&S.full[s], kW4tConvWarps);
       mbar_init(&S.empty[s], 1);
     }
     for (int s = 0; s < a.packed; ++s) {
       mbar_init(&S.pfull[s], 1);
       mbar_init(&S.pempty[s], kW4tConvWarps);
     }
-    for (int j = 0; j < 2; ++j) {
-      mbar_init(&S.acc_full[j], 1);
-      mbar_init(&S.acc_empty[j], kW4tEpiWarps);
-    }
-    mbar_init(&S.drain, 1);
+    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < a.n_acc; ++j) {
+        mbar_init(&S.acc_full[i][j], 1);
+        mbar_init(&S.acc_empty[i][j], 4 * a.sums);
+      }
+    mbar_init(&S.drain, 2);
     S.s_err = 0u;
     fence_mbar_init();
   }
@@ -253,262 +267,234 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, S.tmem_base, 0);
-  const uint32_t a_col = (uint32_t)(a.n_acc * a.n_pad);  // first column of the A tiles
+  const uint32_t a_col = (uint32_t)(2 * a.n_acc * a.n_pad);  // first column of the A tiles
 
   if (warp == 0) {
     if (lane == 0) {
-      int issued[kW4tMaxPacked];  // parity of the last fill of each slot, -1: none
-      for (int j = 0; j < kW4tMaxPacked; ++j) issued[j] = -1;
-      int ps = 0;
-      uint32_t ph = 0u;
+      uint32_t sent = 0u;  // slots filled, and the parity of their last fill
+      uint32_t parity = 0u;
+      W4tRing p;
       bool ok = true;
       for (int t = t0; t < a.tiles && ok; t += G) {
         for (int kb = 0; kb < a.nb; ++kb) {
-          if (!mbar_wait(&S.pempty[ps], ph ^ 1u, a.polls)) {
+          if (!mbar_wait(&S.pempty[p.at], p.phase ^ 1u, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
             break;
           }
-          unsigned char *p = pring + (size_t)ps * pb;
+          unsigned char *to = pring + (size_t)p.at * pb;
           const size_t blk = (size_t)t * a.nb + kb;
-          mbar_expect_tx(&S.pfull[ps], (uint32_t)pb);
-          bulk_g2s(p, reinterpret_cast<const unsigned char *>(a.qw) + blk * kWords, kWords,
-                   &S.pfull[ps]);
-          bulk_g2s(p + kWords, reinterpret_cast<const unsigned char *>(a.scales) + blk * kScales,
-                   kScales, &S.pfull[ps]);
-          if (ZP) bulk_g2s(p + kWords + kScales, a.zeros + blk * kZeros, kZeros, &S.pfull[ps]);
-          issued[ps] = (int)ph;
-          if (++ps == a.packed) {
-            ps = 0;
-            ph ^= 1u;
-          }
+          mbar_expect_tx(&S.pfull[p.at], (uint32_t)pb);
+          bulk_g2s(to, reinterpret_cast<const unsigned char *>(a.qw) + blk * kWords, kWords,
+                   &S.pfull[p.at]);
+          bulk_g2s(to + kWords, reinterpret_cast<const unsigned char *>(a.scales) + blk * kScales,
+                   kScales, &S.pfull[p.at]);
+          if (ZP)
+            bulk_g2s(to + kWords + kScales, a.zeros + blk * kZeros, kZeros, &S.pfull[p.at]);
+          sent |= 1u << p.at;
+          parity = (parity & ~(1u << p.at)) | (p.phase << p.at);
+          p.next(a.packed);
         }
       }
       // every copy this thread issued has landed before the CTA may leave
       for (int j = 0; j < a.packed; ++j)
-        if (issued[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued[j], a.polls))
+        if ((sent >> j) & 1u && !mbar_wait(&S.pfull[j], (parity >> j) & 1u, a.polls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 2) {
     if (lane == 0) {
-      int issued[kW4tMaxStages];
-      for (int j = 0; j < kW4tMaxStages; ++j) issued[j] = -1;
-      int s = 0;
-      uint32_t ph = 0u;
+      uint32_t sent = 0u, parity = 0u;
+      W4tRing p;
       bool ok = true;
-      grid_dep_wait();  // the f16 copy of the hidden rows
       for (int t = t0; t < a.tiles && ok; t += G) {
         for (int kb = 0; kb < a.nb; ++kb) {
-          if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
+          if (!mbar_wait(&S.empty[p.at], p.phase ^ 1u, a.polls)) {
             atomicOr(&S.s_err, kErrCopyTimeout);
             ok = false;
             break;
           }
-          const bool two = 128 * kb + 64 < a.D;
-          unsigned char *at = ring + (size_t)s * sb;
-          mbar_expect_tx(&S.full[s], (uint32_t)(a.n_pad * (two ? 256 : 128)));
-          tma_load_2d(at, &tm_h, 128 * kb, 0, &S.full[s]);
-          if (two) tma_load_2d(at + a.n_pad * 128, &tm_h, 128 * kb + 64, 0, &S.full[s]);
-          issued[s] = (int)ph;
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1u;
-          }
+          unsigned char *at = ring + (size_t)p.at * sb;
+          mbar_expect_tx(&S.hfull[p.at], (uint32_t)(a.n_pad * 256));
+          tma_load_2d(at, &tm_h, 128 * kb, 0, &S.hfull[p.at]);
+          tma_load_2d(at + a.n_pad * 128, &tm_h, 128 * kb + 64, 0, &S.hfull[p.at]);
+          sent |= 1u << p.at;
+          parity = (parity & ~(1u << p.at)) | (p.phase << p.at);
+          p.next(kW4tStages);
         }
       }
-      for (int j = 0; j < a.stages; ++j)
-        if (issued[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued[j], a.polls))
+      for (int j = 0; j < kW4tStages; ++j)
+        if ((sent >> j) & 1u && !mbar_wait(&S.hfull[j], (parity >> j) & 1u, a.polls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 3) {
     // the whole warp walks the loop, so that descriptors and addresses are
     // uniform; one lane issues (by a single lane inside a branch, an MMA took
     // 50 clocks to issue)
     const bool leader = w4t_elect();
-    const uint32_t full0 = smem_u32(&S.full[0]), empty0 = smem_u32(&S.empty[0]);
+    const int mine = warp >> 1;
+    const uint32_t hfull0 = smem_u32(&S.hfull[0]), full0 = smem_u32(&S.full[0]);
+    const uint32_t empty0 = smem_u32(&S.empty[0]);
+    const uint32_t afull0 = smem_u32(&S.acc_full[mine][0]);
+    const uint32_t aempty0 = smem_u32(&S.acc_empty[mine][0]);
+    const uint32_t acc0 = tmem + (uint32_t)(mine * a.n_acc * a.n_pad);
     const uint64_t bd0 = umma_desc_k(smem_u32(ring)), step = sb >> 4;
     const uint64_t half = (uint64_t)(a.n_pad * 128) >> 4;
     const uint32_t idesc = a.idesc;
-    int s = 0;
-    uint32_t ph = 0u;
+    const uint32_t n_acc = (uint32_t)a.n_acc;
+    uint32_t block = 0u;
     bool ok = true;
-    for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
-      const int buf = i % a.n_acc, use = i / a.n_acc;
-      if (use > 0 && !mbar_wait(&S.acc_empty[buf], (uint32_t)((use - 1) & 1), a.polls)) ok = false;
-      const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
-      for (int kb = 0; kb < a.nb && ok; ++kb) {
-        if (!w4t_wait(full0 + 8u * s, ph, a.polls)) {
-          ok = false;
-          break;
-        }
+    for (int t = t0; t < a.tiles && ok; t += G) {
+      for (int kb = 0; kb < a.nb; ++kb, ++block) {
+        if ((block & 1u) != (uint32_t)mine) continue;
+        const uint32_t st = block % kW4tStages, phase = (block / kW4tStages) & 1u;
+        ok = w4t_wait_all(hfull0 + 8u * st, phase, a.polls) &&
+             w4t_wait_all(full0 + 8u * st, phase, a.polls);
+        if (!ok) break;
+        const W4tUse ac(block, n_acc);
+        ok = w4t_wait_all(aempty0 + 8u * ac.at, ac.phase ^ 1u, a.polls);
+        if (!ok) break;
         tc_fence_after();
-        const uint64_t bd = bd0 + step * s;
-        const uint32_t at = tmem + a_col + (uint32_t)(s * kW4tACols);
+        const uint64_t bd = bd0 + step * st;
+        const uint32_t at = tmem + a_col + st * kW4tACols;
+        const uint32_t acc = acc0 + ac.at * (uint32_t)a.n_pad;
         if (leader) {
-          if (128 * kb + 128 <= a.D) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
-                      q > 0 ? 1u : (uint32_t)kb);
-          } else {
-            for (int q = 0; 128 * kb + 16 * q < a.D; ++q)
-              w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc,
-                      (uint32_t)(kb | q));
-          }
-          w4t_commit(empty0 + 8u * s);
+          for (int q = 0; q < 8; ++q)
+            w4t_mma(acc, at + 8u * q, bd + (q >> 2) * half + 2u * (q & 3), idesc, q > 0);
+          w4t_commit(afull0 + 8u * ac.at);
+          w4t_commit(empty0 + 8u * st);
         }
         __syncwarp();
-        if (++s == a.stages) {
-          s = 0;
-          ph ^= 1u;
-        }
       }
-      if (ok && leader) tc_commit(&S.acc_full[buf]);
     }
     if (leader) {
       if (!ok) atomicOr(&S.s_err, kErrCopyTimeout);
       tc_commit(&S.drain);
       if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
     }
-  } else if (warp >= kW4tFirstConv && warp < kW4tFirstConv + kW4tGroups * kW4tConvWarps) {
-    const int group = (warp - kW4tFirstConv) / kW4tConvWarps;
+  } else if (team < a.groups) {
     const int q4 = warp & 3, m = 32 * q4 + lane;  // this thread's row of the tile
     const W4Bits bits{a.mask, a.magic};
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16) + a_col;
-    int s = 0, ps = 0, turn = 0;
-    uint32_t ph = 0u, pph = 0u;
-    bool ok = group < a.groups;
+    W4tRing st, pk;
+    int turn = 0;
+    uint32_t block = 0u;
+    bool ok = true;
     for (int t = t0; t < a.tiles && ok; t += G) {
-      const float mul = __ldg(a.row_mul + t * kW4Tile + m);
-      for (int kb = 0; kb < a.nb && ok; ++kb) {
-        const bool mine = turn == group;
+      for (int kb = 0; kb < a.nb; ++kb, ++block) {
+        const bool mine = turn == team;
         if (++turn == a.groups) turn = 0;
-        if (!mine) {  // another group's block: step over its slot and stages
-          if (++ps == a.packed) {
-            ps = 0;
-            pph ^= 1u;
-          }
-          if (++s == a.stages) {
-            s = 0;
-            ph ^= 1u;
-          }
+        if (!mine) {  // another group's block: step over its slot and stage
+          pk.next(a.packed);
+          st.next(kW4tStages);
           continue;
         }
-        if (!mbar_wait(&S.pfull[ps], pph, a.polls)) {
-          atomicOr(&S.s_err, kErrCopyTimeout);
-          ok = false;
-          break;
-        }
-        const unsigned char *pk = pring + (size_t)ps * pb;
+        ok = w4t_wait_group(smem_u32(&S.pfull[pk.at]), pk.phase, a.polls, 1 + team, q4 == 0);
+        if (!ok) break;
+        const unsigned char *p = pring + (size_t)pk.at * pb;
         uint4 q[4];
-        uint32_t sc[GPK], zz[GPK];  // scales (f16 pairs), zero points
 #pragma unroll
-        for (int c = 0; c < 4; ++c) q[c] = lds128(pk + (c * kW4Tile + m) * 16);
-#pragma unroll
-        for (int g = 0; g < GPK; ++g) {
-          const uint16_t bits = reinterpret_cast<const uint16_t *>(pk + kWords)[m * GPK + g];
-          const __half2 h = __float2half2_rn(W4Num<T>::scale(bits) * mul);
-          sc[g] = *reinterpret_cast<const uint32_t *>(&h);
-          zz[g] = ZP ? (uint32_t)pk[kWords + kScales + m * GPK + g] : 8u;
-        }
+        for (int c = 0; c < 4; ++c) q[c] = lds128(p + (c * kW4Tile + m) * 16);
+        const uint16_t scale = reinterpret_cast<const uint16_t *>(p + kWords)[m];
+        const W4Zero<T> zero(ZP ? (uint32_t)p[kWords + kScales + m] : 8u);
         __syncwarp();
-        if (lane == 0) mbar_arrive_cta(&S.pempty[ps]);
-        if (++ps == a.packed) {
-          ps = 0;
-          pph ^= 1u;
-        }
-        if (!mbar_wait(&S.empty[s], ph ^ 1u, a.polls)) {
-          atomicOr(&S.s_err, kErrCopyTimeout);
-          ok = false;
-        }
-        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (lane == 0) mbar_arrive_cta(&S.pempty[pk.at]);
+        pk.next(a.packed);
+        ok = w4t_wait_group(smem_u32(&S.empty[st.at]), st.phase ^ 1u, a.polls, 1 + team, q4 == 0);
         if (!ok) break;
         tc_fence_after();
+        reinterpret_cast<uint16_t *>(sring + (block % kW4tScaleSlots) * kScales)[m] = scale;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int g = j * GPK / 4;
-          const W4Zero<__half> zero(zz[g]);
           uint32_t x[16];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t w = j == 0 ? q[c].x : j == 1 ? q[c].y : j == 2 ? q[c].z : q[c].w;
             uint32_t y[4];
-            w4_unpack<__half>(w, bits, zero, y);
+            w4_unpack<T>(w, bits, zero, y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&y[e]),
-                                        *reinterpret_cast<const __half2 *>(&sc[g]));
-              x[4 * c + e] = *reinterpret_cast<const uint32_t *>(&v);
-            }
+            for (int e = 0; e < 4; ++e) x[4 * c + e] = y[e];
           }
-          w4t_st16(lane_base + (uint32_t)(s * kW4tACols + 16 * j), x);
+          w4t_st16(lane_base + (uint32_t)(st.at * kW4tACols + 16 * j), x);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cta(&S.full[s]);
-        if (++s == a.stages) {
-          s = 0;
-          ph ^= 1u;
-        }
+        if (lane == 0) mbar_arrive_cta(&S.full[st.at]);
+        st.next(kW4tStages);
       }
     }
-  } else if (warp > 3) {
-    const int q = warp & 3;  // TMEM lane quadrant of this warp
-    const int et = tid - 32 * (kW4tFirstConv + kW4tGroups * kW4tConvWarps);
-    grid_dep_wait();
-    for (int i = et; i < kW4tMaxN; i += 32 * kW4tEpiWarps)
-      S.fac[i] = a.row_fac && i < a.rows ? a.row_fac[i] : 1.f;
-    nbar_sync(1, 32 * kW4tEpiWarps);
+    if (!ok && lane == 0) atomicOr(&S.s_err, kErrCopyTimeout);
+  } else if (team >= kW4tTeams - a.sums) {
+    const int q4 = warp & 3, m = 32 * q4 + lane;
+    const int e = team - (kW4tTeams - a.sums), c0 = kW4tCols * e;  // first hidden row
+    const bool two = c0 + 16 < a.n_pad;
+    const uint32_t base = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)c0;
+    const uint32_t afull0 = smem_u32(&S.acc_full[0][0]), aempty0 = smem_u32(&S.acc_empty[0][0]);
+    unsigned char *stage8 = oring + (size_t)(4 * e + q4) * kW4tOutBytes;
+    T *stage = reinterpret_cast<T *>(stage8);
+    T *out = reinterpret_cast<T *>(a.out);
+    const uint32_t n_acc = (uint32_t)a.n_acc;
+    uint32_t block = 0u;
     bool ok = true;
-    for (int t = t0, i = 0; t < a.tiles && ok; t += G, ++i) {
-      const int buf = i % a.n_acc, use = i / a.n_acc;
-      if (!mbar_wait(&S.acc_full[buf], (uint32_t)(use & 1), a.polls)) {
-        atomicOr(&S.s_err, kErrCopyTimeout);
-        ok = false;
-      }
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const int v0 = t * kW4Tile + 32 * q, v = v0 + lane;
-      const float back = 1.f / __ldg(a.row_mul + v);  // a power of two
-      T *out = reinterpret_cast<T *>(a.out);
-      T *stage = reinterpret_cast<T *>(S.out[warp - kW4tEpi]);
-      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * a.n_pad);
-      for (int c = 0; c < a.n_pad; c += 32) {
-        uint32_t x[2][16];
-        tc_ld16(base + (uint32_t)c, x[0]);
-        if (c + 16 < a.n_pad) tc_ld16(base + (uint32_t)(c + 16), x[1]);
-        float4 fac[8];  // read before the stores below, which may alias them
+    for (int t = t0; t < a.tiles && ok; t += G) {
+      float sum[kW4tCols];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) fac[j] = *reinterpret_cast<const float4 *>(&S.fac[c + 4 * j]);
+      for (int j = 0; j < kW4tCols; ++j) sum[j] = 0.f;
+      for (int kb = 0; kb < a.nb && ok; ++kb, ++block) {
+        const uint32_t odd = block & 1u;
+        const W4tUse ac(block, n_acc);
+        const uint32_t bar = 8u * (odd * kW4tMaxAcc + ac.at);
+        ok = w4t_wait_group(afull0 + bar, ac.phase, a.polls, 1 + team, q4 == 0);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = base + (odd * n_acc + ac.at) * (uint32_t)a.n_pad;
+        uint32_t x[16];
+        tc_ld16(acc, x);
+        // (written before the MMAs that the wait was for)
+        const float scale = W4Num<T>::scale(
+            reinterpret_cast<const uint16_t *>(sring + (block % kW4tScaleSlots) * kScales)[m]);
         tc_wait_ld();
-        // through shared memory: 16-byte stores instead of 2-byte ones
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[j] = fmaf(scale, __uint_as_float(x[j]), sum[j]);
+        if (two) {
+          tc_ld16(acc + 16u, x);
+          tc_wait_ld();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) w4t_arrive(aempty0 + bar);
+        if (two)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            sum[16 + j] = fmaf(scale, __uint_as_float(x[j]), sum[16 + j]);
+      }
+      if (!ok) break;
+      // through shared memory: 16-byte stores instead of 2-byte ones
+      const int v0 = t * kW4Tile + 32 * q4, v = v0 + lane;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !two) break;
+        const int r0 = c0 + 16 * h;
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float4 f = fac[j >> 2];
-          const float fj = (j & 3) == 0 ? f.x : (j & 3) == 1 ? f.y : (j & 3) == 2 ? f.z : f.w;
-          stage[32 * j + lane] = from_float<T>(__uint_as_float(x[j >> 4][j & 15]) * back * fj);
-        }
+        for (int j = 0; j < 16; ++j) stage[32 * j + lane] = from_float<T>(sum[16 * h + j]);
         __syncwarp();
         if (a.vec) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = c + 8 * i + (lane >> 2), vv = v0 + 8 * (lane & 3);
+          for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 8 * i + (lane >> 2), vv = v0 + 8 * (lane & 3);
             if (r < a.rows && vv < a.V)
               *reinterpret_cast<uint4 *>(out + (long long)r * a.ldo + vv) =
-                  S.out[warp - kW4tEpi][32 * i + lane];
+                  lds128(stage8 + (32 * i + lane) * 16);
           }
         } else if (v < a.V) {
-          for (int j = 0; j < 32 && c + j < a.rows; ++j)
-            out[(long long)(c + j) * a.ldo + v] = stage[32 * j + lane];
+          for (int j = 0; j < 16 && r0 + j < a.rows; ++j)
+            out[(long long)(r0 + j) * a.ldo + v] = stage[32 * j + lane];
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cta(&S.acc_empty[buf]);
     }
+    if (!ok && lane == 0) atomicOr(&S.s_err, kErrCopyTimeout);
   }
   tc_fence_before();
   __syncthreads();

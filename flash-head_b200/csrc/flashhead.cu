@@ -29,6 +29,7 @@
 #include "fh_sample.cuh"
 #include "fh_w4.cuh"
 #include "fh_w4_tc.cuh"
+#include "fh_w4_split.cuh"
 
 static_assert(fh::kS2MaskWords == 8, "the selection kernel writes 8 bit-map words per cluster");
 
@@ -1783,13 +1784,11 @@ static fh::W4Args w4_args(const fh_w4_desc *d, const void *hidden, int rows, voi
   return a;
 }
 
-constexpr int kW4SmemMax = 227 * 1024;
-
 template <typename T, int GPK, bool ZP>
 static cudaError_t launch_w4_mv_t(const fh::W4Args &a, int grid, cudaStream_t s) {
   static bool done[128];
   auto kern = fh::k_w4_mv<T, GPK, ZP>;
-  const cudaError_t e = raise_smem(kern, kW4SmemMax, done);
+  const cudaError_t e = raise_smem(kern, fh::kW4SmemMax, done);
   if (e != cudaSuccess) return e;
   return launch(kern, dim3(grid), dim3(32 * fh::kW4Warps), fh::w4_mv_smem_bytes(a.nb), s, false,
                 a);
@@ -1801,14 +1800,24 @@ static cudaError_t launch_w4_probes_t(const fh::W4Args &a, unsigned grid, cudaSt
                 a);
 }
 
-template <typename T, int GPK, bool ZP>
+template <typename T, bool ZP>
 static cudaError_t launch_w4_tc_t(const CUtensorMap &tm, const fh::W4TcArgs &a, int grid,
-                                  size_t smem, bool pdl, cudaStream_t s) {
+                                  size_t smem, cudaStream_t s) {
   static bool done[128];
-  auto kern = fh::k_w4_tc<T, GPK, ZP>;
-  const cudaError_t e = raise_smem(kern, fh::kW4tSmemMax, done);
+  auto kern = fh::k_w4_tc<T, ZP>;
+  const cudaError_t e = raise_smem(kern, fh::kW4SmemMax, done);
   if (e != cudaSuccess) return e;
-  return launch(kern, dim3(grid), dim3(fh::kW4tThreads), smem, s, pdl, tm, a);
+  return launch(kern, dim3(grid), dim3(fh::kW4tThreads), smem, s, false, tm, a);
+}
+
+template <typename T, int GPK, bool ZP>
+static cudaError_t launch_w4_split_t(const CUtensorMap &tm, const fh::W4SplitArgs &a, int grid,
+                                     size_t smem, cudaStream_t s) {
+  static bool done[128];
+  auto kern = fh::k_w4_split<T, GPK, ZP>;
+  const cudaError_t e = raise_smem(kern, fh::kW4SmemMax, done);
+  if (e != cudaSuccess) return e;
+  return launch(kern, dim3(grid), dim3(fh::kW4sThreads), smem, s, false, tm, a);
 }
 
 // Calls f(T *, groups per block, zero points) for a descriptor.
@@ -1830,17 +1839,52 @@ static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
 #undef FH_W4_CASE
 }
 
+// What the two kernels for many rows share.
+template <typename Args>
+static Args w4_many_args(const fh_w4_desc *desc, int64_t out_stride, void *workspace) {
+  Args a;
+  memset(&a, 0, sizeof(a));
+  a.qw = desc->qweight;
+  a.scales = desc->scales;
+  a.zeros = desc->zeros;
+  a.V = desc->vocab;
+  a.D = desc->hidden;
+  a.nb = (desc->hidden + fh::kW4Block - 1) / fh::kW4Block;
+  a.tiles = (desc->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
+  a.mask = fh::kW4Mask;
+  a.magic = desc->dtype == FH_BF16 ? fh::W4Num<__nv_bfloat16>::kMagic : fh::W4Num<__half>::kMagic;
+  a.ldo = out_stride;
+  a.err = reinterpret_cast<uint32_t *>(workspace);
+  a.polls = 1u << 18;  // a wait is for one block: microseconds
+  return a;
+}
+
+// Rows r0 .. r0 + n of a call: the launch's outputs and its tensor map.
+template <typename Args>
+static bool w4_many_rows(const fh_w4_desc *desc, const void *hidden, int r0, int n, void *out,
+                         Args &a, CUtensorMap *tm) {
+  a.rows = n;
+  a.n_pad = (n + 15) / 16 * 16;
+  a.idesc = fh::s1tc_idesc(desc->dtype == FH_BF16, a.n_pad);
+  a.out = reinterpret_cast<char *>(out) + (size_t)r0 * a.ldo * 2;
+  a.vec = a.V % 8 == 0 && a.ldo % 8 == 0 && aligned16(a.out);
+  return encode_rows_map(tm, reinterpret_cast<const char *>(hidden) + (size_t)r0 * a.D * 2,
+                         desc->dtype, a.D, n, a.n_pad);
+}
+
 extern "C" {
 
 // Rows of a call that go through k_w4_mv (8 rows per pass of the weight); more
-// run on the tensor-core kernel. 2048 x 128256: 35 us for up to 8 rows against
-// 45..50 us there; 9..16 rows would be two passes, 70 us.
+// run on the tensor-core kernels. 2048 x 128256: 35 us for up to 8 rows against
+// 47..62 us there; 9..16 rows would be two passes, 70 us.
 constexpr int kW4MvRows = 8;
 
 FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows) {
   if (!desc || rows <= kW4MvRows) return 0;
-  size_t n = 256;
-  if (desc->dtype == FH_BF16)  // factors and the f16 copy of the hidden rows
+  size_t n = 256;  // the error word
+  // Not used since hidden rows are read as they are; callers that hold a
+  // workspace of this size keep it.
+  if (desc->dtype == FH_BF16)
     n += round_up((size_t)rows * sizeof(float), 256) + (size_t)rows * desc->hidden * 2;
   return n;
 }
@@ -1870,77 +1914,76 @@ static int run_w4_mv(const fh_w4_desc *desc, fh::W4Args a, int sms, cudaStream_t
   return FH_OK;
 }
 
+// Groups of 128: an accumulator per group.
 static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void *out,
-                     int64_t out_stride, void *workspace, size_t workspace_bytes, int sms,
-                     cudaStream_t s) {
-  if (!workspace || workspace_bytes < fh_w4_workspace_bytes(desc, rows))
-    return fail(FH_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu",
-                fh_w4_workspace_bytes(desc, rows), workspace ? workspace_bytes : (size_t)0);
-  if (!aligned16(workspace))
-    return fail(FH_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
-  unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
-  const int D = desc->hidden, gpk = fh::kW4Block / desc->group_size;
+                     int64_t out_stride, void *workspace, int sms, cudaStream_t s) {
   const bool zp = desc->zeros != nullptr;
-  fh::W4TcArgs a;
-  memset(&a, 0, sizeof(a));
-  a.qw = desc->qweight;
-  a.scales = desc->scales;
-  a.zeros = desc->zeros;
-  a.row_mul = desc->row_mul;
-  a.V = desc->vocab;
-  a.nb = (D + fh::kW4Block - 1) / fh::kW4Block;
-  a.D = D;
-  a.mask = fh::kW4Mask;
-  a.magic = fh::W4Num<__half>::kMagic;
-  a.tiles = (desc->vocab + fh::kW4Tile - 1) / fh::kW4Tile;
-  a.ldo = out_stride;
-  a.err = reinterpret_cast<uint32_t *>(ws);
-  a.polls = 1u << 18;  // a wait is for one block: microseconds
-  const void *hop = hidden;
-  float *fac = nullptr;
-  bool pdl = false;
-  if (desc->dtype == FH_BF16) {
-    fac = reinterpret_cast<float *>(ws + 256);
-    uint4 *h16 = reinterpret_cast<uint4 *>(ws + 256 + round_up((size_t)rows * sizeof(float), 256));
-    FH_CHECK_LAUNCH(launch(fh::k_w4_hidden, dim3(rows), dim3(256), 0, s, false,
-                           reinterpret_cast<const uint4 *>(hidden), h16, fac, D / 8, a.err),
-                    "hidden f16 copy launch");
-    hop = h16;
-    pdl = true;
-  } else {
-    FH_CHECK_LAUNCH(cudaMemsetAsync(ws, 0, sizeof(uint32_t), s), "error word reset");
-  }
-  for (int r0 = 0; r0 < rows; r0 += fh::kW4tMaxN) {
-    const int n = std::min(fh::kW4tMaxN, rows - r0);
-    a.rows = n;
-    a.n_pad = (n + 15) / 16 * 16;
-    // stages of 128 columns; the rest of shared memory is the packed ring
-    a.stages = a.n_pad <= 64 ? 4 : a.n_pad <= 128 ? 3 : 2;
-    // accumulators and A tiles share the 512 TMEM columns
-    a.n_acc = 2 * a.n_pad + a.stages * fh::kW4tACols <= 512 ? 2 : 1;
-    a.tmem_cols = 32;
-    while (a.tmem_cols < a.n_acc * a.n_pad + a.stages * fh::kW4tACols) a.tmem_cols *= 2;
-    a.idesc = fh::s1tc_idesc(false, a.n_pad);
-    a.row_fac = fac ? fac + r0 : nullptr;
-    a.out = reinterpret_cast<char *>(out) + (size_t)r0 * out_stride * 2;
-    const size_t used = 1024 + sizeof(fh::W4TcCtrl) + a.stages * fh::w4t_stage_bytes(a.n_pad);
-    a.packed = (int)std::min<size_t>(fh::kW4tMaxPacked, ((size_t)fh::kW4tSmemMax - used) /
-                                                            fh::w4t_packed_bytes(gpk, zp));
-    a.groups = fh::w4t_groups(a.stages, a.packed);
-    if (a.groups < 1) return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
-    a.vec = desc->vocab % 8 == 0 && out_stride % 8 == 0 && aligned16(a.out);
-    const size_t smem = fh::w4t_smem_bytes(a.n_pad, a.stages, a.packed, gpk, zp);
+  fh::W4TcArgs a = w4_many_args<fh::W4TcArgs>(desc, out_stride, workspace);
+  // launches of about the same number of rows
+  const int launches = (rows + fh::kW4tMaxN - 1) / fh::kW4tMaxN;
+  const int per = ((rows + launches - 1) / launches + 15) / 16 * 16;
+  for (int r0 = 0; r0 < rows; r0 += per) {
     CUtensorMap tm;
-    if (!encode_rows_map(&tm, reinterpret_cast<const char *>(hop) + (size_t)r0 * D * 2, FH_FP16, D,
-                         n, a.n_pad))
+    if (!w4_many_rows(desc, hidden, r0, std::min(per, rows - r0), out, a, &tm))
       return fail(FH_ERR_UNSUPPORTED, "hidden-state tensor map");
+    // accumulators (two warps') and A tiles share the 512 TMEM columns
+    a.n_acc = a.n_pad <= 64 ? 2 : 1;
+    a.sums = (a.n_pad + fh::kW4tCols - 1) / fh::kW4tCols;
+    a.tmem_cols = 32;
+    while (a.tmem_cols < 2 * a.n_acc * a.n_pad + fh::kW4tStages * fh::kW4tACols) a.tmem_cols *= 2;
+    // the groups that do not sum unpack, 4 or 2 of them; the rest of shared memory
+    // is the packed ring
+    const int most = fh::kW4tTeams - a.sums >= 4 ? 4 : 2;
+    const size_t other = fh::w4t_other_bytes(a.n_pad, a.sums), pb = fh::w4_packed_bytes(1, zp);
+    a.packed = (int)std::min<size_t>(fh::kW4tMaxPacked, ((size_t)fh::kW4SmemMax - other) / pb);
+    a.packed -= a.packed % most;
+    a.groups = std::min(fh::w4t_groups(fh::kW4tStages, a.packed), most);
+    if (a.groups < 1) return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
     const int grid = std::min(sms, a.tiles);
+    const size_t smem = other + a.packed * pb;
+    const cudaError_t e =
+        desc->dtype == FH_BF16
+            ? (zp ? launch_w4_tc_t<__nv_bfloat16, true>(tm, a, grid, smem, s)
+                  : launch_w4_tc_t<__nv_bfloat16, false>(tm, a, grid, smem, s))
+            : (zp ? launch_w4_tc_t<__half, true>(tm, a, grid, smem, s)
+                  : launch_w4_tc_t<__half, false>(tm, a, grid, smem, s));
+    FH_CHECK_LAUNCH(e, "4-bit tensor-core launch");
+  }
+  return FH_OK;
+}
+
+// Smaller groups: weights as the sum of two operands.
+static int run_w4_split(const fh_w4_desc *desc, const void *hidden, int rows, void *out,
+                        int64_t out_stride, void *workspace, int sms, cudaStream_t s) {
+  const int gpk = fh::kW4Block / desc->group_size;
+  const bool zp = desc->zeros != nullptr;
+  fh::W4SplitArgs a = w4_many_args<fh::W4SplitArgs>(desc, out_stride, workspace);
+  a.row_mul = desc->row_mul;
+  for (int r0 = 0; r0 < rows; r0 += fh::kW4sMaxN) {
+    CUtensorMap tm;
+    if (!w4_many_rows(desc, hidden, r0, std::min(fh::kW4sMaxN, rows - r0), out, a, &tm))
+      return fail(FH_ERR_UNSUPPORTED, "hidden-state tensor map");
+    // stages of 128 columns; the rest of shared memory is the packed ring.
+    // Accumulators and A tiles share the 512 TMEM columns.
+    a.stages = a.n_pad <= 64 ? 3 : 2;
+    a.n_acc = a.n_pad <= 128 ? 2 : 1;
+    a.tmem_cols = 32;
+    while (a.tmem_cols < a.n_acc * a.n_pad + a.stages * fh::kW4sACols) a.tmem_cols *= 2;
+    const size_t used = fh::w4s_smem_bytes(a.n_pad, a.stages, 0, gpk, zp);
+    a.packed = (int)std::min<size_t>(fh::kW4sMaxPacked, ((size_t)fh::kW4SmemMax - used) /
+                                                            fh::w4_packed_bytes(gpk, zp));
+    a.groups = fh::w4s_groups(a.stages, a.packed);
+    if (a.groups < 1) return fail(FH_ERR_UNSUPPORTED, "4-bit rings do not fit");
+    const int grid = std::min(sms, a.tiles);
+    const size_t smem = fh::w4s_smem_bytes(a.n_pad, a.stages, a.packed, gpk, zp);
     const cudaError_t e = w4_dispatch(desc, [&](auto *t, auto g, auto z) {
       using T = std::remove_pointer_t<decltype(t)>;
-      return launch_w4_tc_t<T, decltype(g)::value, decltype(z)::value>(tm, a, grid, smem, pdl, s);
+      if constexpr (decltype(g)::value > 1)
+        return launch_w4_split_t<T, decltype(g)::value, decltype(z)::value>(tm, a, grid, smem, s);
+      else
+        return cudaErrorInvalidValue;
     });
     FH_CHECK_LAUNCH(e, "4-bit tensor-core launch");
-    pdl = false;
   }
   return FH_OK;
 }
@@ -1955,8 +1998,16 @@ FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows, vo
                 desc->vocab);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  if (rows > kW4MvRows)
-    return run_w4_tc(desc, hidden, rows, out, out_stride, workspace, workspace_bytes, sms, s);
+  if (rows > kW4MvRows) {
+    if (!workspace || workspace_bytes < fh_w4_workspace_bytes(desc, rows))
+      return fail(FH_ERR_WORKSPACE, "workspace of %zu bytes needed, got %zu",
+                  fh_w4_workspace_bytes(desc, rows), workspace ? workspace_bytes : (size_t)0);
+    if (!aligned16(workspace))
+      return fail(FH_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    FH_CHECK_LAUNCH(cudaMemsetAsync(workspace, 0, sizeof(uint32_t), s), "error word reset");
+    auto run = desc->group_size == fh::kW4Block ? run_w4_tc : run_w4_split;
+    return run(desc, hidden, rows, out, out_stride, workspace, sms, s);
+  }
   fh::W4Args a = w4_args(desc, hidden, rows, out);
   a.ldo = out_stride;
   return run_w4_mv(desc, a, sms, s);

@@ -10,9 +10,9 @@ w[v, k] = (q[v, k] - z[v, g]) * s[v, g], q in 0..15, one scale (and zero point;
 8 without zero points) per group g = k // group_size of a row. The kernels
 (``csrc/fh_w4.cuh``) sum exact products of q - z and the hidden states in fp32
 and scale each group's sum in fp32; results are rounded once, to the hidden
-states' dtype. ``w4_logits`` of more than 8 rows runs on the tensor cores with w
-rounded to 11 bits (``csrc/fh_w4_tc.cuh``). ``w4_block_sparse_logits`` is the 4-bit form of
-``flash_head.fused.block_sparse_logits`` (reference
+states' dtype. ``w4_logits`` of more than 8 rows runs on ``csrc/fh_w4_tc.cuh``,
+or ``csrc/fh_w4_split.cuh``, which sum the same products in another order. ``w4_block_sparse_logits`` is the
+4-bit form of ``flash_head.fused.block_sparse_logits`` (reference
 ``src/flash_head/fused.py:82-93``).
 """
 
@@ -84,11 +84,10 @@ class W4Weight:
         d.dtype = _lib.dtype_code(scales.dtype)
         d.qweight, d.scales = qweight.data_ptr(), scales.data_ptr()
         d.zeros = None if zeros is None else zeros.data_ptr()
-        # powers of two that bring a row's largest scale to [1, 2)
+        # rows whose weights may pass the type's largest number, brought down by 2^-4
         top = scales.float().abs().amax(dim=(1, 3)).view(-1)
-        fine = torch.isfinite(top) & (top > 0)
-        exp = torch.frexp(torch.where(fine, top, torch.ones_like(top))).exponent
-        self.row_mul = torch.ldexp(torch.ones_like(top), 1 - exp).contiguous()
+        limit = 2.0 ** (12 if scales.dtype == torch.float16 else 124)
+        self.row_mul = torch.where(torch.isfinite(top) & (top > limit), 2.0 ** -4, 1.0)
         d.row_mul = self.row_mul.data_ptr()
         self.desc, self.ref = d, ctypes.byref(d)
 

@@ -367,10 +367,11 @@ FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
 /*
  * Products with a head weight held in 4 bits (no counterpart in the
  * reference): w[v, k] = (q[v, k] - z[v, g]) * s[v, g] with q in 0..15 and one
- * scale s (and zero point z) per group g = k / group_size of a row. Up to 8
- * rows, and for probed clusters, the products (q - z) * h are exact, summed in
- * fp32 and scaled in fp32 by group; beyond, (q - z) * s is rounded to 11 bits
- * once. Results are rounded once, to the hidden states' type.
+ * scale s (and zero point z) per group g = k / group_size of a row. The
+ * products (q - z) * h are exact, summed in fp32 and scaled in fp32 by group;
+ * results are rounded once, to the hidden states' type. The order of the sums
+ * depends on the number of rows (up to 8, or more). A hidden row that holds an
+ * infinity or a NaN has logits that are infinite or NaN.
  *
  *   vocab      V, weight rows
  *   hidden     D, columns: a multiple of group_size, at most FH_W4_MAX_HIDDEN
@@ -382,8 +383,9 @@ FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
  *              4i..4i+3, e = 2i + 1 in bits 16+4i..19+4i
  *   scales     [T][B][128][128 / group_size]; 0 in padded rows and groups
  *   zeros      u8, the shape of scales; NULL: every zero point is 8
- *   row_mul    fp32 [128 T], powers of two that bring the largest scale of each
- *              row to [1, 2) (1 for a row without finite scales above 0)
+ *   row_mul    fp32 [128 T], a power of two per row, divided out again: 2^-4 for a
+ *              row whose largest scale is finite and above 2^12 (FH_FP16) or
+ *              2^124 (FH_BF16), so that 15 s is a number of the type; else 1
  * The Python loader (flash_head/w4.py) makes this layout. Pointers 16-byte
  * aligned, device memory.
  */
