@@ -36,8 +36,9 @@
 // Bound: the issue of the MMAs, some 46 clocks each whatever N is up to 128 (twice
 // the warps that unpack changed nothing), their rate beyond. 2048 x 128256, zero
 // points: 16 rows 62 us, 64 68 us, 256 183 us.
-// Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
-// drains its own copies and MMAs (bounded) and frees TMEM before it returns.
+// Every wait is bounded; on a timeout the CTA drains its own copies and MMAs
+// (bounded), frees TMEM, fills the logits of its tiles with NaN and records
+// kErrCopyTimeout.
 #pragma once
 
 #include "fh_w4_tc.cuh"
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
       }
       // every copy this thread issued has landed before the CTA may leave
       for (int j = 0; j < a.packed; ++j)
-        if (issued[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued[j], a.polls))
+        if (issued[j] >= 0 && !mbar_wait(&S.pfull[j], (uint32_t)issued[j], kW4DrainPolls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 2) {
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
         }
       }
       for (int j = 0; j < a.stages; ++j)
-        if (issued[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued[j], a.polls))
+        if (issued[j] >= 0 && !mbar_wait(&S.full[j], (uint32_t)issued[j], kW4DrainPolls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 1) {
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
     if (leader) {
       if (!ok) atomicOr(&S.s_err, kErrCopyTimeout);
       tc_commit(&S.drain);
-      if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
+      if (!mbar_wait(&S.drain, 0u, kW4DrainPolls)) atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp >= kW4sFirstConv && warp < kW4sFirstConv + kW4sGroups * kW4sConvWarps) {
     const int group = (warp - kW4sFirstConv) / kW4sConvWarps;
@@ -422,7 +423,10 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
                  "r"(a.tmem_cols)
                  : "memory");
   }
-  if (tid == 0 && S.s_err) atomicOr(a.err, S.s_err);
+  if (S.s_err) {
+    w4t_fill(reinterpret_cast<T *>(a.out), a.ldo, a.rows, a.V, t0, a.tiles, G);
+    if (tid == 0) atomicOr(a.err, S.s_err);
+  }
 }
 
 }  // namespace fh

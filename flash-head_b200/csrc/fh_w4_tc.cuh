@@ -43,8 +43,9 @@
 // 75 and 148 us (0.9 PFLOP/s). Tried and slower: polls with a time hint, fp32x2
 // multiply-adds, half as many warps that sum 64 rows each, and twice as many that
 // take every other block.
-// Every wait is bounded; on a timeout the kernel records kErrCopyTimeout,
-// drains its own copies and MMAs (bounded) and frees TMEM before it returns.
+// Every wait is bounded; on a timeout the CTA drains its own copies and MMAs
+// (bounded), frees TMEM, fills the logits of its tiles with NaN and records
+// kErrCopyTimeout.
 #pragma once
 
 #include "fh_s1_tc.cuh"
@@ -71,6 +72,9 @@ constexpr int kW4tScaleSlots = 8;
 static_assert(kW4tScaleSlots >= kW4tStages + 2 * kW4tMaxAcc, "a slot may still be read");
 constexpr int kW4tOutBytes = 32 * 16 * 2;  // a warp's outputs, 16 hidden rows at a time
 constexpr int kW4SmemMax = 227 * 1024;
+// Polls for copies and MMAs in flight before a CTA leaves: milliseconds, for what
+// takes microseconds. (The limit of the other waits may be set to less.)
+constexpr uint32_t kW4DrainPolls = 1u << 14;
 
 struct W4TcArgs {
   const uint32_t *qw;
@@ -126,6 +130,18 @@ __host__ __device__ inline size_t w4_stage_bytes(int n_pad) {
 __host__ __device__ inline size_t w4t_other_bytes(int n_pad, int sums) {
   return 1024 + kW4tStages * w4_stage_bytes(n_pad) + (size_t)kW4tScaleSlots * kW4Tile * 2 +
          (size_t)sums * 4 * kW4tOutBytes + sizeof(W4TcCtrl);
+}
+
+// NaN in the rows x 128 logits of a CTA's tiles t, t + step, ...
+template <typename T>
+__device__ __noinline__ void w4t_fill(T *out, long long ldo, int rows, int V, int t, int tiles,
+                                      int step) {
+  const T nan = from_float<T>(__int_as_float(0x7FFFFFFF));
+  for (; t < tiles; t += step)
+    for (int i = threadIdx.x; i < rows * kW4Tile; i += blockDim.x) {
+      const int v = t * kW4Tile + i % kW4Tile;
+      if (v < V) out[(long long)(i / kW4Tile) * ldo + v] = nan;
+    }
 }
 
 // mbar_wait by shared-memory address.
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
       }
       // every copy this thread issued has landed before the CTA may leave
       for (int j = 0; j < a.packed; ++j)
-        if ((sent >> j) & 1u && !mbar_wait(&S.pfull[j], (parity >> j) & 1u, a.polls))
+        if ((sent >> j) & 1u && !mbar_wait(&S.pfull[j], (parity >> j) & 1u, kW4DrainPolls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 2) {
@@ -323,7 +339,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
         }
       }
       for (int j = 0; j < kW4tStages; ++j)
-        if ((sent >> j) & 1u && !mbar_wait(&S.hfull[j], (parity >> j) & 1u, a.polls))
+        if ((sent >> j) & 1u && !mbar_wait(&S.hfull[j], (parity >> j) & 1u, kW4DrainPolls))
           atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (warp == 1 || warp == 3) {
@@ -370,7 +386,7 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
     if (leader) {
       if (!ok) atomicOr(&S.s_err, kErrCopyTimeout);
       tc_commit(&S.drain);
-      if (!mbar_wait(&S.drain, 0u, a.polls)) atomicOr(&S.s_err, kErrCopyTimeout);
+      if (!mbar_wait(&S.drain, 0u, kW4DrainPolls)) atomicOr(&S.s_err, kErrCopyTimeout);
     }
   } else if (team < a.groups) {
     const int q4 = warp & 3, m = 32 * q4 + lane;  // this thread's row of the tile
@@ -505,7 +521,10 @@ __global__ void __launch_bounds__(kW4tThreads, 1)
                  "r"(a.tmem_cols)
                  : "memory");
   }
-  if (tid == 0 && S.s_err) atomicOr(a.err, S.s_err);
+  if (S.s_err) {
+    w4t_fill(reinterpret_cast<T *>(a.out), a.ldo, a.rows, a.V, t0, a.tiles, G);
+    if (tid == 0) atomicOr(a.err, S.s_err);
+  }
 }
 
 }  // namespace fh

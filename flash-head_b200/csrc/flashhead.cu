@@ -1839,6 +1839,11 @@ static cudaError_t w4_dispatch(const fh_w4_desc *d, F f) {
 #undef FH_W4_CASE
 }
 
+// Polls of a wait of the kernels for many rows; a wait is for one block:
+// microseconds.
+constexpr uint32_t kW4Polls = 1u << 18;
+static std::atomic<uint32_t> g_w4_polls{kW4Polls};
+
 // What the two kernels for many rows share.
 template <typename Args>
 static Args w4_many_args(const fh_w4_desc *desc, int64_t out_stride, void *workspace) {
@@ -1855,7 +1860,7 @@ static Args w4_many_args(const fh_w4_desc *desc, int64_t out_stride, void *works
   a.magic = desc->dtype == FH_BF16 ? fh::W4Num<__nv_bfloat16>::kMagic : fh::W4Num<__half>::kMagic;
   a.ldo = out_stride;
   a.err = reinterpret_cast<uint32_t *>(workspace);
-  a.polls = 1u << 18;  // a wait is for one block: microseconds
+  a.polls = g_w4_polls.load(std::memory_order_relaxed);
   return a;
 }
 
@@ -2011,6 +2016,10 @@ FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows, vo
   fh::W4Args a = w4_args(desc, hidden, rows, out);
   a.ldo = out_stride;
   return run_w4_mv(desc, a, sms, s);
+}
+
+FH_API uint32_t fh_w4_wait_polls(uint32_t polls) {
+  return g_w4_polls.exchange(std::min(polls, kW4Polls), std::memory_order_relaxed);
 }
 
 FH_API int fh_w4_block_sparse_logits(const fh_w4_desc *desc, const void *hs, int T,

@@ -131,6 +131,7 @@ SIGNATURES = {
     "fh_sample_logits": (_I, [_P, _I, _I, _I, _I64, ctypes.POINTER(SampleParams), _P, _P, _P]),
     "fh_w4_workspace_bytes": (_SZ, [ctypes.POINTER(W4Desc), _I]),
     "fh_w4_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I64, _P, _SZ, _P]),
+    "fh_w4_wait_polls": (ctypes.c_uint32, [ctypes.c_uint32]),
     "fh_w4_block_sparse_logits": (_I, [ctypes.POINTER(W4Desc), _P, _I, _P, _I, _I, _I, _P, _P]),
     "fh_spec_accept": (_I, [_P, _P, _P, _P, _I, _I, ctypes.c_int32, _P, _P]),
 }

@@ -10,9 +10,10 @@ w[v, k] = (q[v, k] - z[v, g]) * s[v, g], q in 0..15, one scale (and zero point;
 8 without zero points) per group g = k // group_size of a row. The kernels
 (``csrc/fh_w4.cuh``) sum exact products of q - z and the hidden states in fp32
 and scale each group's sum in fp32; results are rounded once, to the hidden
-states' dtype. ``w4_logits`` of more than 8 rows runs on ``csrc/fh_w4_tc.cuh``,
-or ``csrc/fh_w4_split.cuh``, which sum the same products in another order. ``w4_block_sparse_logits`` is the
-4-bit form of ``flash_head.fused.block_sparse_logits`` (reference
+states' dtype. ``w4_logits`` of more than 8 rows runs on ``csrc/fh_w4_tc.cuh`` or
+``csrc/fh_w4_split.cuh``, which sum the same products in another order.
+``w4_block_sparse_logits`` is the 4-bit form of
+``flash_head.fused.block_sparse_logits`` (reference
 ``src/flash_head/fused.py:82-93``).
 """
 
@@ -232,7 +233,10 @@ def _check(hs: torch.Tensor, w: W4Weight) -> torch.Tensor:
 def w4_logits(hs: torch.Tensor, w: W4Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, D] hidden states -> [T, V] logits in their dtype.
 
-    ``out`` may be any [T, V] tensor of that dtype with contiguous rows."""
+    ``out`` may be any [T, V] tensor of that dtype with contiguous rows. Should one
+    of the kernels' bounded waits run out (more than 8 rows; none does on a GPU that
+    works), the logits that depend on it are NaN, which ``sample_logits`` takes for
+    masked: -1 for a row without any other."""
     hs = _check(hs, w)
     T = hs.shape[0]
     if out is None:

@@ -406,11 +406,17 @@ typedef struct fh_w4_desc {
  * flash_head.py:292-301). out_stride >= V, in elements. The workspace
  * (fh_w4_workspace_bytes; where that is 0, NULL is fine) needs no zeroing; its
  * first 32-bit word is 0 after a call, or has bit 1 set where a bounded wait
- * inside the call ran out (the outputs are then meaningless). */
+ * inside the call ran out: the logits that depend on it are then NaN. */
 FH_API size_t fh_w4_workspace_bytes(const fh_w4_desc *desc, int rows);
 FH_API int fh_w4_logits(const fh_w4_desc *desc, const void *hidden, int rows,
                         void *out, int64_t out_stride, void *workspace,
                         size_t workspace_bytes, fh_stream_t stream);
+
+/* Polls after which a wait inside a later fh_w4_logits call gives up (at most, and
+ * by default, 2^18: far beyond what a wait takes); returns the number before.
+ * 0 makes every call of more than 8 rows give up at once, which shows a caller what
+ * that looks like. */
+FH_API uint32_t fh_w4_wait_polls(uint32_t polls);
 
 /* fused.py:82-93 over a 4-bit w_perm (weight row = cluster * cluster_size +
  * slot): ci [T, P] int64 cluster ids, out [T, P * cluster_size]. Candidates of
