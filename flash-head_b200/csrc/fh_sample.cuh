@@ -219,9 +219,10 @@ __constant__ double kSmpExp2[10] = {
 // the integer next to ref * c, so that x c - k0 is rounded once (fma) however
 // large the two are. With 1.5 * 2^52 added, the sum's low word is its nearest
 // integer n; the rest f is within 1/2, 2^f a polynomial, and n is added to the
-// exponent. Masses below 2^-72 of the reference's are dropped: less than the
-// rounding of their sum. `depth` is the same exponent, falling and in fp32: a
-// monotone measure of how far down a logit lies.
+// exponent. Masses below 2^-1000 of the reference's are none (2^n would leave the
+// normal numbers); all others count, as u = 0 draws the first kept column however
+// small its mass. `depth` is the same exponent, falling and in fp32: a monotone
+// measure of how far down a logit lies.
 // For |ref| c above 2^40 neighbouring fp32 logits differ by a factor of 2^(2^16):
 // c is held there, where only the reference's equals keep a mass (`held`).
 struct SmpMass {
@@ -234,7 +235,7 @@ struct SmpMass {
     c = held ? most / fabs((double)ref) : c0;
     k0 = rint((double)ref * c);
     k1 = 6755399441055744.0 - k0;
-    xlo = fminf((float)((double)ref - 72.0 / c), nextafterf(ref, -INFINITY));
+    xlo = fminf((float)((double)ref - 1000.0 / c), nextafterf(ref, -INFINITY));
     cf = fminf((float)(2.0 * c), 3.402823466e38f);
   }
   // halved first: ref - x may pass the largest fp32. Rounded here, so that it
@@ -872,7 +873,9 @@ __device__ __forceinline__ float smp_segment(Ctx &C, const SmpMass &w, const Smp
 }
 
 // The draw from the prefix `cut` of the whole row: the segments' masses are in
-// warp_* of every CTA, in units of 2^warp_k; w gives masses in units of 2^w.k0.
+// warp_* of every CTA, in units of 2^warp_k; w gives masses in units of 2^w.k0. A
+// segment whose largest logit has no mass in those units has none, whatever its sum
+// in its own: the walk through the segment of the draw has to find a mass.
 template <typename E, typename Ctx>
 __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const SmpMass &w,
                                              const SmpCut &cut, double tie_w, int r, double u) {
@@ -896,6 +899,7 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
     seg_ties = R->warp_i[tid % kSmpWarps];
     const double shift = R->warp_k[tid % kSmpWarps] - w.k0;
     if (shift != 0.0) mass = ldexp(mass, (int)fmax(-2000.0, fmin(shift, 2000.0)));
+    if (!(R->warp_f[tid % kSmpWarps] > above)) mass = 0.0;
   }
   long long left = cut.ties;
   if (cut.ties > 0) {

@@ -1,0 +1,73 @@
+"""Filtered sampling where the draw lies at an end of the row: every row's id
+and probability are written, and are the definition's in 64 bits.
+
+An entry counts while e_i is a 64-bit number well above the smallest (the rows
+here stay above 2^-1000 of the largest), so u = 0 takes the first kept column
+however small its mass. Ids must be equal; the probability is rounded once, to
+fp32 (see test_gpu_sampling.py for the 64-bit errors).
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from flash_head.sampling import sample_logits
+from test_gpu_sampling import logits, oracle_row
+
+pytestmark = pytest.mark.gpu
+
+LAST = 1.0 - 2.0 ** -53
+
+
+def check(x, u, T=1.0, k=0, p=1.0, m=0.0, alike=False):
+    """alike: every row has the same logits and the same u."""
+    B = x.shape[0]
+    out = torch.full((B,), -77, dtype=torch.int64, device="cuda")
+    got, prob = sample_logits(x, u, T, k, p, m, out=out, return_prob=True)
+    f32 = [np.float64(np.float32(v)) for v in (T, p, m)]
+    some = 1 if alike else B
+    xn, un = x[:some].float().cpu().double().numpy(), u.cpu().numpy()
+    want = [oracle_row(xn[r], un[r], f32[0], k, f32[1], f32[2]) for r in range(some)]
+    want *= B // some
+    cols = np.array([c for c, _ in want])
+    assert np.array_equal(got.cpu().numpy(), cols), \
+        [(int(r), int(got[r]), int(cols[r])) for r in np.flatnonzero(got.cpu().numpy() != cols)[:8]]
+    pw = np.array([q for _, q in want])
+    assert (np.abs(prob.cpu().double().numpy() - pw) <= pw * (2.0 ** -24 + 2.0 ** -40) + 1e-40).all()
+
+
+def ends(B):
+    """u = 0 and the largest below 1, by turns."""
+    return torch.tensor([0.0, LAST], dtype=torch.float64, device="cuda").repeat(B)[:B]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,n", [(2, 128256), (8, 40000), (300, 20000)])
+@pytest.mark.parametrize("bits", [60, 80, 300, 800, 940])
+def test_a_first_stretch_far_below_the_largest(B, n, bits, dtype):
+    """The first eighth of the row lies `bits` binary orders below its largest."""
+    T = 0.5
+    x = logits(B, n, dtype, 5, sigma=0.5, peak=False)
+    x[:, n // 8:] += bits * T * 0.6931472
+    u = ends(B)
+    check(x, u, T=T)
+    check(x, u, T=T, m=1e-30)
+    check(x, u, T=T, k=n - 5)
+    check(x, u, T=T, p=0.9999999)
+
+
+@pytest.mark.parametrize("u", [0.0, 2.0 ** -24, LAST])
+def test_a_kept_entry_far_below_the_largest(u):
+    """Short rows: the list of the candidates has the same rule."""
+    B = 4
+    for n in (50, 3000, 9000):
+        x = torch.full((B, n), float("-inf"))
+        x[:, 3] = -120.0
+        x[:, n // 2] = 5.0
+        x[:, n - 2] = 4.0
+        x = x.cuda()
+        uu = torch.full((B,), u, dtype=torch.float64, device="cuda")
+        for kw in ({}, {"k": 3}, {"k": 2}, {"p": 0.999}, {"T": 0.25, "k": 3}):
+            check(x, uu, **kw)
