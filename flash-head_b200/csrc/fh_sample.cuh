@@ -923,12 +923,38 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
   __syncthreads();
   if (seg / kSmpWarps != C.rank) return;
   // the segment in pieces of kSmpChunk vectors: their masses, then the vector
-  // of the draw, then its entry
+  // of the draw, then its entry. The target may lie past the end by rounding:
+  // the last entry with a mass then, which any piece may hold.
   const int sv0 = (int)((long long)C.span.row.nv * seg / segs);
   const int sv1 = (int)((long long)C.span.row.nv * (seg + 1) / segs);
   constexpr int kEach = kSmpChunk / kSmpThreads;
   double run = S.seg_before;
   left = S.seg_left;
+  // the first entry of vector v beyond the target, or the last kept one; `to`:
+  // the mass before it, `ties`: how many equal entries are still kept there
+  const auto emit = [&](int v, double to, long long ties) {
+    float f[kVec];
+    C.span.row.unpack(C.span.row.raw(v), f);
+    int col = -1;
+    double x = 0.0;
+    bool found = false;
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) {
+      double e = 0.0;
+      if (f[q] > above)
+        e = w.raw(f[q]);
+      else if (cut.ties > 0 && f[q] == xc && ties-- > 0)
+        e = tie_w;
+      to += e;
+      if (e > 0.0 && !found) {
+        col = C.span.row.column(v) + q;
+        x = e;
+        found = to > target;
+      }
+    }
+    smp_emit<E>(a, r, col, x / total);
+  };
+  int kept = -1;  // the last vector with a mass of the pieces so far
   for (int c0 = sv0; c0 < sv1; c0 += kSmpChunk) {
     const int cn = min(kSmpChunk, sv1 - c0);
     __syncthreads();
@@ -989,43 +1015,29 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
     if (hit != 0x7FFFFFFF) atomicMin(&S.best, hit);
     if (last >= 0) atomicMax(&S.last, last);
     __syncthreads();
-    // past the end by rounding: the last vector with a mass
-    const int at = S.best != 0x7FFFFFFF ? S.best : c0 + kSmpChunk >= sv1 ? S.last : -1;
-    if (at >= 0) {
-      if (at / kEach == tid) {
-        // the vector's entries: the first beyond the target, or the last kept
+    const int at = S.best;
+    const int in = at != 0x7FFFFFFF ? at : S.last;  // the vector to go back to
+    if (in >= 0) {
+      kept = c0 + in;
+      if (in / kEach == tid) {
         double to = base;
-        long long lft = 0;
+        long long ties = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-          if (tid * kEach + i < at) to += m[i];
-          if (cut.ties > 0 && tid * kEach + i == at) lft = l[i];
+          if (tid * kEach + i < in) to += m[i];
+          if (cut.ties > 0 && tid * kEach + i == in) ties = l[i];
         }
-        float f[kVec];
-        C.span.row.unpack(C.span.row.raw(c0 + at), f);
-        int col = -1;
-        double x = 0.0;
-        bool found = false;
-#pragma unroll
-        for (int q = 0; q < kVec; ++q) {
-          double e = 0.0;
-          if (f[q] > above)
-            e = w.raw(f[q]);
-          else if (cut.ties > 0 && f[q] == xc && lft-- > 0)
-            e = tie_w;
-          to += e;
-          if (e > 0.0 && !found) {
-            col = C.span.row.column(c0 + at) + q;
-            x = e;
-            found = to > target;
-          }
-        }
-        smp_emit<E>(a, r, col, x / total);
+        if (at != 0x7FFFFFFF)
+          emit(kept, to, ties);
+        else
+          S.seg_left = ties;
       }
-      return;
     }
+    if (at != 0x7FFFFFFF) return;
     run += piece;
   }
+  __syncthreads();
+  if (tid == 0) emit(kept, -INFINITY, S.seg_left);
 }
 
 // The first pass of the list path: the thread's largest logit, the entries

@@ -71,3 +71,17 @@ def test_a_kept_entry_far_below_the_largest(u):
         uu = torch.full((B,), u, dtype=torch.float64, device="cuda")
         for kw in ({}, {"k": 3}, {"k": 2}, {"p": 0.999}, {"T": 0.25, "k": 3}):
             check(x, uu, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("left", [1, 3, 2100 * 8, 60000])
+def test_a_masked_tail_of_a_long_segment(left, dtype):
+    """One CTA per row, so that a warp's segment is walked in several pieces;
+    the row's last entries are masked, and u is at its end."""
+    B, n = 300, 151936
+    x = logits(B, n, dtype, 8, sigma=1.5, peak=False)
+    x[:, left:] = float("-inf")
+    u = torch.full((B,), LAST, dtype=torch.float64, device="cuda")
+    check(x, u)
+    check(x, u, m=1e-6)
+    check(x, torch.full_like(u, 1.5))
