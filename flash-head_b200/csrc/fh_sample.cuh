@@ -1459,10 +1459,14 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xFFFFFFFFu, ref, o));
-    if (!(fabsf(ref) < INFINITY)) ref = 0.f;
+    // (0 stands in for first entries that are all masked, or +inf: then the
+    // others' masses are good only near it)
+    const bool known = fabsf(ref) < INFINITY;
+    if (!known) ref = 0.f;
     w = SmpMass(ref, T);
     m = smp_segment<true, false>(C, w, cut);
-    bad = w.held || w.depth(m) < -900.f;
+    const float deep = w.depth(m);
+    bad = w.held || deep < -900.f || (!known && m > -INFINITY && deep > 60.f);
   } else if (fast) {
     if (a.n > kSmpList)
       smp_sample(C, use_k ? 1.1f * (float)k + 10.f * sqrtf((float)k) + 32.f : 600.f, fast_lo, ref);

@@ -85,3 +85,27 @@ def test_a_masked_tail_of_a_long_segment(left, dtype):
     check(x, u)
     check(x, u, m=1e-6)
     check(x, torch.full_like(u, 1.5))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,n", [(2, 128256), (300, 40000)])
+@pytest.mark.parametrize("T,level", [(1.0, -30.0), (1.0, -80.0), (0.1, -90.0), (1.0, -2000.0)])
+def test_masked_beginnings_and_logits_far_below_zero(B, n, T, level, dtype):
+    """Log-probabilities, and a mask over the first entries of every warp's
+    segment: what is left lies far from the 0 that a mask leaves as a reference."""
+    x = logits(B, n, dtype, 6, sigma=1.0, peak=False) + level
+    segments = 64 if B == 2 else 8
+    at = torch.arange(n, device="cuda") % (n // segments)
+    x[:, at < 400] = float("-inf")
+    g = torch.Generator().manual_seed(4)
+    u = torch.rand(B, generator=g, dtype=torch.float64).cuda()
+    check(x, u, T=T)
+    check(x, torch.zeros_like(u), T=T)
+    # At 1 - 2^-53 the mass behind the draw is no more than the rounding of the
+    # sums (n of them, half a step each): any of the columns there will do.
+    got = sample_logits(x, torch.full_like(u, LAST), T,
+                        out=torch.full((B,), -77, dtype=torch.int64, device="cuda"))
+    e = torch.exp((x.double() - x.double().amax(1, keepdim=True)) / float(np.float32(T)))
+    share = (e.cumsum(1) / e.sum(1, keepdim=True)).gather(1, got.clamp_min(0).view(B, 1))
+    assert (got >= 0).all() and (share >= 1 - n * 2.0 ** -52).all()
+    assert (x.gather(1, got.view(B, 1)) > float("-inf")).all()
