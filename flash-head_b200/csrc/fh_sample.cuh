@@ -1042,11 +1042,15 @@ __device__ __forceinline__ void smp_draw_row(Ctx &C, const SampleArgs &a, const 
 
 // The first pass of the list path: the thread's largest logit, the entries
 // above `lo` into the CTA's list and, MASS, the row's mass relative to `ref` in
-// fp32, kSmpSlack of it off at most: with t = (x - ref) c, the difference is
-// off by 2^-24 |t| (t > -100, and below 2^-32 nothing counts), c's second word
-// corrects its product, and ex2 (2^-22), the products and a vector's sum add
-// 2^-20.
-constexpr double kSmpSlack = 3.8147e-6;  // 2^-18
+// fp32, smp_slack of it off at most: with t = (x - ref) c, the difference is
+// off by 2^-24 |t| (t > -100, and below 2^-32 nothing counts; above the reference
+// up to the row's largest t), c's second word corrects its product, and ex2
+// (2^-22), the products and a vector's sum add 2^-20.
+constexpr double kSmpSlack = 3.8147e-6;  // 2^-18, where no logit is above `ref`
+__device__ __forceinline__ double smp_slack(float m, float ref, double c) {
+  const double t = ((double)m - (double)ref) * c;
+  return kSmpSlack + (t > 0.0 ? 0x1p-24 * t : 0.0);
+}
 __device__ __forceinline__ float smp_ex2(float t) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
@@ -1316,7 +1320,7 @@ __device__ __forceinline__ SmpDeep smp_deep(Ctx &C, const SampleArgs &a, const S
       if (C.rank == 0) {
         const double slack = kSmpSlack + 0x1p-24 * (32.0 + (double)C.span.row.n /
                                                                (double)(kSmpThreads * C.size));
-        const double target = (double)p * z * exp2((double)ref * w.c - w.k0);
+        const double target = (double)p * z * exp2(fma((double)ref, w.c, -w.k0));
         bool sure = false;
         const SmpPick pick = smp_pick(S, w, got, least, 0, (double)p, target * (1.0 - slack), 0.0,
                                       target * (1.0 + slack), &sure);
@@ -1581,14 +1585,15 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
       smp_gather(C);
       if (rank != 0 && known) return;
       if (rank == 0) {
-        // a row's mass known to a factor of 1 +- kSmpSlack is enough, unless the
+        // a row's mass known to a factor of 1 +- smp_slack is enough, unless the
         // cut falls between the two
         double target = -1.0, most = 0.0;
         bool sure = false;
         if (!known) {
-          target = (double)p * z_row * exp2((double)ref * w.c - w.k0);
-          most = target * (1.0 + kSmpSlack);
-          target *= 1.0 - kSmpSlack;
+          const double slack = smp_slack(m, ref, c);
+          target = (double)p * z_row * exp2(fma((double)ref, w.c, -w.k0));
+          most = target * (1.0 + slack);
+          target *= 1.0 - slack;
         }
         const SmpPick pick = smp_pick(S, w, (int)listed, cut.key, use_k ? k : 0,
                                       use_p ? (double)p : 1.0, target, 0.0, most, &sure);

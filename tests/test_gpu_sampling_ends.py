@@ -87,6 +87,54 @@ def test_a_masked_tail_of_a_long_segment(left, dtype):
     check(x, torch.full_like(u, 1.5))
 
 
+@pytest.mark.parametrize("B,n", [(1, 151936), (300, 151936), (3, 128256)])
+@pytest.mark.parametrize("T,low,top", [
+    (0.1, 1.6745601, 9.715551), (0.1, 1.0, 9.3), (0.05, -3.0, 1.2), (0.2, 0.0, 17.0),
+    (1.0, 0.0, 80.0), (1.0, -20.0, 10.0)])
+def test_top_p_next_to_a_border_at_low_temperatures(B, n, T, low, top):
+    """A few equal logits hold all the mass, and top_p is the next number above
+    (below) the share of some of them: the cut is decided exactly. (Where top_p is
+    that share, the others' mass decides, which is above 0 and less than a step of
+    64 bits: one entry more by the definition, none more by its sums in 64 bits.)"""
+    for count, kept in ((2, 1), (4, 2), (8, 2), (8, 4)):
+        x = torch.full((1, n), low)
+        x[:, ::3] -= 1.0
+        x[:, [17 + i * (n // count) + 5 * i for i in range(count)]] = top
+        x = x.cuda().repeat(B, 1)
+        share = np.float32(kept / count)
+        for p in (np.nextafter(share, np.float32(1)), share, np.nextafter(share, np.float32(0))):
+            for u in (0.2, 0.99):
+                uu = torch.full((B,), u, dtype=torch.float64, device="cuda")
+                if p != share:
+                    check(x, uu, T=T, p=float(p), alike=True)
+                    continue
+                got, prob = sample_logits(x, uu, T, top_p=float(p), return_prob=True)
+                some = [c for c in (kept, kept + 1) if abs(float(prob[0]) * c - 1) < 1e-6]
+                assert some and (prob == prob[0]).all()
+                assert (got == x[0].topk(count).indices.sort().values[int(u * some[0])]).all()
+
+
+@pytest.mark.parametrize("B,n", [(1, 151936), (40, 151936), (300, 151936)])
+@pytest.mark.parametrize("T,low,top", [
+    (0.1, 1.6745601, 9.715551), (0.1, 1.1, 9.6), (0.07, -3.1, 2.4), (0.2, 0.3, 17.1),
+    (1.0, 0.7, 83.1), (0.9, -20.3, 30.2), (0.1, 1.6745601, 5.1), (0.05, 2.3, 4.7)])
+def test_top_p_above_what_a_sample_shows(B, n, T, low, top):
+    """The few logits that hold the mass lie between the vectors that the kernel
+    samples for its reference, up to 127 binary orders above it."""
+    g = torch.Generator().manual_seed(2)
+    base = low - 0.5 * torch.rand(1, n, generator=g)
+    base[0, 0] = low
+    for count, kept in ((2, 1), (4, 2), (8, 2), (8, 4)):
+        x = base.clone()
+        x[:, [17 + i * (n // count) + 5 * i for i in range(count)]] = top
+        x = x.cuda().repeat(B, 1)
+        share = np.float32(kept / count)
+        for p in (np.nextafter(share, np.float32(1)), np.nextafter(share, np.float32(0))):
+            for u in (0.2, 0.99):
+                uu = torch.full((B,), u, dtype=torch.float64, device="cuda")
+                check(x, uu, T=T, p=float(p), alike=True)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("B,n", [(2, 128256), (300, 40000)])
 @pytest.mark.parametrize("T,level", [(1.0, -30.0), (1.0, -80.0), (0.1, -90.0), (1.0, -2000.0)])
