@@ -115,14 +115,31 @@ def _step_min_p(md, n: int):
     return None
 
 
+def _filtered_rows(rows, filters, vocab):
+    """Which of ``rows`` (a CPU index tensor) a filter of the step is on for: vLLM
+    fills a step's tensors for every request once one has a filter, with values
+    that keep everything (top_k = vocabulary, top_p = 1, min_p = 0) for the rest."""
+    on = torch.zeros(rows.numel(), dtype=torch.bool)
+    for name, v in filters.items():
+        if v is None:
+            continue
+        v = v.detach().reshape(-1).cpu().index_select(0, rows)
+        if name == "top_k":
+            on |= (v > 0) if vocab is None else (v > 0) & (v < vocab)
+        else:
+            on |= (v < 1) if name == "top_p" else (v > 0)
+    return on
+
+
 def step_sampled_ids(greedy_ids: torch.Tensor, sampling_metadata):
     """The last FlashHead step's ids with each non-greedy request sampled at its
     own settings; greedy rows keep greedy_ids. Where the reference hook decodes
     every request greedily (patches/logits_processor.py:38), this routes vLLM's
-    per-request settings to the sampling kernels: with top-k, top-p or min-p in
-    the step, all its random rows in one call over the step's candidates
-    (FlashHead.get_next_token_filtered); with temperatures alone, one call per
-    distinct temperature (FlashHead.get_next_token_batched(do_sample=True))."""
+    per-request settings to the sampling kernels: the rows with a top-k, top-p or
+    min-p of their own in one call over the step's candidates
+    (FlashHead.get_next_token_filtered); those with a temperature alone in one call
+    per distinct temperature (FlashHead.get_next_token_batched(do_sample=True)),
+    whatever the others' settings are."""
     md = sampling_metadata
     if md is None or getattr(md, "all_greedy", True) or getattr(md, "temperature", None) is None:
         return greedy_ids
@@ -136,16 +153,18 @@ def step_sampled_ids(greedy_ids: torch.Tensor, sampling_metadata):
     random_rows = torch.nonzero(temps >= _SAMPLING_EPS).view(-1)
     filters = {"top_k": getattr(md, "top_k", None), "top_p": getattr(md, "top_p", None),
                "min_p": _step_min_p(md, n)}
-    if any(f is not None for f in filters.values()) and random_rows.numel():
-        idx = random_rows.to(h.device)
+    shape = getattr(fh, "original_shape", None)
+    on = _filtered_rows(random_rows, filters, None if shape is None else shape[0])
+    rows, random_rows = random_rows[on], random_rows[~on]
+    if rows.numel():
+        idx = rows.to(h.device)
         per_row = {k: None if f is None else f.reshape(-1)[:n].to(h.device).index_select(0, idx)
                    for k, f in filters.items()}
         ids = fh.get_next_token_filtered(
             h.index_select(0, idx),
-            _row_uniforms(random_rows.tolist(), getattr(md, "generators", None), h.device),
-            temperature=temps[random_rows].to(h.device), **per_row)
+            _row_uniforms(rows.tolist(), getattr(md, "generators", None), h.device),
+            temperature=temps[rows].to(h.device), **per_row)
         out.view(-1).index_copy_(0, idx.to(out.device), ids.to(out.dtype).view(-1))
-        return out
     for t in torch.unique(temps[random_rows]).tolist():
         rows = random_rows[temps[random_rows] == t]
         idx = rows.to(h.device)
