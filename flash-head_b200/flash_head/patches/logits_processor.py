@@ -105,13 +105,27 @@ def _row_uniforms(rows, generators, device):
     return u.to(device)
 
 
+_warned = set()
+
+
+def _warn_once(key, msg):
+    if key not in _warned:
+        _warned.add(key)
+        logger.warning(msg)
+
+
 def _step_min_p(md, n: int):
-    """vLLM keeps min-p in a logits processor of the step; [n] or None."""
+    """vLLM keeps min-p in a logits processor of the step; [n] or None. Rows behind
+    the end of its tensor have none."""
     for proc in getattr(getattr(md, "logitsprocs", None), "argmax_invariant", None) or ():
         v = getattr(proc, "min_p", None)
         if isinstance(v, torch.Tensor) and getattr(proc, "min_p_count", 0):
             v = v.reshape(-1)
-            return v[:n] if v.numel() >= n else None
+            if v.numel() < n:
+                _warn_once("min_p", f"[FlashHead] min-p of {v.numel()} requests for {n} rows: "
+                                    "the rows behind them are sampled without one")
+                v = torch.cat([v, v.new_zeros(n - v.numel())])
+            return v[:n]
     return None
 
 

@@ -3,6 +3,8 @@ its neighbours in the step have set (CPU, a fake head)."""
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -68,3 +70,19 @@ def test_values_that_keep_everything_are_no_filter(step):
     lp.step_sampled_ids(greedy, metadata(top_k=torch.tensor([1000, 0, -1, 5000]),
                                          top_p=torch.ones(4)))
     assert not head.filtered and len(head.plain) == 3
+
+
+def test_a_min_p_shorter_than_the_step_is_kept_for_its_rows(step, caplog):
+    """It used to be dropped for every row, without a word."""
+    head, greedy = step
+    lp._warned.clear()
+    proc = SimpleNamespace(min_p=torch.tensor([[0.1], [0.2]]), min_p_count=2)
+    with caplog.at_level("WARNING"):
+        for _ in range(2):
+            lp.step_sampled_ids(greedy, metadata(
+                logitsprocs=SimpleNamespace(argmax_invariant=[proc])))
+    hs, _, _, k, p, m = head.filtered[0]
+    assert hs[:, 0].tolist() == [1.0] and k is None and p is None
+    assert torch.allclose(m, torch.tensor([0.2]))
+    assert [c[0] for c in head.plain[:2]] == [[3.0], [2.0]]  # rows 3 and 2, by temperature
+    assert sum("min-p" in r.getMessage() for r in caplog.records) == 1
