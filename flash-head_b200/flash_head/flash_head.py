@@ -251,18 +251,24 @@ class FlashHead(nn.Module):
 
     def candidate_logits(self, hidden: torch.Tensor, probes: Optional[torch.Tensor] = None):
         """(logits [N, C], ids [N, C] int32) of a step's candidates: the tokens
-        of each row's probed clusters (``probes`` [N, p] int64; default: the
+        of each row's probed clusters (``probes`` [N, p] integers; default: the
         greedy stage 1), then the special tokens, -inf where a probed cluster
-        holds them already. Logits are in the head's dtype, from the 4-bit
-        weight after ``quantize_head``."""
+        holds them already. A probe that names no cluster, or one that an earlier
+        probe of its row names, gives -inf. Logits are in the head's dtype, from
+        the 4-bit weight after ``quantize_head``."""
         from .fused import block_sparse_logits
         from .w4 import w4_block_sparse_logits
         nh = self.native()
         h = nh._h(hidden)
         N, cap, K = h.shape[0], self._cap, self._K
-        if probes is None:
+        given = probes is not None
+        if not given:
             probes = nh.top_clusters(h)
-        probes = probes.to(torch.int64)
+        elif probes.dim() != 2 or probes.shape[0] != N or probes.is_floating_point():
+            raise ValueError(f"probes must be integers [{N}, p], got {tuple(probes.shape)} "
+                             f"{probes.dtype}")
+        probes = probes.to(device=h.device, dtype=torch.int64)
+        P = probes.shape[1]
         w4 = self.quantized()
 
         def product(ci, n, size):
@@ -270,8 +276,15 @@ class FlashHead(nn.Module):
                 return w4_block_sparse_logits(h, w4, ci, n, size)
             return block_sparse_logits(h, self.w_perm.view(-1), ci, n, size)
         logits = product(probes, K, cap)
+        at = probes
+        if given:
+            gone = (probes < 0) | (probes >= K)
+            gone |= (probes.unsqueeze(2) == probes.unsqueeze(1)).tril(-1).any(dim=2)
+            logits = logits.view(N, P, cap).masked_fill(gone.unsqueeze(2), float("-inf"))
+            logits = logits.view(N, P * cap)
+            at = probes.clamp(0, K - 1)
         vocab = nh.bufs["vocab_map"]
-        ids = vocab.view(K, cap).index_select(0, probes.view(-1)).view(N, -1)
+        ids = vocab.view(K, cap).index_select(0, at.reshape(-1)).view(N, P * cap)
         slots = nh.bufs["special_slots"]
         if slots is not None:
             at = slots.to(torch.int64).unsqueeze(0).expand(N, -1)
