@@ -135,6 +135,7 @@ class FlashHead(nn.Module):
 
         st = [int(t) for t in ([special_token_ids] if isinstance(special_token_ids, int)
                                else list(special_token_ids or [])) if 0 <= int(t) < V]
+        st = list(dict.fromkeys(st))  # one given twice would count twice in a draw
         if st:
             sp = torch.tensor(st, dtype=torch.int64, device=vocab_maps_tensor.device)
             found = (vocab_maps_tensor.reshape(-1).to(torch.int64).unsqueeze(0)

@@ -91,3 +91,10 @@ def test_no_rows(head):
     assert logits.shape == ids.shape == (0, P * CAP + 2)
     logits, ids = head.candidate_logits(rows(0), torch.zeros(0, 2, dtype=torch.int64))
     assert logits.shape == ids.shape == (0, 2 * CAP + 2)
+
+
+def test_a_special_token_given_twice_is_one_candidate():
+    lm = nn.Linear(D, K * CAP, bias=False).to(torch.bfloat16)
+    fh = FlashHead(lm, torch.randn(D, K), torch.arange(K * CAP).view(K, CAP), n_probes=P,
+                   special_token_ids=[7, 21, 7, 21, 3])
+    assert fh.special_token_ids_tensor.tolist() == [7, 21, 3]
