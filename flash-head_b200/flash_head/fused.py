@@ -27,6 +27,9 @@ from . import _lib
 def _check(hs: torch.Tensor, ci: torch.Tensor, w_perm_flat: torch.Tensor):
     assert hs.dim() == 2 and hs.is_contiguous()
     assert ci.dim() == 2 and ci.dtype == torch.int64
+    if ci.shape[0] != hs.shape[0] or ci.device != hs.device:
+        raise ValueError(f"ci {tuple(ci.shape)} on {ci.device} does not fit hidden states "
+                         f"{tuple(hs.shape)} on {hs.device}")
     if not hs.is_cuda:
         raise RuntimeError("FlashHead kernels need CUDA tensors (there is no CPU path)")
     if w_perm_flat.dtype != hs.dtype:

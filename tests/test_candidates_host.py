@@ -98,3 +98,14 @@ def test_a_special_token_given_twice_is_one_candidate():
     fh = FlashHead(lm, torch.randn(D, K), torch.arange(K * CAP).view(K, CAP), n_probes=P,
                    special_token_ids=[7, 21, 7, 21, 3])
     assert fh.special_token_ids_tensor.tolist() == [7, 21, 3]
+
+
+def test_block_sparse_probes_of_other_rows_are_refused():
+    """(Their rows would be read past the end.)"""
+    h, w = torch.zeros(3, D), torch.zeros(K * CAP * D)
+    ci = torch.zeros(2, P, dtype=torch.int64)
+    for call in (lambda: fused.block_sparse_logits(h, w, ci, K, CAP),
+                 lambda: fused.block_sparse_logits_argmax(h, w, ci, torch.zeros(K * CAP), K, CAP),
+                 lambda: fused.block_sparse_argmax_atomic(h, w, ci, torch.zeros(K * CAP), K, CAP)):
+        with pytest.raises(ValueError, match="does not fit"):
+            call()
