@@ -68,7 +68,9 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor,
     uniforms: [B] numbers in [0, 1), float64 (float32 is converted).
     temperature, top_k, top_p, min_p: a number, or [B] values on the logits'
         device; temperature 0 is greedy, top_k 0, top_p 1 and min_p 0 (or None)
-        switch a filter off.
+        switch a filter off. Values outside [0, inf], [0, 2^31), [0, 1] and [0, 1] are
+        refused as numbers; in a tensor (not read on the host) those below or above
+        switch the filter off, or are greedy, as at the ends.
     ids: int32 [n] or [B, n], the id of every column (default: the column).
     out: [B] int64 for the ids.
     return_prob: also return [B] float32, the drawn entry's share of the kept
@@ -101,6 +103,8 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor,
         kt = _per_row("top_k", top_k, B, _I32, dev)
     elif top_k is not None:
         k = int(_number("top_k", top_k, 0, 2 ** 31 - 1))
+        if k != top_k:
+            raise ValueError(f"top_k must be an integer, got {top_k}")
     if isinstance(top_p, torch.Tensor):
         pt = _per_row("top_p", top_p, B, _F32, dev)
     elif top_p is not None:
