@@ -144,8 +144,8 @@ class W4Weight:
 
         Without zero points a group's scale is its largest magnitude / 7; with
         them the group's range (0 included) is spread over 0..15. Scales are
-        held in the weight's dtype, and weights are rounded against the held
-        scale."""
+        held in the weight's dtype, at least its smallest normal number, and
+        weights are rounded against the held scale. The weight has to be finite."""
         if weight.dim() != 2 or weight.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"weight must be a 2-D bf16 or fp16 tensor, got "
                              f"{tuple(weight.shape)} {weight.dtype}")
@@ -165,6 +165,9 @@ class W4Weight:
                 else:
                     s = (x.abs().amax(dim=2) / 7.0).clamp_min(tiny).to(weight.dtype)
                     z = torch.full_like(s, 8.0, dtype=torch.float32)
+                if not bool(torch.isfinite(s).all()):
+                    raise ValueError("the weight holds numbers that are not finite, or a group "
+                                     "whose range is not")
                 q = (x / s.float().unsqueeze(2)).round_() + z.unsqueeze(2)
                 q = q.clamp_(0, 15).to(torch.uint8).view(-1, D)
                 qs.append(q[:, 0::2] | (q[:, 1::2] << 4))

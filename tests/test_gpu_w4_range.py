@@ -113,3 +113,17 @@ def test_smallest_and_largest_scales(T, top):
     h = (hidden(T, D, torch.float32, T) * (2.0 ** 60 if top < 1 else 2.0 ** -100))
     h = h.to(torch.bfloat16).cuda()
     check(w4_logits(h, w), h, W, group)
+
+
+@pytest.mark.parametrize("T", [8, 9, 70])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype,top,small", [
+    (torch.float16, 60000.0, 2.0 ** -12), (torch.bfloat16, 2.0 ** 126, 2.0 ** -126)])
+def test_weights_beyond_the_largest_number(dtype, top, small, group, T):
+    """15 times the scale is no number of the type; the logits are."""
+    V, D = 200, 256
+    s = torch.full((V, D // group), top, dtype=torch.float64)
+    s[::2] = 1.0
+    w, W, group = build(*weight(V, D, group, True, dtype, 11, s))
+    h = (hidden(T, D, torch.float32, T) * small).to(dtype).cuda()
+    check(w4_logits(h, w), h, W, group)
