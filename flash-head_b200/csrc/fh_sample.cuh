@@ -17,8 +17,8 @@
 //
 // A row is read by a cluster of 1..8 CTAs; warp w of the cluster owns the
 // w-th contiguous segment of the row. Passes over the row:
-//   1  its largest logit. Without a filter, the masses too. A row that does not
-//      fit in shared memory also yields its candidates, the entries above a
+//   1  its largest logit. Without a filter, the masses too. A row that is not kept
+//      in shared memory also yields its candidates, the entries above a
 //      threshold that a sample of the row gives, and under a top-p its mass in
 //      fp32, whose error is bounded;
 //   2  the candidates (at most 2048, in column order) are joined, sorted in
@@ -51,9 +51,9 @@ namespace fh {
 
 constexpr int kSmpThreads = 256;
 // CTAs per SM, of 64 registers a thread (rows in shared memory: half as many).
-// Two of 128 registers are better for fp64 chains alone (256 unfiltered rows: 60
-// us against 66), four for everything with candidates (64 rows of mixed filters:
-// 91 us against 77; 256 fp32 rows with top-p: 281 against 245).
+// Two of 128 registers are better for fp64 chains alone (256 unfiltered rows: 63
+// us against 70), four for everything with candidates (256 rows with top-k 50 and
+// top-p: 98 us against 74; 256 fp32 rows with top-p: 233 against 197).
 constexpr int kSmpResident = 4;
 constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBands = 16;
@@ -63,7 +63,9 @@ constexpr int kSmpChunk = 2048;  // vectors of the segment of the draw looked at
 constexpr int kSmpList = 2048;   // candidates one CTA sorts
 constexpr int kSmpPart = 512;    // candidates of one warp
 constexpr int kSmpMaxK = 1024;   // largest top-k that goes through the list
-constexpr int kSmpCache = 8;     // vectors of a row that a thread keeps (CACHED)
+// Vectors of a row that a thread keeps at most (CACHED): what two CTAs of an SM have
+// room for.
+constexpr int kSmpCache = 14;
 
 struct SampleArgs {
   const void *logits;
@@ -81,6 +83,7 @@ struct SampleArgs {
   long long ids_stride;
   int64_t *out;
   float *prob;  // or null
+  int cache;    // vectors that a thread keeps (CACHED)
 };
 
 struct __align__(16) SmpShared {
@@ -270,7 +273,8 @@ struct SmpSpan {
   SmpRow<E> row;
   int v0, v1;
   int lane;
-  uint4 *cache;  // this thread's share of the row in shared memory (CACHED)
+  uint4 *cache;  // this thread's share of the row in shared memory (CACHED),
+  int keep;      // of so many vectors
 
   // f(vector, kVec values), a lane every 32 vectors, by whole warps: lanes past
   // the segment get -inf. FIRST: the row is read for the first time; a CACHED
@@ -281,10 +285,14 @@ struct SmpSpan {
     float x[kVec];
     if constexpr (CACHED) {
       if (FIRST) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < keep; i0 += 4) {
 #pragma unroll
-        for (int i = 0; i < kSmpCache; ++i) {
-          const int v = v0 + lane + 32 * i;
-          cache[kSmpThreads * i] = v < v1 ? row.raw(v) : make_uint4(no, no, no, no);
+          for (int i = i0; i < i0 + 4; ++i) {
+            const int v = v0 + lane + 32 * i;
+            if (i < keep)
+              cache[kSmpThreads * i] = v < v1 ? row.raw(v) : make_uint4(no, no, no, no);
+          }
         }
       }
 #pragma unroll 1
@@ -1408,7 +1416,7 @@ __device__ __forceinline__ SmpDeep smp_deep(Ctx &C, const SampleArgs &a, const S
   return kCut;
 }
 
-// CACHED: every lane's share of the row is at most kSmpCache vectors, kept in
+// CACHED: every lane's share of the row is at most a.cache vectors, kept in
 // shared memory.
 template <typename E, bool CACHED>
 __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpResident) k_sample(SampleArgs a) {
@@ -1422,7 +1430,7 @@ __global__ void __launch_bounds__(kSmpThreads, CACHED ? kSmpResident / 2 : kSmpR
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   SmpCtx<E, CACHED> C{
       {SmpRow<E>(reinterpret_cast<const E *>(a.logits) + (long long)r * a.stride, a.n), 0, 0, lane,
-       reinterpret_cast<uint4 *>(smp_raw + sizeof(SmpShared)) + tid},
+       reinterpret_cast<uint4 *>(smp_raw + sizeof(SmpShared)) + tid, a.cache},
       S, rank, size, 0, tid, warp, lane};
   {
     const int gw = rank * kSmpWarps + warp, warps = size * kSmpWarps;

@@ -1647,15 +1647,17 @@ template <typename E, bool CACHED>
 static cudaError_t launch_sample_c(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
   static bool done[128];
   auto kern = fh::k_sample<E, CACHED>;
-  const size_t smem = sizeof(fh::SmpShared) +
-                      (CACHED ? sizeof(uint4) * fh::kSmpCache * fh::kSmpThreads : 0);
-  const cudaError_t e = raise_smem(kern, (int)smem, done);
+  constexpr size_t vec = sizeof(uint4) * fh::kSmpThreads;  // one vector of every thread
+  static_assert(2 * (sizeof(fh::SmpShared) + fh::kSmpCache * vec + 1024) <= 228 * 1024,
+                "two CTAs to an SM");
+  const cudaError_t e =
+      raise_smem(kern, (int)(sizeof(fh::SmpShared) + (CACHED ? fh::kSmpCache * vec : 0)), done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)rows * (unsigned)cluster);
   cfg.blockDim = dim3(fh::kSmpThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(fh::SmpShared) + (CACHED ? a.cache * vec : 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1667,13 +1669,24 @@ static cudaError_t launch_sample_c(const fh::SampleArgs &a, int rows, int cluste
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+// Rows are kept in shared memory, where they are read again and again, if a lane's
+// share fits and the grid has at most `keep` CTAs: two to an SM then, against four
+// that read their rows from L2. us, kept against not: 64 bf16 rows of 151936 with
+// mixed filters 57 / 90, 90 of them 80 / 96, 120 104 / 106; with top-p 64 rows 90 /
+// 112, 90 120 / 131, 120 158 / 145; with top-k and top-p, which need one more pass
+// at most, 64 41 / 38, 90 60 / 50; one row 17.4 / 21.7; without a filter 4 rows of
+// 128256 12.6 / 15.2, 24 16.2 / 17.9, 37 (two CTAs to every SM) 25.7 / 22.0.
 template <typename E>
-static cudaError_t launch_sample_t(const fh::SampleArgs &a, int rows, int cluster, cudaStream_t s) {
+static cudaError_t launch_sample_t(fh::SampleArgs a, int rows, int cluster, long long keep,
+                                   cudaStream_t s) {
   // vectors of a row (at most one more than its length: it may start inside one)
   const long long nv = ((long long)a.n + 2 * fh::SmpElem<E>::kVec - 2) / fh::SmpElem<E>::kVec;
   const long long per_warp = (nv + cluster * fh::kSmpWarps - 1) / (cluster * fh::kSmpWarps);
-  return per_warp <= 32 * fh::kSmpCache ? launch_sample_c<E, true>(a, rows, cluster, s)
-                                        : launch_sample_c<E, false>(a, rows, cluster, s);
+  const long long per_lane = (per_warp + 31) / 32;
+  a.cache = (int)std::min<long long>(per_lane, fh::kSmpCache);
+  return per_lane <= fh::kSmpCache && (long long)rows * cluster <= keep
+             ? launch_sample_c<E, true>(a, rows, cluster, s)
+             : launch_sample_c<E, false>(a, rows, cluster, s);
 }
 
 extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, int n,
@@ -1718,8 +1731,10 @@ extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, 
   // for others, which shorter CTAs in two waves even out: 8 (256 fp32 rows of
   // 151936, top-p 0.9 at temperature 0.8: 207 us, with 4 per SM 223, with 16
   // 257). Rows that the first candidates settle run in one wave: 4 (256 bf16 rows
-  // of 128256, top-k 50: 52 us, with 8 per SM 68). 2 where no row has a filter
-  // and all are alike (the same rows: 66 us, with 8 per SM 72).
+  // of 128256, top-k 50: 52 us, with 8 per SM 68); a top-k in an array is not seen
+  // here, and such a launch takes the rule of a top-p (74 us with one of 0.95 too).
+  // 2 where no row has a filter and all are alike (the same rows: 66 us, with 8 per
+  // SM 72).
   const bool some_p = params->top_p || params->top_p_all < 1.f;
   const bool plain = !params->top_k && !some_p && !params->min_p && params->top_k_all <= 0 &&
                      !(params->min_p_all > 0.f);
@@ -1731,9 +1746,10 @@ extern "C" FH_API int fh_sample_logits(const void *logits, int dtype, int rows, 
          n / (cluster * 2) >= 4096)
     cluster *= 2;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == FH_BF16   ? launch_sample_t<__nv_bfloat16>(a, rows, cluster, s)
-                        : dtype == FH_FP16 ? launch_sample_t<__half>(a, rows, cluster, s)
-                                           : launch_sample_t<float>(a, rows, cluster, s);
+  const long long keep = plain ? 2ll * sms - 1 : 5ll * sms;
+  const cudaError_t e = dtype == FH_BF16   ? launch_sample_t<__nv_bfloat16>(a, rows, cluster, keep, s)
+                        : dtype == FH_FP16 ? launch_sample_t<__half>(a, rows, cluster, keep, s)
+                                           : launch_sample_t<float>(a, rows, cluster, keep, s);
   FH_CHECK_LAUNCH(e, "sampling launch");
   return FH_OK;
 }
