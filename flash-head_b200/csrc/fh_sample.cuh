@@ -37,9 +37,9 @@
 // rows of 128256 entries against 10 us of reading. Filtered rows are bound by
 // latency: a chain of passes, exchanges, a sort and scans, which the rows of
 // other clusters cover in part. Measured, bf16 rows of 128256 unless said
-// otherwise: one row with top-k and top-p 17.4 us; 64 rows of mixed filters 54
-// us; 256 rows without a filter 66 us (1.0 TB/s), with top-k 50 52 us (1.3
-// TB/s); 256 fp32 rows of 151936 with top-p 208 us, 114 us where the cut lies
+// otherwise: one row with top-k and top-p 16.4 us; 64 rows of mixed filters 55
+// us; 256 rows without a filter 70 us (0.9 TB/s), with top-k 50 52 us (1.3
+// TB/s); 256 fp32 rows of 151936 with top-p 197 us, 114 us where the cut lies
 // among the first candidates.
 #pragma once
 

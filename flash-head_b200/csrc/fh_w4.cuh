@@ -272,9 +272,11 @@ __host__ __device__ inline size_t w4_mv_smem_bytes(int nb) {
 // warps; a unit is 32 weight rows, taken by ksplit warps (each every
 // ksplit-th block of 128 columns). Units go to CTAs round-robin, so every SM
 // reads the same share of the weight.
-// Bound: turning nibbles into operands, about 5 integer instructions a word
-// against 1/2 mma, next to HBM: one row of a 2048 x 128256 head, groups of 128
-// in bf16 and no zero points, 35 us (3.8 TB/s), 8 rows of 4096 x 128256 69 us.
+// Bound: no unit is full. Turning nibbles into operands, 9 to 11 instructions a word
+// for half an mma, keeps the ALU pipe 56 to 61 % busy, issue 51 to 58 %, DRAM 45
+// to 47 %: each of an SM's 16 warps loads, unpacks and multiplies in turn. One row of
+// a 2048 x 128256 head, groups of 128 in bf16 and no zero points, 35 us (3.8
+// TB/s), 8 rows of 4096 x 128256 69 us.
 // mma.sync, not tcgen05: its operand is made in registers, where the words
 // arrive, and a tcgen05 tile of 8 columns would wait for the same words.
 template <typename T, int GPK, bool ZP>
@@ -412,8 +414,9 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) k_w4_mv(W4Args a) {
 // Probed clusters: out[r, i * cap + s] = logit of weight row ci[r, i] * cap + s
 // for hidden row r. A CTA takes 16 candidate slots of one row and its 8 warps
 // share the columns. Cluster ids outside [0, K) give -inf.
-// Bound: latency for one row, then HBM sectors: a cluster of 16 neighbouring
-// rows is 256 bytes in each quad of a block. 256 clusters of 16, 2048 columns,
+// Bound: latency for one row, then the same pipe (60 %) and HBM sectors (29 %): a
+// cluster of 16 neighbouring rows is 256 bytes in each quad of a block, and no load
+// is issued ahead. 256 clusters of 16, 2048 columns,
 // one row 4.7 us; 4096 columns with zero points, 12 rows 40 us (2.7 TB/s of the
 // words, scales and zero points of every row's own clusters).
 constexpr int kW4ProbeWarps = 8;

@@ -227,7 +227,9 @@ class FlashHead(nn.Module):
         which use it from then on; returns the weight. Greedy and
         temperature-only steps keep the 16-bit weight. A head moved, cast or
         written to afterwards has to be quantised again: until then the 16-bit
-        weight serves (and ``head_logits`` refuses)."""
+        weight serves (and ``head_logits`` refuses). Writes that torch does not
+        count are not seen and leave the 4-bit weight as it was: those through
+        ``.data``, and those to a ``w_perm`` made in inference mode."""
         from .w4 import W4Weight
         w = W4Weight.from_dense(self.w_perm.view(-1, self._D), group_size, zeros)
         self._w4 = (self._w4_key(), w)

@@ -326,7 +326,7 @@ FH_API int fh_block_sparse_argmax_atomic(const void *hs, int T, int D,
  *
  * The entries above -inf (NaN counts as masked) of a row are ordered by
  * falling logit, then rising column; e_i = exp((x_i - max) / T), held in 64
- * bits. Every filter keeps a prefix of that order:
+ * bits (below 2^-1000: 0). Every filter keeps a prefix of that order:
  *   min_p  the entries with e_i >= min_p (the largest always; off at <= 0)
  *   top_k  the first k of them (off at <= 0)
  *   top_p  the shortest prefix that holds top_p of their mass (off at >= 1;
