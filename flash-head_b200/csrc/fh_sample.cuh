@@ -129,7 +129,8 @@ struct __align__(16) SmpShared {
   long long cut_ties;
 };
 
-// Order of the logits: monotone in x, with -0 equal to +0.
+// Order of the logits: monotone in x, with -0 equal to +0. A NaN has no key (what
+// comes out for one is some number's).
 __device__ __forceinline__ uint32_t smp_key(float x) { return mono(x + 0.0f); }
 
 // A key as a threshold that logits are compared with. No logit has the key of
@@ -203,7 +204,7 @@ struct SmpRow {
       x.e[i] = c0 + i >= 0 && c0 + i < n ? p[c0 + i] : SmpElem<E>::none();
     return x.u;
   }
-  // NaN stays: it fails every comparison (and key range) below, as -inf does
+  // NaN stays: it fails every comparison below, as -inf does
   __device__ __forceinline__ static void unpack(const uint4 &u, float *f) {
     SmpElem<E>::unpack(u, f);
   }
@@ -422,7 +423,7 @@ __device__ __forceinline__ void smp_key_bands(Ctx &C, const SmpMass &w, uint32_t
 #pragma unroll
     for (int i = 0; i < decltype(C.span)::kVec; ++i) {
       const uint32_t k = smp_key(f[i]);
-      if (k >= lo && k <= hi) {
+      if (k >= lo && k <= hi && f[i] == f[i]) {
         const int b = (int)((k - lo) >> shift);
         S.band.cnt[b][C.tid] += 1u;
         if (MASS) S.band.mass[b][C.tid] += w(f[i]);

@@ -157,3 +157,26 @@ def test_masked_beginnings_and_logits_far_below_zero(B, n, T, level, dtype):
     share = (e.cumsum(1) / e.sum(1, keepdim=True)).gather(1, got.clamp_min(0).view(B, 1))
     assert (got >= 0).all() and (share >= 1 - n * 2.0 ** -52).all()
     assert (x.gather(1, got.view(B, 1)) > float("-inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,n", [(3, 1580), (2, 4217), (5, 9000), (2, 150000)])
+def test_nan_masks_where_the_cut_descends_by_keys(B, n, dtype):
+    """A top-k beyond the list of candidates, or a cut among thousands of equal
+    logits: a NaN is not counted among the entries above it, whatever its bits."""
+    x = logits(B, n, torch.float32, 9, sigma=1.0, peak=False)
+    gone = torch.rand(B, n, generator=torch.Generator().manual_seed(5)).cuda() < 0.3
+    left = int((~gone).sum(1).min())
+    u = torch.rand(B, generator=torch.Generator().manual_seed(6), dtype=torch.float64).cuda()
+    for y in (x, x.round()):
+        y = y.to(dtype)
+        bits = y.view(torch.int16 if dtype != torch.float32 else torch.int32)
+        for negative in (True, False):
+            y[gone] = float("nan")
+            if negative:
+                bits[gone] = -1  # every bit set
+            for k in (1025, left - 1, left, left + 1, n - 1):
+                check(y, u, T=2.0, k=k)
+                check(y, u, T=2.0, k=k, p=0.9)
+            check(y, u, T=50.0, p=0.7)
+            check(y, u, T=2.0, p=0.7, m=1e-3)
