@@ -38,7 +38,7 @@
 // More than 128 rows take several launches: two more sets of accumulators would
 // not fit beside the operand, nor their sums in the registers.
 // Bound: the chain of barriers that every block passes (a wait costs some 130
-// clocks, met or not) and the issue slots (72 %): 9 rows of a 2048 x 128256 head
+// clocks, met or not) and the issue slots (73 to 75 %): 9 rows of a 2048 x 128256 head
 // 49 us, 64 of a 1536 x 151936 one 54 us (2.2 TB/s), 128 and 256 of 2048 x 128256
 // 75 and 148 us (0.9 PFLOP/s). Tried and slower: polls with a time hint, fp32x2
 // multiply-adds, half as many warps that sum 64 rows each, and twice as many that
