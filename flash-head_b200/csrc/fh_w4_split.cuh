@@ -1,10 +1,11 @@
 // Logits of a 4-bit head with scale groups of 32 or 64 columns for many rows, on
 // the 5th-generation tensor cores:
-// out[b, v] = sum_k w[v, k] h[b, k], M = 128 weight rows, N = up to 256 hidden
-// rows per launch. (Groups of 128: fh_w4_tc.cuh, which is faster for them: 64 rows
-// of a 1536 x 151936 head 54 us against 60, 256 of 2048 x 128256 148 against 176,
-// but reads accumulators back once per group: with groups of 32, 64 rows of 2048 x
-// 128256 took it 137 us against 68 here, with groups of 64 128 rows 139 against 97.)
+// out[b, v] = sum_k w[v, k] h[b, k], M = 128 weight rows, N = up to 128 hidden
+// rows per launch. (Groups of 128: fh_w4_tc.cuh, which is faster for them: with one
+// accumulator for both parts, 64 rows of a 1536 x 151936 head 54 us against 60, 256
+// of 2048 x 128256 148 against 176, but reads accumulators back once per group:
+// with groups of 32, 64 rows of 2048 x 128256 took it 137 us against 72 here, with
+// groups of 64 128 rows 139 against 105.)
 //
 // A weight (q - z) s is the product of an integer of up to 4 bits and a scale of 8
 // (bf16) or 11 (fp16): it has up to 15 bits, more than the hidden states' 16-bit
@@ -12,8 +13,10 @@
 // rounded, and lo, what was rounded off, which one fused multiply-add gives. Both
 // are operands, so that no weight and no hidden state is rounded, however far
 // apart scales or hidden states lie, and logits differ from k_w4_mv's only in the
-// order of their fp32 sums. (A hidden row that holds an infinity is the exception:
-// lo is zero for many weights, and the row's logits are NaN instead of infinite.)
+// order of their fp32 sums. Each part has an accumulator of its own: the tensor
+// core truncates its fp32 sum at every step, of which one accumulator would see
+// twice as many, and an infinite hidden state times a lo of 0 would make NaN of an
+// infinite logit.
 // 15 s may pass the type's largest number: rows with a scale above 2^12 (fp16) or
 // 2^124 (bf16) are brought down by 2^-4 (row_mul), undone in the epilogue.
 //
@@ -32,10 +35,10 @@
 //               and stores 32 columns' pairs, hi and lo (16 TMEM columns each) at a
 //               time;
 //   warps 16-19 epilogue: a thread has one weight row and all hidden rows; up to
-//               128 hidden rows the accumulators are double-buffered.
-// Bound: the issue of the MMAs, some 46 clocks each whatever N is up to 128 (twice
-// the warps that unpack changed nothing), their rate beyond. 2048 x 128256, zero
-// points: 16 rows 62 us, 64 68 us, 256 183 us.
+//               32 hidden rows the accumulators are double-buffered.
+// Bound: the issue of the MMAs, some 46 clocks each whatever N is (twice the warps
+// that unpack changed nothing). 2048 x 128256, zero points: 16 rows 62 us, 64
+// 72 us, 128 105 us, 256 217 us in two launches (183 in one, with one accumulator).
 // Every wait is bounded; on a timeout the CTA drains its own copies and MMAs
 // (bounded), frees TMEM, fills the logits of its tiles with NaN and records
 // kErrCopyTimeout.
@@ -51,7 +54,7 @@ constexpr int kW4sEpiWarps = 4;
 constexpr int kW4sFirstConv = 4;  // warp
 constexpr int kW4sEpi = kW4sFirstConv + kW4sGroups * kW4sConvWarps;
 constexpr int kW4sThreads = 32 * (kW4sFirstConv + kW4sGroups * kW4sConvWarps + kW4sEpiWarps);
-constexpr int kW4sMaxN = 256;
+constexpr int kW4sMaxN = 128;
 constexpr int kW4sMaxStages = 3;
 constexpr int kW4sACols = 128;  // TMEM columns of a stage's A tiles: 128 numbers per row, hi and lo
 constexpr int kW4sMaxPacked = 12;
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, S.tmem_base, 0);
-  const uint32_t a_col = (uint32_t)(a.n_acc * a.n_pad);  // first column of the A tiles
+  const uint32_t a_col = (uint32_t)(2 * a.n_acc * a.n_pad);  // first column of the A tiles
 
   if (warp == 0) {
     if (lane == 0) {
@@ -259,7 +262,8 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
       const int buf = i % a.n_acc, use = i / a.n_acc;
       if (use > 0)
         ok = w4t_wait_all(smem_u32(&S.acc_empty[buf]), (uint32_t)((use - 1) & 1), a.polls);
-      const uint32_t acc = tmem + (uint32_t)(buf * a.n_pad);
+      const uint32_t acc = tmem + (uint32_t)(2 * buf * a.n_pad);
+      const uint32_t acc_lo = acc + (uint32_t)a.n_pad;
       for (int kb = 0; kb < a.nb && ok; ++kb) {
         ok = w4t_wait_all(full0 + 8u * s, ph, a.polls);
         if (!ok) break;
@@ -272,13 +276,13 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
             for (int q = 0; q < 8; ++q) {
               const uint64_t b = bd + (q >> 2) * half + 2u * (q & 3);
               w4t_mma(acc, at + 8u * q, b, idesc, q > 0 ? 1u : (uint32_t)kb);
-              w4t_mma(acc, at + 64u + 8u * q, b, idesc, 1u);
+              w4t_mma(acc_lo, at + 64u + 8u * q, b, idesc, q > 0 ? 1u : (uint32_t)kb);
             }
           } else {
             for (int q = 0; 128 * kb + 16 * q < a.D; ++q) {
               const uint64_t b = bd + (q >> 2) * half + 2u * (q & 3);
               w4t_mma(acc, at + 8u * q, b, idesc, (uint32_t)(kb | q));
-              w4t_mma(acc, at + 64u + 8u * q, b, idesc, 1u);
+              w4t_mma(acc_lo, at + 64u + 8u * q, b, idesc, (uint32_t)(kb | q));
             }
           }
           w4t_commit(empty0 + 8u * s);
@@ -383,17 +387,25 @@ __global__ void __launch_bounds__(kW4sThreads, 1)
       const float back = 1.f / __ldg(a.row_mul + v);  // a power of two
       T *out = reinterpret_cast<T *>(a.out);
       T *stage = reinterpret_cast<T *>(S.out[warp - kW4sEpi]);
-      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * a.n_pad);
+      const uint32_t base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(2 * buf * a.n_pad);
       for (int c = 0; c < a.n_pad; c += 32) {
-        uint32_t x[2][16];
-        tc_ld16(base + (uint32_t)c, x[0]);
-        if (c + 16 < a.n_pad) tc_ld16(base + (uint32_t)(c + 16), x[1]);
-        tc_wait_ld();
         // through shared memory: 16-byte stores instead of 2-byte ones
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          stage[32 * j + lane] = from_float<T>(__uint_as_float(x[j >> 4][j & 15]) * back);
+        for (int half = 0; half < 32; half += 16) {
+          if (c + half >= a.n_pad) break;
+          uint32_t hi[16], lo[16];
+          tc_ld16(base + (uint32_t)(c + half), hi);
+          tc_ld16(base + (uint32_t)(a.n_pad + c + half), lo);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            // (an infinite hidden state times a lo of 0 is NaN: hi says what it is)
+            float x = __uint_as_float(hi[j]);
+            if (fabsf(x) < INFINITY) x += __uint_as_float(lo[j]);
+            stage[32 * (half + j) + lane] = from_float<T>(x * back);
+          }
+        }
         __syncwarp();
         if (a.vec) {
 #pragma unroll

@@ -1880,6 +1880,12 @@ static Args w4_many_args(const fh_w4_desc *desc, int64_t out_stride, void *works
   return a;
 }
 
+// Launches of at most `most` rows (a multiple of 16), of about the same number each.
+static int w4_rows_per_launch(int rows, int most) {
+  const int launches = (rows + most - 1) / most;
+  return ((rows + launches - 1) / launches + 15) / 16 * 16;
+}
+
 // Rows r0 .. r0 + n of a call: the launch's outputs and its tensor map.
 template <typename Args>
 static bool w4_many_rows(const fh_w4_desc *desc, const void *hidden, int r0, int n, void *out,
@@ -1940,9 +1946,7 @@ static int run_w4_tc(const fh_w4_desc *desc, const void *hidden, int rows, void 
                      int64_t out_stride, void *workspace, int sms, cudaStream_t s) {
   const bool zp = desc->zeros != nullptr;
   fh::W4TcArgs a = w4_many_args<fh::W4TcArgs>(desc, out_stride, workspace);
-  // launches of about the same number of rows
-  const int launches = (rows + fh::kW4tMaxN - 1) / fh::kW4tMaxN;
-  const int per = ((rows + launches - 1) / launches + 15) / 16 * 16;
+  const int per = w4_rows_per_launch(rows, fh::kW4tMaxN);
   for (int r0 = 0; r0 < rows; r0 += per) {
     CUtensorMap tm;
     if (!w4_many_rows(desc, hidden, r0, std::min(per, rows - r0), out, a, &tm))
@@ -1980,16 +1984,19 @@ static int run_w4_split(const fh_w4_desc *desc, const void *hidden, int rows, vo
   const bool zp = desc->zeros != nullptr;
   fh::W4SplitArgs a = w4_many_args<fh::W4SplitArgs>(desc, out_stride, workspace);
   a.row_mul = desc->row_mul;
-  for (int r0 = 0; r0 < rows; r0 += fh::kW4sMaxN) {
+  const int per = w4_rows_per_launch(rows, fh::kW4sMaxN);
+  for (int r0 = 0; r0 < rows; r0 += per) {
     CUtensorMap tm;
-    if (!w4_many_rows(desc, hidden, r0, std::min(fh::kW4sMaxN, rows - r0), out, a, &tm))
+    if (!w4_many_rows(desc, hidden, r0, std::min(per, rows - r0), out, a, &tm))
       return fail(FH_ERR_UNSUPPORTED, "hidden-state tensor map");
-    // stages of 128 columns; the rest of shared memory is the packed ring.
-    // Accumulators and A tiles share the 512 TMEM columns.
+    // stages of 128 columns; the rest of shared memory is the packed ring. The parts'
+    // accumulators and A tiles share the 512 TMEM columns: a third stage is worth
+    // more than accumulators for the next tile (64 rows of 2048 x 128256 71.5 us
+    // against 72.2, 48 rows 63 against 66).
     a.stages = a.n_pad <= 64 ? 3 : 2;
-    a.n_acc = a.n_pad <= 128 ? 2 : 1;
+    a.n_acc = a.n_pad <= 32 ? 2 : 1;
     a.tmem_cols = 32;
-    while (a.tmem_cols < a.n_acc * a.n_pad + a.stages * fh::kW4sACols) a.tmem_cols *= 2;
+    while (a.tmem_cols < 2 * a.n_acc * a.n_pad + a.stages * fh::kW4sACols) a.tmem_cols *= 2;
     const size_t used = fh::w4s_smem_bytes(a.n_pad, a.stages, 0, gpk, zp);
     a.packed = (int)std::min<size_t>(fh::kW4sMaxPacked, ((size_t)fh::kW4SmemMax - used) /
                                                             fh::w4_packed_bytes(gpk, zp));

@@ -5,7 +5,7 @@ Tolerance. The products (q - z) * h are exact; a group's fp32 sum and the groups
 scaled sums are at most group / 16 + G + 16 additions, each off by 2^-22 of
 A = sum |w| |h| at worst. Calls of more than 8 rows with groups below 128 sum the
 exact products of a weight's two parts instead, 16 columns at a time: D / 8
-additions. Then one rounding to the output type, half a step. Nothing is rounded
+additions (of which an accumulator sees half). Then one rounding to the output type, half a step. Nothing is rounded
 to 16 bits before that.
 """
 
@@ -37,13 +37,14 @@ def build(v, s, z):
     return w, (x * s.double().unsqueeze(2)).view(v.shape).cuda(), group
 
 
-def check(got, h, W, group):
+def check(got, h, W, group, rows=None):
+    """rows: of the call, when h holds some of them."""
     hd = h.double()
     want, mag = hd @ W.t(), hd.abs() @ W.abs().t()
     info = torch.finfo(h.dtype)
     # below the smallest normal number a step no longer shrinks with the value
     D = h.shape[1]
-    adds = D / 8 if h.shape[0] > 8 and group < 128 else group / 16 + D / group + 16
+    adds = D / 8 if (rows or h.shape[0]) > 8 and group < 128 else group / 16 + D / group + 16
     tol = info.eps / 2 * want.abs().clamp_min(info.tiny) + adds * 2.0 ** -22 * mag
     err = (got.double() - want).abs()
     bad = ~(err <= tol)
@@ -127,3 +128,25 @@ def test_weights_beyond_the_largest_number(dtype, top, small, group, T):
     w, W, group = build(*weight(V, D, group, True, dtype, 11, s))
     h = (hidden(T, D, torch.float32, T) * small).to(dtype).cuda()
     check(w4_logits(h, w), h, W, group)
+
+
+@pytest.mark.parametrize("T", [3, 9, 40, 140])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_infinite_hidden_states(group, dtype, T):
+    """An infinite hidden state makes infinite logits of the weight's sign, and NaN
+    where its weight is zero; other rows are as they were."""
+    V, D = 300, 256
+    g = torch.Generator().manual_seed(5)
+    s = 0.002 + 0.02 * torch.rand(V, D // group, generator=g)
+    w, W, group = build(*weight(V, D, group, True, dtype, 13, s))
+    h = hidden(T, D, dtype, T).cuda()
+    h[1, 77], h[2, 200] = float("inf"), float("-inf")
+    got = w4_logits(h, w)
+    for r, k in ((1, 77), (2, 200)):
+        want = W[:, k] * h[r, k].double()
+        assert want.isnan().any() and want.isinf().any()
+        assert torch.equal(got[r].isnan(), want.isnan())
+        assert torch.equal(got[r][~want.isnan()].double(), want[~want.isnan()])
+    keep = [r for r in range(T) if r not in (1, 2)]
+    check(got[keep], h[keep], W, group, rows=T)
